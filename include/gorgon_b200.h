@@ -72,7 +72,8 @@ GORGON_API const char* gorgon_last_error(void);
  * outside the cache, bit 2 = a verifier tree/draft entry out of range, bit 3 =
  * a sequence shorter than its tree, bit 4 = a bounded wait inside a
  * tensor-core kernel ran out (the kernel stopped early and its outputs are
- * incomplete), bit 5 = a candidate tree was cut at max_nodes.  The offending
+ * incomplete), bit 5 = a candidate tree was cut at max_nodes, bit 6 = a page
+ * number outside the pool, or a length past the block table.  The offending
  * element is skipped, never dereferenced.  clear != 0 resets it. */
 GORGON_API int gorgon_device_error(uint32_t* out_flags, int clear);
 
@@ -393,6 +394,144 @@ typedef struct {
 GORGON_API size_t gorgon_head_candidate_tree_workspace_size(const gorgon_head_candidate_params* p);
 GORGON_API int gorgon_head_candidate_tree(const gorgon_head_candidate_params* p, void* workspace,
                                           size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Key/value cache in pages.  No counterpart in the reference, whose cache is
+ * one contiguous tensor per layer (src/gorgon/inference/kv_cache.py:21-86):
+ * these are its append, read and trim for a cache that a server keeps in
+ * pages, and tree_attention / chunked causal attention over it.
+ *
+ * Pages are [num_pages, heads_kv, page_size, head_dim] for K and for V
+ * (element strides, head_dim contiguous).  Position p of sequence b lies in
+ * page block_table[b, p / page_size], row p % page_size; the entries of the
+ * pages that a call does not need are not read, so they may hold anything.
+ * seq_lens[b] counts a sequence's rows with the call's new rows, which are its
+ * last.  seq_lens[b] == 0 marks an unused slot of a padded batch.
+ *
+ * storage: NATIVE pages hold `dtype`; INT8 and E4M3 pages hold a byte per
+ * value, which stands for byte * scale with an fp32 scale per (page, kv head,
+ * row).  inv = largest / amax cut to 12 significant bits (largest 127 / 448;
+ * amax the row's largest magnitude, at least 2^-100), stored =
+ * round-to-nearest-even(x * inv), scale = 1 / inv.  A row that holds an
+ * infinity or a NaN is stored with scale NaN and reads back as NaN.
+ *
+ * A block-table entry outside [0, num_pages), or a length past the table's
+ * columns, sets bit 6 of the device error word; the row is skipped, never
+ * dereferenced.  seq_lens[b] below the sequence's new rows sets bit 3, and
+ * the sequence is treated as an unused slot.
+ * ---------------------------------------------------------------------- */
+typedef enum {
+  GORGON_KV_NATIVE = 0,
+  GORGON_KV_INT8 = 1,
+  GORGON_KV_E4M3 = 2
+} gorgon_kv_storage;
+
+typedef struct {
+  int32_t dtype;    /* gorgon_dtype of NATIVE pages and of the rows written, read or attended with */
+  int32_t storage;  /* gorgon_kv_storage */
+  int64_t num_pages, page_size, heads_kv, head_dim;  /* head_dim <= 256 */
+  void* k_pages;  int64_t k_stride_p, k_stride_h, k_stride_s;
+  void* v_pages;  int64_t v_stride_p, v_stride_h, v_stride_s;
+  float* k_scale; int64_t ks_stride_p, ks_stride_h, ks_stride_s;  /* 8-bit storage only */
+  float* v_scale; int64_t vs_stride_p, vs_stride_h, vs_stride_s;
+  const int32_t* block_table; int64_t table_stride_b, table_cols;  /* int32 [batch, table_cols] */
+  const int32_t* seq_lens;                                        /* int32 [batch] */
+  int64_t batch;
+} gorgon_paged_kv;
+
+/* Writes new rows behind each sequence: k, v [batch, heads_kv, n, head_dim]
+ * by strides, or with cu_q (int32 [batch + 1]) packed rows: sequence b's are
+ * cu_q[b] .. cu_q[b + 1] - 1 of `rows` packed rows (the batch stride is
+ * ignored).  Row i of a sequence with c new rows goes to position
+ * seq_lens[b] - c + i.  Two sequences must not write the same row of a page:
+ * its contents are then undefined (nothing faults). */
+typedef struct {
+  gorgon_paged_kv kv;
+  const void* k; int64_t k_stride_b, k_stride_h, k_stride_n;
+  const void* v; int64_t v_stride_b, v_stride_h, v_stride_n;
+  int64_t n;            /* rows per sequence (without cu_q) */
+  int64_t rows;         /* packed rows (with cu_q) */
+  const int32_t* cu_q;  /* nullable */
+} gorgon_paged_append_params;
+
+GORGON_API int gorgon_paged_append(const gorgon_paged_append_params* p, void* stream);
+
+/* Reads rows back: row cu_rows[b] + i of k and v [rows, heads_kv, head_dim]
+ * (strides, head_dim contiguous, dtype out_dtype) is position starts[b] + i
+ * of sequence b (starts NULL: 0), for i < cu_rows[b + 1] - cu_rows[b]; rows
+ * from cu_rows[batch] on are left as they are.  8-bit values stop at
+ * out_dtype's largest finite value.  kv.seq_lens is not used. */
+typedef struct {
+  gorgon_paged_kv kv;
+  int32_t out_dtype;
+  void* k; int64_t k_stride_n, k_stride_h;
+  void* v; int64_t v_stride_n, v_stride_h;
+  int64_t rows;
+  const int32_t* cu_rows;  /* int32 [batch + 1] */
+  const int32_t* starts;   /* nullable, int32 [batch] */
+} gorgon_paged_read_params;
+
+GORGON_API int gorgon_paged_read(const gorgon_paged_read_params* p, void* stream);
+
+/* gorgon_kv_trim for pages, all layers in one launch: row dst_start[b] + r of
+ * sequence b takes row src_idx[b, r] for r < lens[b], bytes and scales as
+ * stored, in every layer and head; all rows of a (layer, sequence, head) are
+ * read before any is written.  A layer's pages lie k_stride_l / v_stride_l
+ * elements (scales ks_stride_l / vs_stride_l) after the one before; all
+ * layers share the block table.  max_len <= 256; kv.seq_lens is not used.
+ * A bad index sets bit 1 of the device error word and leaves the sequence as
+ * it is, as in gorgon_kv_trim; so does a page outside the pool, with bit 6. */
+typedef struct {
+  gorgon_paged_kv kv;
+  int64_t layers, k_stride_l, v_stride_l, ks_stride_l, vs_stride_l;
+  const int32_t* src_idx; int64_t idx_stride_b, max_len;
+  const int32_t* lens;
+  const int32_t* dst_start;  /* nullable */
+} gorgon_paged_trim_params;
+
+GORGON_API int gorgon_paged_trim(const gorgon_paged_trim_params* p, void* stream);
+
+/* Attention of each sequence's new rows over its pages (the new rows' K and V
+ * are already there: gorgon_paged_append first).
+ *   q, out [batch, heads_q, n, head_dim] by strides, or with cu_q packed rows
+ *   (sequence b's are cu_q[b] .. cu_q[b + 1] - 1; the batch stride is
+ *   ignored; n is then the largest count of new rows).
+ * Row i of a sequence with c new rows, P = seq_lens[b] - c, sees position j
+ *   without parents: iff j <= P + i;
+ *   with parents (int32 [batch, n], stride 0 shared, every sequence brings n
+ *   rows): iff j < P, or j - P is i or one of its ancestors within max_depth
+ *   hops (max_depth < 0: all); its position is P + depth(i), depth counting
+ *   the hops to its root;
+ * and with window > 0 only if j's position is less than `window` positions
+ * before the row's own (a tree row's position as above), or j < sinks.
+ * Hidden rows contribute nothing, whatever they hold.
+ * out = softmax(q k^T * scale) v over the visible rows (scale 0: 1 /
+ * sqrt(head_dim)); lse (nullable, float, strides) the natural-log sum of
+ * exponentials.  Rows of an unused slot are 0 with lse -inf; packed rows
+ * from cu_q[batch] on are left as they are. */
+typedef struct {
+  gorgon_paged_kv kv;
+  int64_t heads_q, n;
+  const void* q;  int64_t q_stride_b, q_stride_h, q_stride_n;
+  void* out;      int64_t o_stride_b, o_stride_h, o_stride_n;
+  float* lse;     int64_t lse_stride_b, lse_stride_h, lse_stride_n;
+  const int32_t* cu_q;     /* nullable */
+  const int32_t* parents;  /* nullable */
+  int64_t parents_stride_b;
+  int32_t max_depth;
+  int64_t window, sinks;
+  float scale;
+  int32_t backend;         /* gorgon_paged_backend */
+} gorgon_paged_attn_params;
+
+typedef enum {
+  GORGON_PAGED_AUTO = 0,
+  GORGON_PAGED_SIMT = 1  /* CUDA cores: any dtype, head_dim and alignment */
+} gorgon_paged_backend;
+
+GORGON_API size_t gorgon_paged_attn_workspace_size(const gorgon_paged_attn_params* p);
+GORGON_API int gorgon_paged_attn(const gorgon_paged_attn_params* p, void* workspace, size_t workspace_bytes,
+                                 void* stream);
 
 #ifdef __cplusplus
 }

@@ -30,6 +30,10 @@ ERR_BAD_VERIFY_INPUT = 1 << 2
 ERR_BAD_SEQLEN = 1 << 3
 ERR_TIMEOUT = 1 << 4
 ERR_CAND_CAPACITY = 1 << 5
+ERR_BAD_PAGE = 1 << 6
+
+KV_NATIVE, KV_INT8, KV_E4M3 = 0, 1, 2
+PAGED_AUTO, PAGED_SIMT = 0, 1
 
 
 class TreeAttnParams(Structure):
@@ -106,6 +110,65 @@ class HeadCandidateParams(Structure):
     ]
 
 
+class PagedKV(Structure):
+    _fields_ = [
+        ("dtype", c_int32), ("storage", c_int32),
+        ("num_pages", c_int64), ("page_size", c_int64), ("heads_kv", c_int64), ("head_dim", c_int64),
+        ("k_pages", c_void_p), ("k_stride_p", c_int64), ("k_stride_h", c_int64), ("k_stride_s", c_int64),
+        ("v_pages", c_void_p), ("v_stride_p", c_int64), ("v_stride_h", c_int64), ("v_stride_s", c_int64),
+        ("k_scale", c_void_p), ("ks_stride_p", c_int64), ("ks_stride_h", c_int64), ("ks_stride_s", c_int64),
+        ("v_scale", c_void_p), ("vs_stride_p", c_int64), ("vs_stride_h", c_int64), ("vs_stride_s", c_int64),
+        ("block_table", c_void_p), ("table_stride_b", c_int64), ("table_cols", c_int64),
+        ("seq_lens", c_void_p),
+        ("batch", c_int64),
+    ]
+
+
+class PagedAppendParams(Structure):
+    _fields_ = [
+        ("kv", PagedKV),
+        ("k", c_void_p), ("k_stride_b", c_int64), ("k_stride_h", c_int64), ("k_stride_n", c_int64),
+        ("v", c_void_p), ("v_stride_b", c_int64), ("v_stride_h", c_int64), ("v_stride_n", c_int64),
+        ("n", c_int64), ("rows", c_int64), ("cu_q", c_void_p),
+    ]
+
+
+class PagedReadParams(Structure):
+    _fields_ = [
+        ("kv", PagedKV),
+        ("out_dtype", c_int32),
+        ("k", c_void_p), ("k_stride_n", c_int64), ("k_stride_h", c_int64),
+        ("v", c_void_p), ("v_stride_n", c_int64), ("v_stride_h", c_int64),
+        ("rows", c_int64), ("cu_rows", c_void_p), ("starts", c_void_p),
+    ]
+
+
+class PagedTrimParams(Structure):
+    _fields_ = [
+        ("kv", PagedKV),
+        ("layers", c_int64), ("k_stride_l", c_int64), ("v_stride_l", c_int64),
+        ("ks_stride_l", c_int64), ("vs_stride_l", c_int64),
+        ("src_idx", c_void_p), ("idx_stride_b", c_int64), ("max_len", c_int64),
+        ("lens", c_void_p), ("dst_start", c_void_p),
+    ]
+
+
+class PagedAttnParams(Structure):
+    _fields_ = [
+        ("kv", PagedKV),
+        ("heads_q", c_int64), ("n", c_int64),
+        ("q", c_void_p), ("q_stride_b", c_int64), ("q_stride_h", c_int64), ("q_stride_n", c_int64),
+        ("out", c_void_p), ("o_stride_b", c_int64), ("o_stride_h", c_int64), ("o_stride_n", c_int64),
+        ("lse", c_void_p), ("lse_stride_b", c_int64), ("lse_stride_h", c_int64), ("lse_stride_n", c_int64),
+        ("cu_q", c_void_p),
+        ("parents", c_void_p), ("parents_stride_b", c_int64),
+        ("max_depth", c_int32),
+        ("window", c_int64), ("sinks", c_int64),
+        ("scale", c_float),
+        ("backend", c_int32),
+    ]
+
+
 MAX_PEERS = 8  # GORGON_MAX_PEERS
 
 
@@ -143,6 +206,12 @@ SIGNATURES = {
     "gorgon_candidate_tree": (c_int, [POINTER(CandidateTreeParams), c_void_p, c_size_t, c_void_p]),
     "gorgon_head_candidate_tree_workspace_size": (c_size_t, [POINTER(HeadCandidateParams)]),
     "gorgon_head_candidate_tree": (c_int, [POINTER(HeadCandidateParams), c_void_p, c_size_t, c_void_p]),
+    # the paged operators take their parameters as packed bytes (_paged.py) or byref(structure)
+    "gorgon_paged_append": (c_int, [c_void_p, c_void_p]),
+    "gorgon_paged_read": (c_int, [c_void_p, c_void_p]),
+    "gorgon_paged_trim": (c_int, [c_void_p, c_void_p]),
+    "gorgon_paged_attn_workspace_size": (c_size_t, [c_void_p]),
+    "gorgon_paged_attn": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,74 @@
+// gorgon_paged_attn: argument checking and kernel choice.
+#include <algorithm>
+#include <string>
+
+#include "paged_attn.cuh"
+
+namespace gorgon {
+namespace {
+
+int make_args(const gorgon_paged_attn_params* p, PagedAttn* a) {
+  if (!p) return set_error(GORGON_ERR_INVALID, "gorgon_paged_attn: params is null");
+  PagedAttn& x = *a;
+  x = PagedAttn{};
+  int rc = make_pool(&p->kv, "gorgon_paged_attn", &x.pool);
+  if (rc) return rc;
+  if (p->heads_q < 0 || p->n < 0 || p->window < 0 || p->sinks < 0)
+    return set_error(GORGON_ERR_INVALID, "gorgon_paged_attn: negative size");
+  if (p->heads_q % p->kv.heads_kv != 0)
+    return set_error(GORGON_ERR_INVALID, "gorgon_paged_attn: heads_q must be a multiple of heads_kv");
+  if (p->heads_q > 65535 || p->n > (int64_t(1) << 24) || p->n * (p->heads_q / p->kv.heads_kv) > (int64_t(1) << 28))
+    return set_error(GORGON_ERR_UNSUPPORTED, "gorgon_paged_attn: too many query rows");
+  if (p->parents && p->n > kPagedMaxNodes)
+    return set_error(GORGON_ERR_UNSUPPORTED, "gorgon_paged_attn: trees above 1024 nodes");
+  if (p->parents && p->cu_q)
+    return set_error(GORGON_ERR_UNSUPPORTED, "gorgon_paged_attn: a tree needs n rows in every sequence (no cu_q)");
+  if (p->backend < GORGON_PAGED_AUTO || p->backend > GORGON_PAGED_SIMT)
+    return set_error(GORGON_ERR_INVALID, "gorgon_paged_attn: unknown backend");
+  if (p->kv.batch * p->heads_q * p->n * p->kv.head_dim > 0 && (!p->q || !p->out || !p->kv.seq_lens))
+    return set_error(GORGON_ERR_INVALID, "gorgon_paged_attn: null q, out or seq_lens");
+  const int64_t es = static_cast<int64_t>(dtype_bytes(p->kv.dtype));
+  x.nr = NewRows{p->cu_q, static_cast<int>(p->n)};
+  x.q = static_cast<const char*>(p->q);
+  x.q_sb = p->q_stride_b * es; x.q_sh = p->q_stride_h * es; x.q_sn = p->q_stride_n * es;
+  x.out = static_cast<char*>(p->out);
+  x.o_sb = p->o_stride_b; x.o_sh = p->o_stride_h; x.o_sn = p->o_stride_n;
+  x.lse = p->lse;
+  x.l_sb = p->lse_stride_b; x.l_sh = p->lse_stride_h; x.l_sn = p->lse_stride_n;
+  x.parents = p->parents;
+  x.par_sb = p->parents_stride_b;
+  x.max_depth = p->max_depth < 0 ? INT32_MAX : p->max_depth;
+  x.window = static_cast<int>(std::min<int64_t>(p->window, int64_t(1) << 30));
+  x.sinks = static_cast<int>(std::min<int64_t>(p->sinks, int64_t(1) << 30));
+  x.hq = static_cast<int>(p->heads_q);
+  x.group = x.hq / x.pool.hkv;
+  x.n = static_cast<int>(p->n);
+  const float scale = p->scale != 0.f ? p->scale : (x.pool.d > 0 ? 1.f / std::sqrt(static_cast<float>(x.pool.d)) : 1.f);
+  x.scale_log2 = scale * 1.4426950408889634f;
+  x.wait_ns = wait_limit_ns();
+  return GORGON_OK;
+}
+
+bool empty(const PagedAttn& a) { return static_cast<int64_t>(a.pool.batch) * a.hq * a.n * a.pool.d == 0; }
+
+}  // namespace
+}  // namespace gorgon
+
+extern "C" size_t gorgon_paged_attn_workspace_size(const gorgon_paged_attn_params* p) {
+  using namespace gorgon;
+  PagedAttn a;
+  if (make_args(p, &a) != GORGON_OK) return 0;
+  return 0;
+}
+
+extern "C" int gorgon_paged_attn(const gorgon_paged_attn_params* p, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
+  using namespace gorgon;
+  PagedAttn a;
+  int rc = make_args(p, &a);
+  if (rc) return rc;
+  if (empty(a)) return GORGON_OK;
+  (void)workspace;
+  (void)workspace_bytes;
+  return launch_paged_simt(a, static_cast<cudaStream_t>(stream));
+}

@@ -1,0 +1,142 @@
+// Paged attention on the CUDA cores: any dtype, head_dim up to 256, any
+// alignment.  The tensor-core kernels take 16-bit rows of whole 16-byte pieces;
+// this one takes the rest, and is the plainest statement of the operator.
+//
+// A CTA per (new row, query head): its warps take every eighth visible key,
+// a lane the values lane, lane + 32, ... of a row; each warp keeps a running
+// max, sum and output row in fp32, joined through shared memory at the end.
+// Bound by the latency of one key at a time per warp.
+#include <cuda_fp8.h>
+
+#include "paged_attn.cuh"
+
+namespace gorgon {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kMaxD = 256;
+
+template <typename T, int ST>
+__device__ __forceinline__ float page_value(const char* row, int d) {
+  if constexpr (ST == GORGON_KV_NATIVE) return Cvt<T>::to_f(reinterpret_cast<const T*>(row)[d]);
+  if constexpr (ST == GORGON_KV_INT8) return static_cast<float>(reinterpret_cast<const int8_t*>(row)[d]);
+  __nv_fp8_e4m3 f;
+  f.__x = reinterpret_cast<const uint8_t*>(row)[d];
+  return static_cast<float>(f);
+}
+
+template <typename T, int ST>
+__global__ void __launch_bounds__(kWarps * 32) paged_simt_kernel(const PagedAttn a) {
+  __shared__ uint32_t s_bits[kPagedMaxNodes / 32];
+  __shared__ int s_depth;
+  __shared__ float s_m[kWarps], s_l[kWarps];
+  __shared__ float s_o[kWarps][kMaxD];
+  const int t = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Seq s = sequence(a, b, threadIdx.x == 0 && t == 0 && h == 0);
+  if (t >= s.c || t >= a.n) return;
+  const int64_t row = a.nr.cu ? a.nr.first(b) + t : t;
+  T* out = reinterpret_cast<T*>(a.out) + (a.nr.cu ? 0 : b * a.o_sb) + h * a.o_sh + row * a.o_sn;
+  float* lse = a.lse ? a.lse + (a.nr.cu ? 0 : b * a.l_sb) + h * a.l_sh + row * a.l_sn : nullptr;
+  const int D = a.pool.d;
+  if (!s.ok) {
+    for (int d = threadIdx.x; d < D; d += blockDim.x) out[d] = Cvt<T>::from_f(0.f);
+    if (lse && threadIdx.x == 0) *lse = -INFINITY;
+    return;
+  }
+  int pos = s.P + t;
+  if (a.parents) {
+    for (int k = threadIdx.x; k < (s.c + 31) / 32; k += blockDim.x) s_bits[k] = 0;
+    __syncthreads();
+    if (threadIdx.x == 0) s_depth = tree_bits(a, s, b, t, s_bits);
+    __syncthreads();
+    pos = s.P + s_depth;
+  }
+  const int lo = a.window ? max(0, pos - a.window + 1) : 0;
+  const int s_end = min(a.sinks, lo);
+  const int hi = a.parents ? s.L : pos + 1;
+  const int kvh = h / a.group;
+  const T* q = reinterpret_cast<const T*>(a.q + (a.nr.cu ? 0 : b * a.q_sb) + h * a.q_sh + row * a.q_sn);
+  float qv[kMaxD / 32], o[kMaxD / 32];
+#pragma unroll
+  for (int k = 0; k < kMaxD / 32; ++k) {
+    const int d = lane + 32 * k;
+    qv[k] = d < D ? Cvt<T>::to_f(q[d]) * a.scale_log2 : 0.f;
+    o[k] = 0.f;
+  }
+  float m = -INFINITY, l = 0.f;
+  const int keys = s_end + max(0, hi - lo);  // sinks, then the window
+  for (int i = warp; i < keys; i += kWarps) {
+    const int j = i < s_end ? i : lo + (i - s_end);
+    if (a.parents && j >= s.P && !((s_bits[(j - s.P) >> 5] >> ((j - s.P) & 31)) & 1u)) continue;
+    int col, r;
+    a.pool.split(j, col, r);
+    const int page = a.pool.page(b, col);
+    if (page < 0) continue;
+    const char* kr = a.pool.k + page * a.pool.k_sp + kvh * a.pool.k_sh + r * a.pool.k_ss;
+    const char* vr = a.pool.v + page * a.pool.v_sp + kvh * a.pool.v_sh + r * a.pool.v_ss;
+    float x = 0.f;
+#pragma unroll
+    for (int k = 0; k < kMaxD / 32; ++k) {
+      const int d = lane + 32 * k;
+      if (d < D) x = fmaf(qv[k], page_value<T, ST>(kr, d), x);
+    }
+    x = warp_sum(x);
+    float vsc = 1.f;
+    if constexpr (ST != GORGON_KV_NATIVE) {
+      x *= a.pool.ks[page * a.pool.ks_sp + kvh * a.pool.ks_sh + r * a.pool.ks_ss];
+      vsc = a.pool.vs[page * a.pool.vs_sp + kvh * a.pool.vs_sh + r * a.pool.vs_ss];
+    }
+    const float mn = fmaxf(m, x);
+    const float base = mn == -INFINITY ? 0.f : mn;
+    const float f = exp2f(m - base), p = exp2f(x - base);
+    m = mn;
+    l = l * f + p;
+#pragma unroll
+    for (int k = 0; k < kMaxD / 32; ++k) {
+      const int d = lane + 32 * k;
+      if (d < D) o[k] = fmaf(p * vsc, page_value<T, ST>(vr, d), o[k] * f);
+    }
+  }
+  if (lane == 0) {
+    s_m[warp] = m;
+    s_l[warp] = l;
+  }
+#pragma unroll
+  for (int k = 0; k < kMaxD / 32; ++k)
+    if (lane + 32 * k < D) s_o[warp][lane + 32 * k] = o[k];
+  __syncthreads();
+  float M = -INFINITY, L = 0.f;
+  for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w]);
+  const float base = M == -INFINITY ? 0.f : M;
+  for (int w = 0; w < kWarps; ++w) L += s_l[w] * exp2f(s_m[w] - base);
+  for (int d = threadIdx.x; d < D; d += blockDim.x) {
+    float x = 0.f;
+    for (int w = 0; w < kWarps; ++w) x = fmaf(s_o[w][d], exp2f(s_m[w] - base), x);
+    out[d] = Cvt<T>::from_f(x / L);
+  }
+  if (lse && threadIdx.x == 0) *lse = (M + log2f(L)) * 0.6931471805599453f;
+}
+
+template <typename T>
+int launch_t(const PagedAttn& a, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>(a.n), static_cast<unsigned>(a.hq), static_cast<unsigned>(a.pool.batch));
+  switch (a.pool.storage) {
+    case GORGON_KV_NATIVE: paged_simt_kernel<T, GORGON_KV_NATIVE><<<grid, kWarps * 32, 0, st>>>(a); break;
+    case GORGON_KV_INT8: paged_simt_kernel<T, GORGON_KV_INT8><<<grid, kWarps * 32, 0, st>>>(a); break;
+    default: paged_simt_kernel<T, GORGON_KV_E4M3><<<grid, kWarps * 32, 0, st>>>(a); break;
+  }
+  return check_cuda(cudaGetLastError(), "gorgon_paged_attn launch");
+}
+
+}  // namespace
+
+int launch_paged_simt(const PagedAttn& a, cudaStream_t st) {
+  switch (a.pool.dtype) {
+    case GORGON_F32: return launch_t<float>(a, st);
+    case GORGON_BF16: return launch_t<__nv_bfloat16>(a, st);
+    default: return launch_t<__half>(a, st);
+  }
+}
+
+}  // namespace gorgon
