@@ -512,6 +512,7 @@ GORGON_API int gorgon_paged_trim(const gorgon_paged_trim_params* p, void* stream
 typedef struct {
   gorgon_paged_kv kv;
   int64_t heads_q, n;
+  int64_t rows;            /* packed rows of q and out (with cu_q) */
   const void* q;  int64_t q_stride_b, q_stride_h, q_stride_n;
   void* out;      int64_t o_stride_b, o_stride_h, o_stride_n;
   float* lse;     int64_t lse_stride_b, lse_stride_h, lse_stride_n;
@@ -526,7 +527,9 @@ typedef struct {
 
 typedef enum {
   GORGON_PAGED_AUTO = 0,
-  GORGON_PAGED_SIMT = 1  /* CUDA cores: any dtype, head_dim and alignment */
+  GORGON_PAGED_SIMT = 1, /* CUDA cores: any dtype, head_dim and alignment */
+  GORGON_PAGED_MMA = 2   /* tensor cores, warp by warp, for few new rows: 16-bit dtype, head_dim
+                            64 or 128, rows of whole 16-byte pieces */
 } gorgon_paged_backend;
 
 GORGON_API size_t gorgon_paged_attn_workspace_size(const gorgon_paged_attn_params* p);

@@ -33,7 +33,7 @@ ERR_CAND_CAPACITY = 1 << 5
 ERR_BAD_PAGE = 1 << 6
 
 KV_NATIVE, KV_INT8, KV_E4M3 = 0, 1, 2
-PAGED_AUTO, PAGED_SIMT = 0, 1
+PAGED_AUTO, PAGED_SIMT, PAGED_MMA = 0, 1, 2
 
 
 class TreeAttnParams(Structure):
@@ -156,7 +156,7 @@ class PagedTrimParams(Structure):
 class PagedAttnParams(Structure):
     _fields_ = [
         ("kv", PagedKV),
-        ("heads_q", c_int64), ("n", c_int64),
+        ("heads_q", c_int64), ("n", c_int64), ("rows", c_int64),
         ("q", c_void_p), ("q_stride_b", c_int64), ("q_stride_h", c_int64), ("q_stride_n", c_int64),
         ("out", c_void_p), ("o_stride_b", c_int64), ("o_stride_h", c_int64), ("o_stride_n", c_int64),
         ("lse", c_void_p), ("lse_stride_b", c_int64), ("lse_stride_h", c_int64), ("lse_stride_n", c_int64),

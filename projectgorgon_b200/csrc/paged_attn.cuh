@@ -12,8 +12,9 @@
 // batches, long single sequences and windows balance by themselves, without
 // the host knowing any length.  A unit inside one CTA's range is finished
 // there; one cut between CTAs leaves unnormalised fp32 rows with their running
-// max and sum in the workspace, and paged_merge_kernel joins them in a fixed
-// order, so results do not depend on timing.
+// max and sum in the workspace (slot 0: the piece that a CTA starts with, slot
+// 1: the one that it ends with), and paged_merge_kernel joins them in the
+// order of the CTAs, so results do not depend on timing.
 #pragma once
 
 #include "paged.cuh"
@@ -36,6 +37,7 @@ struct PagedAttn {
   int max_depth;
   int window, sinks;  // window 0: none
   int hq, group, n;   // n: largest count of new rows
+  int rows;           // packed rows of q and out (with nr.cu)
   float scale_log2;   // softmax scale * log2(e)
   // tensor-core schedule
   int m, bn;          // packed rows per unit, positions per tile
@@ -43,8 +45,16 @@ struct PagedAttn {
   int grid;
   float* part_o;      // [grid * 2][m][d]
   float2* part_ml;    // [grid * 2][m]  running max (log2 units) and sum
-  int* tile_start;    // [batch + 1]
+  struct CutUnit* cut;  // [grid]
   uint64_t wait_ns;
+};
+
+// What CTA c leaves for the merge: the unit that its range starts inside of.
+// pieces == 0: none, or an earlier CTA's entry names the unit.
+struct CutUnit {
+  int b, kvh, qb;
+  int pieces;      // CTAs c - 1, c, ..., c - 2 + pieces
+  int first_slot;  // slot of CTA c - 1's piece (the others are in slot 0)
 };
 
 // A sequence's state: P cached rows before its c new ones.
@@ -53,24 +63,23 @@ struct Seq {
   bool ok;  // has rows to compute
 };
 
+// The sequence's rows lie inside q and out.
+__device__ __forceinline__ bool rows_inside(const PagedAttn& a, int b, int c) {
+  return !a.nr.cu || (a.nr.cu[b] >= 0 && c >= 0 && a.nr.cu[b] <= a.rows - c);
+}
+
 __device__ __forceinline__ Seq sequence(const PagedAttn& a, int b, bool report) {
   Seq s;
   s.L = a.pool.lens[b];
   s.c = a.nr.count(b);
   s.P = s.L - s.c;
-  const bool bad_len = s.L != 0 && (s.c > s.L || s.c > a.n || s.c < 0);
+  const bool bad_len = s.L != 0 && (s.c > s.L || s.c > a.n || s.c < 0 || !rows_inside(a, b, s.c));
   const bool bad_table = static_cast<int64_t>(s.L) > static_cast<int64_t>(a.pool.table_cols) * a.pool.page_size;
   if (report && bad_len) raise_device_error(a.pool.err, kErrBadSeqlen);
   if (report && bad_table) raise_device_error(a.pool.err, kErrBadPage);
   s.ok = s.L > 0 && s.c > 0 && !bad_len && !bad_table;
   return s;
 }
-
-// What a row sees: position j <= hi, and (window) j >= lo or j < sinks; a tree
-// row's hi is P - 1, and its own tree's rows go by its ancestor bits.
-struct RowView {
-  int hi, lo;
-};
 
 // Keys of a unit of rows [t0, t1): its union is [0, s_end) and [lo, hi).
 struct UnitKeys {
@@ -102,11 +111,142 @@ __device__ __forceinline__ bool block_rows(const PagedAttn& a, const Seq& s, int
 }
 
 // Tiles of every row block of one (sequence, kv head).
-__device__ __forceinline__ int head_tiles(const PagedAttn& a, const Seq& s) {
-  int n = 0, t0, t1;
+__device__ __forceinline__ int64_t head_tiles(const PagedAttn& a, const Seq& s) {
+  int64_t n = 0;
+  int t0, t1;
   if (!s.ok) return 0;
   for (int qb = 0; block_rows(a, s, qb, t0, t1); ++qb) n += unit_keys(a, s, t0, t1).tiles;
   return n;
+}
+
+// A position in the list of tiles.
+struct TileCursor {
+  int b, kvh, qb;
+  int i;       // tile within the unit
+  int t0, t1;  // the unit's new rows
+  Seq s;
+  UnitKeys u;
+  __device__ __forceinline__ int tile() const { return u.tile(i); }
+  // To the next tile; the caller knows that there is one.
+  __device__ __forceinline__ void next(const PagedAttn& a) {
+    if (++i < u.tiles) return;
+    i = 0;
+    ++qb;
+    if (!block_rows(a, s, qb, t0, t1)) {
+      qb = 0;
+      if (++kvh == a.pool.hkv) {
+        kvh = 0;
+        do s = sequence(a, ++b, false);
+        while (!s.ok && b < a.pool.batch - 1);
+      }
+      block_rows(a, s, qb, t0, t1);
+    }
+    u = unit_keys(a, s, t0, t1);
+  }
+};
+
+// The CTA's share [g0, g1) of the T tiles (G CTAs have one: no more than there
+// are tiles), and the cursor at g0 (called by all THREADS threads of the CTA;
+// `sh` is shared scratch).  Thread t counts the
+// tiles of sequences [t * per, (t + 1) * per), a block scan places them, and
+// the thread that owns g0 names its sequence.
+struct ShareScratch {
+  int64_t warp_sum[32];
+  int64_t rem;
+  int b;
+};
+struct Share {
+  int64_t g0, g1, T, G;
+};
+template <int THREADS>
+__device__ __forceinline__ bool cta_share(const PagedAttn& a, ShareScratch* sh, Share& r, TileCursor& cur) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (a.pool.batch + THREADS - 1) / THREADS;
+  const int b0 = min(tid * per, a.pool.batch), b1 = min(b0 + per, a.pool.batch);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += head_tiles(a, sequence(a, b, blockIdx.x == 0)) * a.pool.hkv;
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += up;
+  }
+  if (lane == 31) sh->warp_sum[warp] = incl;
+  __syncthreads();
+  int64_t before = 0, T = 0;
+  for (int w = 0; w < THREADS / 32; ++w) {
+    const int64_t x = sh->warp_sum[w];
+    if (w < warp) before += x;
+    T += x;
+  }
+  r.T = T;
+  r.G = min(static_cast<int64_t>(a.grid), T);
+  const bool work = static_cast<int64_t>(blockIdx.x) < r.G;
+  r.g0 = work ? static_cast<int64_t>(blockIdx.x) * T / r.G : T;
+  r.g1 = work ? static_cast<int64_t>(blockIdx.x + 1) * T / r.G : T;
+  const int64_t g0 = r.g0;
+  const int64_t start = before + incl - mine;
+  if (work && g0 >= start && g0 < start + mine) {
+    int64_t rem = g0 - start;
+    int b = b0;
+    for (; b < b1 - 1; ++b) {
+      const int64_t n = head_tiles(a, sequence(a, b, false)) * a.pool.hkv;
+      if (rem < n) break;
+      rem -= n;
+    }
+    sh->b = b;
+    sh->rem = rem;
+  }
+  __syncthreads();
+  if (!work) return false;
+  cur.b = sh->b;
+  cur.s = sequence(a, cur.b, false);
+  const int64_t per_head = head_tiles(a, cur.s);
+  cur.kvh = static_cast<int>(sh->rem / per_head);
+  int64_t rem = sh->rem - cur.kvh * per_head;
+  for (cur.qb = 0;; ++cur.qb) {
+    block_rows(a, cur.s, cur.qb, cur.t0, cur.t1);
+    cur.u = unit_keys(a, cur.s, cur.t0, cur.t1);
+    if (rem < cur.u.tiles) break;
+    rem -= cur.u.tiles;
+  }
+  cur.i = static_cast<int>(rem);
+  return true;
+}
+
+// CTA c's note for the merge; `cur` is at the CTA's first tile.
+__device__ __forceinline__ void note_cut(const PagedAttn& a, bool work, const TileCursor& cur, const Share& r) {
+  CutUnit n{};
+  if (work && cur.i > 0) {
+    const int c = blockIdx.x;
+    const int64_t start = r.g0 - cur.i, end = start + cur.u.tiles;  // the unit's tiles
+    const int64_t prev = static_cast<int64_t>(c - 1) * r.T / r.G;
+    if (start >= prev) {  // the unit starts in CTA c - 1's range (else an earlier CTA names it)
+      const int last = static_cast<int>((end * r.G - 1) / r.T);  // the CTA of tile end - 1
+      n = CutUnit{cur.b, cur.kvh, cur.qb, last - c + 2, start == prev ? 0 : 1};
+    }
+  }
+  a.cut[blockIdx.x] = n;
+}
+
+// Rows of sequences that have nothing to compute: zeros, log-sum-exp -inf.
+template <typename T, int THREADS>
+__device__ __forceinline__ void clear_unused(const PagedAttn& a) {
+  for (int b = blockIdx.x; b < a.pool.batch; b += gridDim.x) {
+    if (sequence(a, b, false).ok) continue;
+    const int c = a.nr.count(b);
+    if (c <= 0 || !rows_inside(a, b, c)) continue;
+    const int64_t first = a.nr.cu ? a.nr.cu[b] : 0;
+    T* out = reinterpret_cast<T*>(a.out) + (a.nr.cu ? 0 : b * a.o_sb);
+    const int64_t values = static_cast<int64_t>(c) * a.hq * a.pool.d;
+    for (int64_t e = threadIdx.x; e < values; e += THREADS) {
+      const int d = static_cast<int>(e % a.pool.d);
+      const int64_t rh = e / a.pool.d;
+      const int64_t r = first + rh / a.hq, h = rh % a.hq;
+      out[r * a.o_sn + h * a.o_sh + d] = Cvt<T>::from_f(0.f);
+      if (a.lse && d == 0) a.lse[(a.nr.cu ? 0 : b * a.l_sb) + r * a.l_sn + h * a.l_sh] = -INFINITY;
+    }
+  }
 }
 
 // Ancestor bits of tree row i (bit j: new row j is visible to it) and its
@@ -130,5 +270,10 @@ __device__ __forceinline__ int tree_bits(const PagedAttn& a, const Seq& s, int b
 }
 
 int launch_paged_simt(const PagedAttn& a, cudaStream_t st);
+int launch_paged_merge(const PagedAttn& a, cudaStream_t st);
+// Tensor-core kernel for few packed rows per (sequence, kv head).
+bool paged_mma_supported(const PagedAttn& a);
+void paged_mma_plan(PagedAttn* a);
+int launch_paged_mma(const PagedAttn& a, cudaStream_t st);
 
 }  // namespace gorgon

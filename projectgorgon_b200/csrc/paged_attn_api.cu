@@ -23,7 +23,9 @@ int make_args(const gorgon_paged_attn_params* p, PagedAttn* a) {
     return set_error(GORGON_ERR_UNSUPPORTED, "gorgon_paged_attn: trees above 1024 nodes");
   if (p->parents && p->cu_q)
     return set_error(GORGON_ERR_UNSUPPORTED, "gorgon_paged_attn: a tree needs n rows in every sequence (no cu_q)");
-  if (p->backend < GORGON_PAGED_AUTO || p->backend > GORGON_PAGED_SIMT)
+  if (p->cu_q && (p->rows < 0 || p->rows > INT32_MAX))
+    return set_error(GORGON_ERR_INVALID, "gorgon_paged_attn: bad count of packed rows");
+  if (p->backend < GORGON_PAGED_AUTO || p->backend > GORGON_PAGED_MMA)
     return set_error(GORGON_ERR_INVALID, "gorgon_paged_attn: unknown backend");
   if (p->kv.batch * p->heads_q * p->n * p->kv.head_dim > 0 && (!p->q || !p->out || !p->kv.seq_lens))
     return set_error(GORGON_ERR_INVALID, "gorgon_paged_attn: null q, out or seq_lens");
@@ -43,6 +45,7 @@ int make_args(const gorgon_paged_attn_params* p, PagedAttn* a) {
   x.hq = static_cast<int>(p->heads_q);
   x.group = x.hq / x.pool.hkv;
   x.n = static_cast<int>(p->n);
+  x.rows = p->cu_q ? static_cast<int>(p->rows) : 0;
   const float scale = p->scale != 0.f ? p->scale : (x.pool.d > 0 ? 1.f / std::sqrt(static_cast<float>(x.pool.d)) : 1.f);
   x.scale_log2 = scale * 1.4426950408889634f;
   x.wait_ns = wait_limit_ns();
@@ -51,14 +54,46 @@ int make_args(const gorgon_paged_attn_params* p, PagedAttn* a) {
 
 bool empty(const PagedAttn& a) { return static_cast<int64_t>(a.pool.batch) * a.hq * a.n * a.pool.d == 0; }
 
+enum class Kernel { kSimt, kMma, kNone };
+
+Kernel choose(const gorgon_paged_attn_params* p, const PagedAttn& a) {
+  const bool mma = paged_mma_supported(a);
+  switch (p->backend) {
+    case GORGON_PAGED_SIMT: return Kernel::kSimt;
+    case GORGON_PAGED_MMA: return mma ? Kernel::kMma : Kernel::kNone;
+    default: return mma ? Kernel::kMma : Kernel::kSimt;
+  }
+}
+
+constexpr size_t kAlign = 256;
+inline size_t align_up(size_t x) { return (x + kAlign - 1) / kAlign * kAlign; }
+
+size_t cut_workspace(const PagedAttn& a) {
+  const size_t rows = static_cast<size_t>(a.grid) * 2 * a.m;
+  return align_up(a.grid * sizeof(CutUnit)) + align_up(rows * sizeof(float2)) + rows * a.pool.d * sizeof(float);
+}
+
+void place_workspace(PagedAttn* a, void* ws) {
+  const size_t rows = static_cast<size_t>(a->grid) * 2 * a->m;
+  char* w = static_cast<char*>(ws);
+  a->cut = reinterpret_cast<CutUnit*>(w);
+  a->part_ml = reinterpret_cast<float2*>(w + align_up(a->grid * sizeof(CutUnit)));
+  a->part_o = reinterpret_cast<float*>(w + align_up(a->grid * sizeof(CutUnit)) + align_up(rows * sizeof(float2)));
+}
+
 }  // namespace
 }  // namespace gorgon
 
 extern "C" size_t gorgon_paged_attn_workspace_size(const gorgon_paged_attn_params* p) {
   using namespace gorgon;
   PagedAttn a;
-  if (make_args(p, &a) != GORGON_OK) return 0;
-  return 0;
+  if (make_args(p, &a) != GORGON_OK || empty(a)) return 0;
+  switch (choose(p, a)) {
+    case Kernel::kMma:
+      paged_mma_plan(&a);
+      return cut_workspace(a);
+    default: return 0;
+  }
 }
 
 extern "C" int gorgon_paged_attn(const gorgon_paged_attn_params* p, void* workspace, size_t workspace_bytes,
@@ -68,7 +103,18 @@ extern "C" int gorgon_paged_attn(const gorgon_paged_attn_params* p, void* worksp
   int rc = make_args(p, &a);
   if (rc) return rc;
   if (empty(a)) return GORGON_OK;
-  (void)workspace;
-  (void)workspace_bytes;
-  return launch_paged_simt(a, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (choose(p, a)) {
+    case Kernel::kSimt: return launch_paged_simt(a, st);
+    case Kernel::kMma: paged_mma_plan(&a); break;
+    default:
+      return set_error(GORGON_ERR_UNSUPPORTED, "gorgon_paged_attn: the requested kernel needs a 16-bit dtype, head_dim 64 or "
+                                               "128 and rows of whole 16-byte pieces");
+  }
+  if (!workspace || workspace_bytes < cut_workspace(a))
+    return set_error(GORGON_ERR_WORKSPACE, "gorgon_paged_attn: workspace smaller than gorgon_paged_attn_workspace_size()");
+  place_workspace(&a, workspace);
+  rc = launch_paged_mma(a, st);
+  if (rc) return rc;
+  return launch_paged_merge(a, st);
 }

@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_simt_kernel(const PagedAttn
   const int t = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Seq s = sequence(a, b, threadIdx.x == 0 && t == 0 && h == 0);
-  if (t >= s.c || t >= a.n) return;
+  if (t >= s.c || t >= a.n || !rows_inside(a, b, s.c)) return;
   const int64_t row = a.nr.cu ? a.nr.first(b) + t : t;
   T* out = reinterpret_cast<T*>(a.out) + (a.nr.cu ? 0 : b * a.o_sb) + h * a.o_sh + row * a.o_sn;
   float* lse = a.lse ? a.lse + (a.nr.cu ? 0 : b * a.l_sb) + h * a.l_sh + row * a.l_sn : nullptr;
@@ -129,7 +129,82 @@ int launch_t(const PagedAttn& a, cudaStream_t st) {
   return check_cuda(cudaGetLastError(), "gorgon_paged_attn launch");
 }
 
+// Joins the pieces of one unit that the schedule cut (see CutUnit): out = sum_k
+// 2^(m_k - M) o_k / sum_k 2^(m_k - M) l_k.  Grid (main grid, row blocks of 16),
+// a warp per row, two rows each; launched to overlap the end of the main
+// kernel, which it waits for before it reads anything.
+constexpr int kMergeWarps = 8;
+template <typename T, int D>
+__global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const PagedAttn a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int c = blockIdx.x;
+  const CutUnit n = a.cut[c];
+  if (n.pieces == 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int V = D / 32;  // columns per lane
+  const Seq s = sequence(a, n.b, false);
+  const int R = s.c * a.group;
+#pragma unroll 1
+  for (int k = 0; k < 16 / kMergeWarps; ++k) {
+    const int row = blockIdx.y * 16 + k * kMergeWarps + warp;
+    const int pr = n.qb * a.m + row;
+    if (row >= a.m || pr >= R) return;
+    auto slot = [&](int p) -> int64_t { return static_cast<int64_t>(c - 1 + p) * 2 + (p == 0 ? n.first_slot : 0); };
+    float M = -INFINITY;
+    for (int p = lane; p < n.pieces; p += 32) M = fmaxf(M, __ldcg(&a.part_ml[slot(p) * a.m + row]).x);
+    M = warp_max(M);
+    const float base = M == -INFINITY ? 0.f : M;
+    float L = 0.f, acc[V] = {};
+#pragma unroll 4
+    for (int p = 0; p < n.pieces; ++p) {
+      const float2 ml = __ldcg(&a.part_ml[slot(p) * a.m + row]);
+      const float f = exp2f(ml.x - base);
+      const float* o = a.part_o + (slot(p) * a.m + row) * D + lane * V;
+      L = fmaf(f, ml.y, L);
+      if constexpr (V == 4) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(o));
+        acc[0] = fmaf(f, x.x, acc[0]);
+        acc[1] = fmaf(f, x.y, acc[1]);
+        acc[2] = fmaf(f, x.z, acc[2]);
+        acc[3] = fmaf(f, x.w, acc[3]);
+      } else {
+        const float2 x = __ldcg(reinterpret_cast<const float2*>(o));
+        acc[0] = fmaf(f, x.x, acc[0]);
+        acc[1] = fmaf(f, x.y, acc[1]);
+      }
+    }
+    const int t = pr / a.group, h = n.kvh * a.group + pr - t * a.group;
+    const int64_t r = a.nr.cu ? a.nr.cu[n.b] + t : t;
+    T* out = reinterpret_cast<T*>(a.out) + (a.nr.cu ? 0 : n.b * a.o_sb) + h * a.o_sh + r * a.o_sn + lane * V;
+    const float inv = 1.f / L;
+#pragma unroll
+    for (int v = 0; v < V; ++v) out[v] = Cvt<T>::from_f(acc[v] * inv);
+    if (a.lse && lane == 0)
+      a.lse[(a.nr.cu ? 0 : n.b * a.l_sb) + h * a.l_sh + r * a.l_sn] = (M + log2f(L)) * 0.6931471805599453f;
+  }
+}
+
 }  // namespace
+
+int launch_paged_merge(const PagedAttn& a, cudaStream_t st) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.grid), static_cast<unsigned>(a.m / 16));
+  cfg.blockDim = dim3(kMergeWarps * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaError_t e;
+  if (a.pool.dtype == GORGON_BF16)
+    e = a.pool.d == 128 ? cudaLaunchKernelEx(&cfg, paged_merge_kernel<__nv_bfloat16, 128>, a)
+                        : cudaLaunchKernelEx(&cfg, paged_merge_kernel<__nv_bfloat16, 64>, a);
+  else
+    e = a.pool.d == 128 ? cudaLaunchKernelEx(&cfg, paged_merge_kernel<__half, 128>, a)
+                        : cudaLaunchKernelEx(&cfg, paged_merge_kernel<__half, 64>, a);
+  return check_cuda(e, "gorgon_paged_attn merge launch");
+}
 
 int launch_paged_simt(const PagedAttn& a, cudaStream_t st) {
   switch (a.pool.dtype) {

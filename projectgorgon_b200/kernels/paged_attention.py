@@ -16,8 +16,8 @@ from .. import _abi
 from .._paged import compute_dtype, device_index, int32, packer, pool_fields
 from .._util import on_device, parents_tensor, stream_ptr, workspace
 
-_ATTN = packer("qq" + "Pqqq" * 3 + "PPqiqqfi")
-_BACKENDS = {"auto": _abi.PAGED_AUTO, "simt": _abi.PAGED_SIMT}
+_ATTN = packer("qqq" + "Pqqq" * 3 + "PPqiqqfi")
+_BACKENDS = {"auto": _abi.PAGED_AUTO, "simt": _abi.PAGED_SIMT, "mma": _abi.PAGED_MMA}
 
 
 def paged_attention(
@@ -139,7 +139,7 @@ def paged_attention(
         raise RuntimeError(f"window must be at least 1, got {window}")
     if sinks < 0:
         raise RuntimeError(f"sinks must not be negative, got {sinks}")
-    params = _ATTN.pack(*pool, hq, n, q.data_ptr(), q_sb, q_sh, q_sn, out.data_ptr(), o_sb, o_sh, o_sn,
+    params = _ATTN.pack(*pool, hq, n, 0 if cu is None else total, q.data_ptr(), q_sb, q_sh, q_sn, out.data_ptr(), o_sb, o_sh, o_sn,
                         l_ptr, l_sb, l_sh, l_sn, 0 if cu is None else cu.data_ptr(), p_ptr, p_sb,
                         -1 if max_depth is None else int(max_depth), 0 if window is None else int(window), int(sinks),
                         0.0 if scale is None else float(scale), be)
