@@ -10,8 +10,10 @@
 // The tiles of all units, in the order (sequence, kv head, row block), form one
 // list that the grid's CTAs share out in equal contiguous ranges, so ragged
 // batches, long single sequences and windows balance by themselves, without
-// the host knowing any length.  A unit inside one CTA's range is finished
-// there; one cut between CTAs leaves unnormalised fp32 rows with their running
+// the host knowing any length.  A unit also costs its start and end (loading
+// Q, joining warps, writing rows), which counts as `unit_cost` empty places
+// before its tiles: a batch of short sequences would otherwise load some CTAs
+// with many units.  A unit inside one CTA's range is finished there; one cut between CTAs leaves unnormalised fp32 rows with their running
 // max and sum in the workspace (slot 0: the piece that a CTA starts with, slot
 // 1: the one that it ends with), and paged_merge_kernel joins them in the
 // order of the CTAs, so results do not depend on timing.
@@ -42,6 +44,7 @@ struct PagedAttn {
   // tensor-core schedule
   int m, bn;          // packed rows per unit, positions per tile
   int qblocks;        // units per (sequence, kv head) at most
+  int unit_cost;      // places in the list that a unit's start and end take
   int grid;
   float* part_o;      // [grid * 2][m][d]
   float2* part_ml;    // [grid * 2][m]  running max (log2 units) and sum
@@ -110,46 +113,59 @@ __device__ __forceinline__ bool block_rows(const PagedAttn& a, const Seq& s, int
   return true;
 }
 
-// Tiles of every row block of one (sequence, kv head).
-__device__ __forceinline__ int64_t head_tiles(const PagedAttn& a, const Seq& s) {
+// Places of every row block of one (sequence, kv head).
+__device__ __forceinline__ int64_t head_places(const PagedAttn& a, const Seq& s) {
   int64_t n = 0;
   int t0, t1;
   if (!s.ok) return 0;
-  for (int qb = 0; block_rows(a, s, qb, t0, t1); ++qb) n += unit_keys(a, s, t0, t1).tiles;
+  for (int qb = 0; block_rows(a, s, qb, t0, t1); ++qb) n += unit_keys(a, s, t0, t1).tiles + a.unit_cost;
   return n;
 }
 
-// A position in the list of tiles.
+// A tile in the list.
 struct TileCursor {
   int b, kvh, qb;
-  int i;       // tile within the unit
-  int t0, t1;  // the unit's new rows
+  int i;        // tile within the unit
+  int t0, t1;   // the unit's new rows
+  int at;       // the tile's place, counted from the CTA's first place
   Seq s;
   UnitKeys u;
   __device__ __forceinline__ int tile() const { return u.tile(i); }
-  // To the next tile; the caller knows that there is one.
-  __device__ __forceinline__ void next(const PagedAttn& a) {
-    if (++i < u.tiles) return;
+  // To the unit after this one; false when there is none.
+  __device__ __forceinline__ bool next_unit(const PagedAttn& a) {
+    at += u.tiles - i + a.unit_cost;
     i = 0;
     ++qb;
     if (!block_rows(a, s, qb, t0, t1)) {
       qb = 0;
       if (++kvh == a.pool.hkv) {
         kvh = 0;
-        do s = sequence(a, ++b, false);
-        while (!s.ok && b < a.pool.batch - 1);
+        do {
+          if (++b >= a.pool.batch) return false;
+          s = sequence(a, b, false);
+        } while (!s.ok);
       }
       block_rows(a, s, qb, t0, t1);
     }
     u = unit_keys(a, s, t0, t1);
+    return true;
+  }
+  // To the next tile before place `end`; false when there is none.
+  __device__ __forceinline__ bool next(const PagedAttn& a, int end) {
+    if (i + 1 < u.tiles) {
+      ++i;
+      ++at;
+      return at < end;
+    }
+    return at + 1 + a.unit_cost < end && next_unit(a) && at < end;
   }
 };
 
-// The CTA's share [g0, g1) of the T tiles (G CTAs have one: no more than there
-// are tiles), and the cursor at g0 (called by all THREADS threads of the CTA;
-// `sh` is shared scratch).  Thread t counts the
-// tiles of sequences [t * per, (t + 1) * per), a block scan places them, and
-// the thread that owns g0 names its sequence.
+// The CTA's share of the list's T places, [g0, g1) (G CTAs have one), and its
+// first tile (called by all THREADS threads of the CTA; `sh` is shared
+// scratch); false when it has no tile.  Thread t counts the places of sequences
+// [t * per, (t + 1) * per), a block scan places them, and the thread that
+// owns g0 names its sequence.
 struct ShareScratch {
   int64_t warp_sum[32];
   int64_t rem;
@@ -164,7 +180,7 @@ __device__ __forceinline__ bool cta_share(const PagedAttn& a, ShareScratch* sh, 
   const int per = (a.pool.batch + THREADS - 1) / THREADS;
   const int b0 = min(tid * per, a.pool.batch), b1 = min(b0 + per, a.pool.batch);
   int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += head_tiles(a, sequence(a, b, blockIdx.x == 0)) * a.pool.hkv;
+  for (int b = b0; b < b1; ++b) mine += head_places(a, sequence(a, b, blockIdx.x == 0)) * a.pool.hkv;
   int64_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -190,7 +206,7 @@ __device__ __forceinline__ bool cta_share(const PagedAttn& a, ShareScratch* sh, 
     int64_t rem = g0 - start;
     int b = b0;
     for (; b < b1 - 1; ++b) {
-      const int64_t n = head_tiles(a, sequence(a, b, false)) * a.pool.hkv;
+      const int64_t n = head_places(a, sequence(a, b, false)) * a.pool.hkv;
       if (rem < n) break;
       rem -= n;
     }
@@ -201,29 +217,33 @@ __device__ __forceinline__ bool cta_share(const PagedAttn& a, ShareScratch* sh, 
   if (!work) return false;
   cur.b = sh->b;
   cur.s = sequence(a, cur.b, false);
-  const int64_t per_head = head_tiles(a, cur.s);
+  const int64_t per_head = head_places(a, cur.s);
   cur.kvh = static_cast<int>(sh->rem / per_head);
-  int64_t rem = sh->rem - cur.kvh * per_head;
+  int rem = static_cast<int>(sh->rem - cur.kvh * per_head);
   for (cur.qb = 0;; ++cur.qb) {
     block_rows(a, cur.s, cur.qb, cur.t0, cur.t1);
     cur.u = unit_keys(a, cur.s, cur.t0, cur.t1);
-    if (rem < cur.u.tiles) break;
-    rem -= cur.u.tiles;
+    if (rem < cur.u.tiles + a.unit_cost) break;
+    rem -= cur.u.tiles + a.unit_cost;
   }
-  cur.i = static_cast<int>(rem);
-  return true;
+  cur.i = max(0, rem - a.unit_cost);
+  cur.at = cur.i + a.unit_cost - rem;
+  return cur.at < r.g1 - r.g0;
 }
 
-// CTA c's note for the merge; `cur` is at the CTA's first tile.
+// CTA c's note for the merge; `cur` is at the CTA's first tile.  When the CTA
+// starts inside a unit's tiles, the tile before is CTA c - 1's; the unit's
+// first tile is too unless an earlier CTA names it.  CTA c - 1 began with this
+// unit if its range starts in it (the place before a unit is a tile).
 __device__ __forceinline__ void note_cut(const PagedAttn& a, bool work, const TileCursor& cur, const Share& r) {
   CutUnit n{};
   if (work && cur.i > 0) {
     const int c = blockIdx.x;
-    const int64_t start = r.g0 - cur.i, end = start + cur.u.tiles;  // the unit's tiles
+    const int64_t first = r.g0 - cur.i, end = first + cur.u.tiles;  // places of the unit's tiles
     const int64_t prev = static_cast<int64_t>(c - 1) * r.T / r.G;
-    if (start >= prev) {  // the unit starts in CTA c - 1's range (else an earlier CTA names it)
-      const int last = static_cast<int>((end * r.G - 1) / r.T);  // the CTA of tile end - 1
-      n = CutUnit{cur.b, cur.kvh, cur.qb, last - c + 2, start == prev ? 0 : 1};
+    if (first >= prev) {
+      const int last = static_cast<int>((end * r.G - 1) / r.T);  // the CTA of place end - 1
+      n = CutUnit{cur.b, cur.kvh, cur.qb, last - c + 2, prev >= first - a.unit_cost ? 0 : 1};
     }
   }
   a.cut[blockIdx.x] = n;

@@ -130,65 +130,82 @@ int launch_t(const PagedAttn& a, cudaStream_t st) {
 }
 
 // Joins the pieces of one unit that the schedule cut (see CutUnit): out = sum_k
-// 2^(m_k - M) o_k / sum_k 2^(m_k - M) l_k.  Grid (main grid, row blocks of 16),
-// a warp per row, two rows each; launched to overlap the end of the main
-// kernel, which it waits for before it reads anything.
+// 2^(m_k - M) o_k / sum_k 2^(m_k - M) l_k.  Grid (main grid, row blocks of 8).
+// A warp per row, or several when fewer than 8 rows are in use: each takes its
+// share of the pieces, eight loads in flight, and their sums meet in shared
+// memory in a fixed order.  Launched to overlap the end of the main kernel,
+// which it waits for before it reads anything.
 constexpr int kMergeWarps = 8;
 template <typename T, int D>
-__global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const PagedAttn a) {
+__global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __grid_constant__ PagedAttn a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  __shared__ float s_acc[kMergeWarps][D];
+  __shared__ float s_l[kMergeWarps];
   const int c = blockIdx.x;
   const CutUnit n = a.cut[c];
   if (n.pieces == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int V = D / 32;  // columns per lane
   const Seq s = sequence(a, n.b, false);
-  const int R = s.c * a.group;
-#pragma unroll 1
-  for (int k = 0; k < 16 / kMergeWarps; ++k) {
-    const int row = blockIdx.y * 16 + k * kMergeWarps + warp;
-    const int pr = n.qb * a.m + row;
-    if (row >= a.m || pr >= R) return;
-    auto slot = [&](int p) -> int64_t { return static_cast<int64_t>(c - 1 + p) * 2 + (p == 0 ? n.first_slot : 0); };
-    float M = -INFINITY;
-    for (int p = lane; p < n.pieces; p += 32) M = fmaxf(M, __ldcg(&a.part_ml[slot(p) * a.m + row]).x);
-    M = warp_max(M);
-    const float base = M == -INFINITY ? 0.f : M;
-    float L = 0.f, acc[V] = {};
-#pragma unroll 4
-    for (int p = 0; p < n.pieces; ++p) {
-      const float2 ml = __ldcg(&a.part_ml[slot(p) * a.m + row]);
-      const float f = exp2f(ml.x - base);
-      const float* o = a.part_o + (slot(p) * a.m + row) * D + lane * V;
-      L = fmaf(f, ml.y, L);
-      if constexpr (V == 4) {
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(o));
-        acc[0] = fmaf(f, x.x, acc[0]);
-        acc[1] = fmaf(f, x.y, acc[1]);
-        acc[2] = fmaf(f, x.z, acc[2]);
-        acc[3] = fmaf(f, x.w, acc[3]);
-      } else {
-        const float2 x = __ldcg(reinterpret_cast<const float2*>(o));
-        acc[0] = fmaf(f, x.x, acc[0]);
-        acc[1] = fmaf(f, x.y, acc[1]);
-      }
+  const int rows = min(8, min(a.m, s.c * a.group - n.qb * a.m) - static_cast<int>(blockIdx.y) * 8);
+  if (rows <= 0) return;
+  const int per = rows <= 1 ? 8 : rows <= 2 ? 4 : rows <= 4 ? 2 : 1;  // warps per row
+  const int sub = warp % per, r8 = warp / per;
+  const bool live = r8 < rows;
+  const int row = blockIdx.y * 8 + (live ? r8 : 0);
+  auto slot = [&](int p) -> int64_t { return static_cast<int64_t>(c - 1 + p) * 2 + (p == 0 ? n.first_slot : 0); };
+  float M = -INFINITY;
+  for (int p = lane; p < n.pieces; p += 32) M = fmaxf(M, __ldcg(&a.part_ml[slot(p) * a.m + row]).x);
+  M = warp_max(M);
+  const float base = M == -INFINITY ? 0.f : M;
+  float L = 0.f, acc[V] = {};
+#pragma unroll 8
+  for (int p = sub; p < n.pieces; p += per) {
+    const float2 ml = __ldcg(&a.part_ml[slot(p) * a.m + row]);
+    const float f = exp2f(ml.x - base);
+    const float* o = a.part_o + (slot(p) * a.m + row) * D + lane * V;
+    L = fmaf(f, ml.y, L);
+    if constexpr (V == 4) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(o));
+      acc[0] = fmaf(f, x.x, acc[0]);
+      acc[1] = fmaf(f, x.y, acc[1]);
+      acc[2] = fmaf(f, x.z, acc[2]);
+      acc[3] = fmaf(f, x.w, acc[3]);
+    } else {
+      const float2 x = __ldcg(reinterpret_cast<const float2*>(o));
+      acc[0] = fmaf(f, x.x, acc[0]);
+      acc[1] = fmaf(f, x.y, acc[1]);
     }
-    const int t = pr / a.group, h = n.kvh * a.group + pr - t * a.group;
-    const int64_t r = a.nr.cu ? a.nr.cu[n.b] + t : t;
-    T* out = reinterpret_cast<T*>(a.out) + (a.nr.cu ? 0 : n.b * a.o_sb) + h * a.o_sh + r * a.o_sn + lane * V;
-    const float inv = 1.f / L;
-#pragma unroll
-    for (int v = 0; v < V; ++v) out[v] = Cvt<T>::from_f(acc[v] * inv);
-    if (a.lse && lane == 0)
-      a.lse[(a.nr.cu ? 0 : n.b * a.l_sb) + h * a.l_sh + r * a.l_sn] = (M + log2f(L)) * 0.6931471805599453f;
   }
+  if (per > 1) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) s_acc[warp][lane * V + v] = acc[v];
+    if (lane == 0) s_l[warp] = L;
+    __syncthreads();
+    if (sub != 0) return;
+    for (int w = 1; w < per; ++w) {
+      L += s_l[warp + w];
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] += s_acc[warp + w][lane * V + v];
+    }
+  }
+  if (!live) return;
+  const int pr = n.qb * a.m + row;
+  const int t = pr / a.group, h = n.kvh * a.group + pr - t * a.group;
+  const int64_t r = a.nr.cu ? a.nr.cu[n.b] + t : t;
+  T* out = reinterpret_cast<T*>(a.out) + (a.nr.cu ? 0 : n.b * a.o_sb) + h * a.o_sh + r * a.o_sn + lane * V;
+  const float inv = 1.f / L;
+#pragma unroll
+  for (int v = 0; v < V; ++v) out[v] = Cvt<T>::from_f(acc[v] * inv);
+  if (a.lse && lane == 0)
+    a.lse[(a.nr.cu ? 0 : n.b * a.l_sb) + h * a.l_sh + r * a.l_sn] = (M + log2f(L)) * 0.6931471805599453f;
 }
 
 }  // namespace
 
 int launch_paged_merge(const PagedAttn& a, cudaStream_t st) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.grid), static_cast<unsigned>(a.m / 16));
+  cfg.gridDim = dim3(static_cast<unsigned>(a.grid), static_cast<unsigned>(ceil_div(a.m, 8)));
   cfg.blockDim = dim3(kMergeWarps * 32);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
