@@ -1,13 +1,15 @@
 // Paged attention for few packed rows per (sequence, kv head): single tokens of
 // grouped heads, short drafts.  Bound by the bytes of the cache.
 //
-// A CTA per SM walks its share of the tile list (paged_attn.cuh).  A tile is one
-// group of 16 keys for each warp, and the warps work on their own: each
-// streams its groups' K and V rows into its own ring of shared memory with
-// 16-byte cp.async copies (about 190 KB an SM in flight or in use, well above
-// what covers the memory latency) and keeps its own running softmax, so there
-// is no barrier in the loop.  Rows are gathered one by one, so pages may be of
-// any size and stride; the table entry of a group is fetched one group ahead.
+// Two CTAs per SM walk their shares of the tile list (paged_attn.cuh).  A tile is
+// one group of 16 or 32 keys for each warp, and the warps work on their own:
+// each streams its groups' K and V rows into its own ring of shared memory
+// with 16-byte cp.async copies (three stages of 8 KB a warp, about 200 KB an SM
+// in flight or in use, well above what covers the memory latency) and keeps
+// its own running softmax, so there is no barrier in the loop.  Rows are
+// gathered one by one, so pages may be of any size and stride; the table entry
+// of a group is fetched one group ahead.  (Bulk copies of a row, which would
+// need fewer instructions, are issued lane by lane: they took more.)
 //
 // Products run on mma.sync m16n8k16 with the keys as M: S^T = K Q^T and
 // O^T = V^T P^T, so that a tile is 16 keys by 8 packed rows and a group of up to
@@ -32,8 +34,7 @@ namespace gorgon {
 namespace {
 
 constexpr int kCtasPerSm = 2;
-constexpr int kRedFloats = 2496;
-constexpr int G = 16;  // keys per warp and tile
+constexpr int kRedFloats = 2480;
 
 template <typename T, int ST, int D_, int NT_>
 struct Cfg {
@@ -41,27 +42,40 @@ struct Cfg {
   static constexpr bool kWide = ST == GORGON_KV_NATIVE;  // 16-bit pages
   using X = std::conditional_t<kWide, T, __half>;        // type of the products' operands
   static constexpr int kRowBytes = kWide ? D * 2 : D;
-  static constexpr int kHalf = G * kRowBytes;            // K (or V) bytes of a stage
-  static constexpr int kMeta = kWide ? 16 : 16 + 8 * G;  // keys' word and first position, then K and V scales
-  static constexpr int kStage = 2 * kHalf + kMeta;
+  static constexpr int KB = kRowBytes == 256 ? 1 : 2;    // blocks of 16 keys per group
+  static constexpr int G = 16 * KB;                      // keys per warp and tile
+  // A stage: K rows, V rows, the group's two words, then K and V scales.
+  static constexpr int kHalf = G * kRowBytes;
+  static constexpr int kOffWord = 2 * kHalf;
+  static constexpr int kStage = kOffWord + (kWide ? 16 : 16 + 8 * G);
   // Two CTAs an SM, so that one's unit ends (barriers, the next unit's Q) pass
-  // under the other's loads.  Warps: as many as the registers allow (a row tile
-  // of D = 128 holds 48 in Q and O); stages fill the shared memory.
-  static constexpr int kWarps = kRowBytes == 256 ? 4 : (NT == 2 && D == 128) ? 6 : 8;
+  // under the other's loads.
+  static constexpr int kWarps = kRowBytes == 64 ? 6 : 4;
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kStages = kRowBytes == 256 ? 3 : kWarps == 6 ? 4 : kRowBytes == 128 ? 3 : 5;
+  static constexpr int kStages = kRowBytes == 64 ? 4 : 3;
   static constexpr int BN = G * kWarps;
   static constexpr int M = 8 * NT;
-  static constexpr int kCpr = kRowBytes / 16;            // 16-byte pieces per row
-  static constexpr int kRpi = 32 / kCpr;                 // rows per copy instruction
+  // 16-byte pieces: kCpr to a row, kRpi rows to a copy instruction.  Piece p of
+  // row r lies at p ^ (r % 8) (rows of 64 bytes: p ^ (r / 2 % 4)), so that a
+  // fragment's reads meet no bank twice; a lane's pieces follow one of
+  // kSwizzles patterns.
+  static constexpr int kCpr = kRowBytes / 16, kRpi = 32 / kCpr, kSwizzles = kRpi >= 8 ? 1 : 8 / kRpi;
+  static __device__ __forceinline__ uint32_t at(int row, int piece) {
+    if constexpr (kCpr >= 8) return static_cast<uint32_t>(row * kCpr + (piece ^ (row & 7))) * 16u;
+    return static_cast<uint32_t>(row * kCpr + (piece ^ ((row >> 1) & (kCpr - 1)))) * 16u;
+  }
   static constexpr int kRing = kStages * kStage;
+  // The block where the warps' rows meet; before that, the scratch of the
+  // schedule, and while a unit runs, its tree's bits and depths and the warps'
+  // maxima and sums.
   static constexpr int kOffRed = kWarps * kRing;
-  static constexpr int kOffMl = kOffRed + kRedFloats * 4;            // [warps][M] max, sum
-  static constexpr int kOffRow = kOffMl + kWarps * M * 8;            // [M] max, sum over the warps
-  static constexpr int kOffBits = kOffRow + M * 8;           // [M][32] ancestor words
+  static constexpr int kOffBits = kOffRed;                                  // [M][32] ancestor words
   static constexpr int kOffDepth = kOffBits + M * (kPagedMaxNodes / 32) * 4;
-  static constexpr int kOffCur = (kOffDepth + M * 4 + 15) / 16 * 16; // [warps] TileCursor
-  static constexpr int kSmem = kOffCur + kWarps * static_cast<int>(sizeof(TileCursor));
+  static constexpr int kOffMl = kOffRed + 4096;                             // [warps][M] max, sum
+  static_assert(kOffDepth + M * 4 <= kOffMl && kOffMl + kWarps * M * 8 <= kOffRed + kRedFloats * 4, "shared block");
+  static constexpr int kOffRow = kOffRed + kRedFloats * 4;                  // [M] max, sum over the warps
+  static constexpr int kOffCur = kOffRow + M * 8;                           // TileCursor of the unit worked on, and each warp's of the unit fetched
+  static constexpr int kSmem = kOffCur + (kWarps + 1) * static_cast<int>(sizeof(TileCursor));
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -132,6 +146,22 @@ __device__ __forceinline__ uint32_t widen(uint32_t a, uint32_t b) {
   }
 }
 
+// The four bytes of a word as two pairs.
+template <int ST>
+__device__ __forceinline__ void widen_word(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (ST == GORGON_KV_INT8) {
+    const uint32_t u = w ^ 0x80808080u, f = 0x64806480u;
+    const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&f));
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&f));
+    lo = *reinterpret_cast<const uint32_t*>(&x);
+    hi = *reinterpret_cast<const uint32_t*>(&y);
+  } else {
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"(static_cast<uint16_t>(w)));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"(static_cast<uint16_t>(w >> 16)));
+  }
+}
+
 // f16 weights times V scales need f16's range: they are taken in units of
 // 2^(E - 6), with 2^E above the largest V scale that the warp has met in the
 // unit, so that they stay below 2^14 (a weight is at most 2^8) and keep a row's
@@ -140,27 +170,60 @@ __device__ __forceinline__ uint32_t widen(uint32_t a, uint32_t b) {
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
 constexpr int kNoExp = -116;  // nothing met yet
 
-template <int CPR>
-__device__ __forceinline__ uint32_t piece_at(int row, int piece) {  // byte offset within a K or V block
-  if constexpr (CPR >= 8) return static_cast<uint32_t>(row * CPR + (piece ^ (row & 7))) * 16u;
-  return static_cast<uint32_t>(row * CPR + (piece ^ ((row >> 1) & (CPR - 1)))) * 16u;
+// What the loop does rarely lives in calls, so that the loop itself stays short
+// and in the instruction cache.
+
+// Bit 4 nt + e: the thread's score (nt, e) is hidden.  `row` is the first of its
+// packed rows, j[] its two keys' positions, held[] whether they were fetched.
+__device__ __noinline__ uint32_t hidden_scores(const PagedAttn& a, const TileCursor* cur, const uint32_t* bits,
+                                               const int* depth, int row, int tiles, int j0, int j1, bool held0, bool held1) {
+  uint32_t out = 0;
+  const int P = cur->s.P, R = cur->s.c * a.group;
+  for (int k = 0; k < tiles * 4; ++k) {
+    const int pr = row + (k >> 2) * 8 + (k & 1), j = k & 2 ? j1 : j0;
+    bool see = (k & 2 ? held1 : held0) && pr < R;
+    if (see) {
+      const int t = pr / a.group;
+      if (a.parents && j >= P) {
+        see = j - P < cur->s.c && ((bits[(t - cur->t0) * (kPagedMaxNodes / 32) + ((j - P) >> 5)] >> ((j - P) & 31)) & 1u);
+      } else {
+        const int pos = P + (a.parents ? depth[t - cur->t0] : t);
+        see = j <= pos && (!a.window || j > pos - a.window || j < a.sinks);
+      }
+    }
+    out |= see ? 0u : 1u << k;
+  }
+  return out;
+}
+
+// A cursor in shared memory to the next unit (one lane); its `at` is `end` or
+// more when the CTA has no tile there.
+__device__ __noinline__ void step_unit(const PagedAttn& a, TileCursor* cur, int end) {
+  TileCursor n = *cur;
+  n.at += n.u.tiles - 1 - n.i;
+  n.i = n.u.tiles - 1;
+  if (!n.next(a, end)) n.at = end;
+  *cur = n;
 }
 
 template <typename T, int ST, int D, int NT>
 __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged_mma_kernel(const __grid_constant__ PagedAttn a) {
   using C = Cfg<T, ST, D, NT>;
   using X = typename C::X;
+  constexpr int KB = C::KB, G = C::G;
+  constexpr uint32_t kAll = G == 32 ? 0xffffffffu : (1u << (G & 31)) - 1u;
   constexpr bool kScaleQ = !C::kWide && std::is_same_v<T, __nv_bfloat16>;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ ShareScratch sh;
+  static_assert(sizeof(ShareScratch) <= kRedFloats * 4, "scratch");
+  ShareScratch* sh = reinterpret_cast<ShareScratch*>(smem + C::kOffRed);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
 
   Share share;
-  TileCursor ahead;
-  const bool work = cta_share<C::kThreads>(a, &sh, share, ahead);
-  if (threadIdx.x == 0) note_cut(a, work, ahead, share);
+  TileCursor first_tile;
+  const bool work = cta_share<C::kThreads>(a, sh, share, first_tile);
+  if (threadIdx.x == 0) note_cut(a, work, first_tile, share);
   clear_unused<T, C::kThreads>(a);
   if (!work) return;
 
@@ -171,38 +234,47 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
   float* s_red = reinterpret_cast<float*>(smem + C::kOffRed);
   float2* s_ml = reinterpret_cast<float2*>(smem + C::kOffMl);
   float2* s_row = reinterpret_cast<float2*>(smem + C::kOffRow);
-  // The unit being worked on.  It lives in shared memory: the loop needs it only
-  // where units begin and end, and for partly hidden groups.
-  TileCursor& cur = reinterpret_cast<TileCursor*>(smem + C::kOffCur)[warp];
-  if (lane == 0) cur = ahead;
-  __syncwarp();
+  // The unit being worked on, and the unit whose tiles are being fetched.  They
+  // live in shared memory: the loop needs little of them.
+  TileCursor& cur = *reinterpret_cast<TileCursor*>(smem + C::kOffCur);
+  TileCursor& ahead = reinterpret_cast<TileCursor*>(smem + C::kOffCur)[1 + warp];
+  if (threadIdx.x == 0) cur = first_tile;
+  if (lane == 0) ahead = first_tile;
+  __syncthreads();
 
-  // ---- loads: `ahead` is the cursor of the next tile to fetch, `page` the page
-  // of key lane % 16 there (-2: not wanted), fetched when the cursor got there.
-  // A stage's word says which keys it holds (bits 0 .. 15), whether every row of
-  // the unit sees them all (kPlain), and whether its tile is the unit's last.
-  constexpr uint32_t kPlain = 1u << 16, kLast = 1u << 17;
-  bool cut_start = ahead.i > 0;  // the CTA's first unit began in another CTA
+  // ---- loads: `page` is the page of key lane % G of the next tile to fetch
+  // (-2: not wanted), fetched when the cursor got there.  A stage's words say
+  // which keys it holds, and the first one's position with, in the top bit,
+  // whether every row of the unit sees them all.
+  constexpr uint32_t kPlain = 1u << 31;
+  bool cut_start = first_tile.i > 0;  // the CTA's first unit began in another CTA
   const int end = static_cast<int>(share.g1 - share.g0);
-  bool more = true;
+  UnitKeys u;              // of `ahead`
+  int tile = 0, left = 0;  // the tile to fetch, and how many of the unit's are left to fetch with it
   int page = -2, prow = 0;
-  const bool one_page = a.pool.page_size % G == 0;  // a group lies in one page
+  const bool in_pages = a.pool.page_size % 16 == 0;  // 16 keys from a multiple of 16 on lie in one page
   const int piece = lane % C::kCpr, rsub = lane / C::kCpr;
+  uint32_t swizzled[C::kSwizzles];
+#pragma unroll
+  for (int k = 0; k < C::kSwizzles; ++k) swizzled[k] = C::at(k * C::kRpi + rsub, piece) - k * C::kRpi * C::kRowBytes;
   const uint32_t k_sp = static_cast<uint32_t>(a.pool.k_sp), v_sp = static_cast<uint32_t>(a.pool.v_sp);
   const uint32_t k_ss = static_cast<uint32_t>(a.pool.k_ss), v_ss = static_cast<uint32_t>(a.pool.v_ss);
-  // lanes 0 .. 15 fetch K scales, 16 .. 31 V scales
-  const uint32_t sc_sp = static_cast<uint32_t>(lane < 16 ? a.pool.ks_sp : a.pool.vs_sp);
-  const uint32_t sc_ss = static_cast<uint32_t>(lane < 16 ? a.pool.ks_ss : a.pool.vs_ss);
-  // per unit: this lane's place in the head's rows, and the positions that every row of the unit sees, [all_lo, all_hi]
-  // and the sinks before it (the rows' last position is at most last: a tree row's depth is below c)
+  // per unit: the head's rows, and the positions that every row of the unit sees, [all_lo, all_hi] and the sinks before
+  // it (the rows' last position is at most last: a tree row's depth is below c)
   const char *kb = nullptr, *vb = nullptr;
-  const float* sb = nullptr;
-  int all_hi = 0, all_lo = 0;
+  const float *ksb = nullptr, *vsb = nullptr;
   const int32_t* tb = nullptr;
+  int all_hi = 0, all_lo = 0;
   auto enter = [&]() {
+    u = ahead.u;
+    tile = ahead.i;
+    left = min(u.tiles - tile, end - ahead.at);
     kb = a.pool.k + ahead.kvh * a.pool.k_sh + piece * 16;
     vb = a.pool.v + ahead.kvh * a.pool.v_sh + piece * 16;
-    if constexpr (!C::kWide) sb = lane < 16 ? a.pool.ks + ahead.kvh * a.pool.ks_sh : a.pool.vs + ahead.kvh * a.pool.vs_sh;
+    if constexpr (!C::kWide) {
+      ksb = a.pool.ks + ahead.kvh * a.pool.ks_sh;
+      vsb = a.pool.vs + ahead.kvh * a.pool.vs_sh;
+    }
     tb = a.pool.table + static_cast<int64_t>(ahead.b) * a.pool.table_sb;
     all_hi = a.parents ? ahead.s.P - 1 : ahead.s.P + ahead.t0;
     const int last = ahead.s.P + (a.parents ? ahead.s.c : ahead.t1) - 1;
@@ -210,109 +282,107 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
   };
   auto look_up = [&]() {
     page = -2;
-    const int j = ahead.tile() * C::BN + warp * G + (lane & 15);
-    if (ahead.u.wanted(j)) {
+    const int j = u.tile(tile) * C::BN + warp * G + (lane & (G - 1));
+    if (u.wanted(j)) {
       int col;
       a.pool.split(j, col, prow);
       page = __ldg(tb + col);  // col is inside: L fits the table
     }
   };
   auto issue = [&](int stage) {
-    if (more) {
-      const bool wanted = page != -2;
+    if (left > 0) {
       const bool held = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pool.num_pages);
-      if (wanted && !held) raise_device_error(a.pool.err, kErrBadPage);
-      const uint32_t valid = __ballot_sync(0xffffffffu, held) & 0xffffu;
+      if (page != -2 && !held) raise_device_error(a.pool.err, kErrBadPage);
+      const uint32_t valid = __ballot_sync(0xffffffffu, held) & kAll;
       const uint32_t dst = ring_s + stage * C::kStage;
-      const int j0 = ahead.tile() * C::BN + warp * G;
-      const bool plain = valid == 0xffffu && j0 + G - 1 <= all_hi && (j0 >= all_lo || j0 + G <= a.sinks);
+      const int j0 = u.tile(tile) * C::BN + warp * G;
+      const bool plain = valid == kAll && j0 + G - 1 <= all_hi && (j0 >= all_lo || j0 + G <= a.sinks);
       if (lane == 0)
-        *reinterpret_cast<uint2*>(ring + stage * C::kStage + 2 * C::kHalf) =
-            make_uint2(valid | (plain ? kPlain : 0u) | (ahead.i + 1 == ahead.u.tiles ? kLast : 0u), static_cast<uint32_t>(j0));
+        *reinterpret_cast<uint2*>(ring + stage * C::kStage + C::kOffWord) =
+            make_uint2(valid, static_cast<uint32_t>(j0) | (plain ? kPlain : 0u));
       if (valid) {
-        if (one_page) {
-          const int src = __ffs(valid) - 1;
-          const uint32_t pg = __shfl_sync(0xffffffffu, page, src);
-          const uint32_t r0 = __shfl_sync(0xffffffffu, prow, src) - src + rsub;
-          const char* kr = kb + static_cast<uint64_t>(pg) * k_sp + static_cast<uint64_t>(r0) * k_ss;
-          const char* vr = vb + static_cast<uint64_t>(pg) * v_sp + static_cast<uint64_t>(r0) * v_ss;
-          const uint32_t mine = valid >> rsub;
+        if (in_pages) {
 #pragma unroll
-          for (int it = 0; it < G / C::kRpi; ++it) {
-            const bool take = (mine >> (it * C::kRpi)) & 1u;
-            const uint32_t at = piece_at<C::kCpr>(it * C::kRpi + rsub, piece);
-            cp16(dst + at, kr, take);
-            cp16(dst + C::kHalf + at, vr, take);
-            kr += static_cast<uint64_t>(C::kRpi) * k_ss;
-            vr += static_cast<uint64_t>(C::kRpi) * v_ss;
+          for (int kbk = 0; kbk < KB; ++kbk) {
+            const uint32_t mine = (valid >> (16 * kbk)) & 0xffffu;
+            const int src = __ffs(mine | 0x10000u) - 1;  // a wanted key of the block: its page is the block's
+            const uint32_t pg = __shfl_sync(0xffffffffu, page, 16 * kbk + (src & 15));
+            const uint32_t r0 = __shfl_sync(0xffffffffu, prow, 16 * kbk + (src & 15)) - (src & 15) + rsub;
+            const char* kr = kb + static_cast<uint64_t>(pg) * k_sp + static_cast<uint64_t>(r0) * k_ss;
+            const char* vr = vb + static_cast<uint64_t>(pg) * v_sp + static_cast<uint64_t>(r0) * v_ss;
+            if (mine == 0xffffu) {
+#pragma unroll
+              for (int it = 0; it < 16 / C::kRpi; ++it) {
+                const uint32_t at = dst + (kbk * 16 + it * C::kRpi) * C::kRowBytes + swizzled[it % C::kSwizzles];
+                cp16(at, kr + it * C::kRpi * static_cast<uint64_t>(k_ss), true);
+                cp16(at + C::kHalf, vr + it * C::kRpi * static_cast<uint64_t>(v_ss), true);
+              }
+            } else {
+#pragma unroll 1
+              for (int it = 0; it < 16 / C::kRpi; ++it) {
+                const bool take = (mine >> (it * C::kRpi + rsub)) & 1u;
+                const uint32_t at = dst + C::at(kbk * 16 + it * C::kRpi + rsub, piece);
+                cp16(at, take ? kr + it * C::kRpi * static_cast<uint64_t>(k_ss) : kb, take);
+                cp16(at + C::kHalf, take ? vr + it * C::kRpi * static_cast<uint64_t>(v_ss) : vb, take);
+              }
+            }
           }
         } else {
           const uint32_t pg = held ? page : 0, pr = held ? prow : 0;
           const uint64_t ko = static_cast<uint64_t>(pg) * k_sp + static_cast<uint64_t>(pr) * k_ss;
           const uint64_t vo = static_cast<uint64_t>(pg) * v_sp + static_cast<uint64_t>(pr) * v_ss;
-#pragma unroll
+#pragma unroll 1
           for (int it = 0; it < G / C::kRpi; ++it) {
             const int r = it * C::kRpi + rsub;
             const bool take = (valid >> r) & 1u;
-            const uint32_t at = piece_at<C::kCpr>(r, piece);
-            cp16(dst + at, kb + __shfl_sync(0xffffffffu, ko, r), take);
-            cp16(dst + C::kHalf + at, vb + __shfl_sync(0xffffffffu, vo, r), take);
+            const uint32_t at = dst + C::at(r, piece);
+            cp16(at, kb + __shfl_sync(0xffffffffu, ko, r), take);
+            cp16(at + C::kHalf, vb + __shfl_sync(0xffffffffu, vo, r), take);
           }
         }
         if constexpr (!C::kWide) {
+          static_assert(C::kWide || G == 32, "a lane for each key's scales");
           const uint32_t pg = held ? page : 0, pr = held ? prow : 0;
-          cp4(dst + 2 * C::kHalf + 16 + lane * 4, sb + static_cast<uint64_t>(pg) * sc_sp + static_cast<uint64_t>(pr) * sc_ss, held);
+          const uint32_t at = dst + C::kOffWord + 16 + lane * 4;
+          cp4(at, ksb + static_cast<uint64_t>(pg) * static_cast<uint32_t>(a.pool.ks_sp) + static_cast<uint64_t>(pr) * static_cast<uint32_t>(a.pool.ks_ss), held);
+          cp4(at + 4 * G, vsb + static_cast<uint64_t>(pg) * static_cast<uint32_t>(a.pool.vs_sp) + static_cast<uint64_t>(pr) * static_cast<uint32_t>(a.pool.vs_ss), held);
         }
       }
-      const int unit = ahead.at - ahead.i;
-      more = ahead.next(a, end);
-      if (more) {
-        if (ahead.at - ahead.i != unit) enter();
-        look_up();
+      ++tile;
+      if (--left == 0) {
+        if (lane == 0) step_unit(a, &ahead, end);
+        __syncwarp();
+        if (ahead.at < end) enter();
+        __syncwarp();
       }
+      if (left > 0) look_up();
     }
     cp_commit();
   };
   enter();
   look_up();
-#pragma unroll
-  for (int s = 0; s < C::kStages; ++s) issue(s);
+#pragma unroll 1
+  for (int k = 0; k < C::kStages; ++k) issue(k);
 
-  // ---- this unit's state.  A thread's rows are nt * 8 + 2 c + {0, 1} for scores
+  // ---- the unit's state.  A thread's rows are nt * 8 + 2 c + {0, 1} for scores
   // and output, nt * 8 + g for Q.
   uint32_t qf[NT][D / 16][2];
   float o[NT][D / 16][4];
   float m[NT][2], l[NT][2], qscale[NT][2];
   int unit_exp = kNoExp;
-  bool fresh = true;            // the unit's state is to be set up
+  float unit_scale = 1.f;
   bool first_unit = true;
-  int tiles_done = 0, in_unit = min(cur.u.tiles - cur.i, end - cur.at);  // of the unit, in this CTA
-
-  auto sees = [&](int nt, int e, int j) -> bool {
-    const int pr = cur.qb * C::M + nt * 8 + 2 * c + e;
-    if (pr >= cur.s.c * a.group) return false;
-    const int t = pr / a.group, P = cur.s.P;
-    if (a.parents && j >= P) {
-      const int n = j - P;
-      return n < cur.s.c && ((s_bits[(t - cur.t0) * (kPagedMaxNodes / 32) + (n >> 5)] >> (n & 31)) & 1u);
-    }
-    const int pos = P + (a.parents ? s_depth[t - cur.t0] : t);
-    return j <= pos && (!a.window || j > pos - a.window || j < a.sinks);
-  };
-
   int stage = 0;
-  bool more_tiles = true;
-  while (more_tiles) {
-    if (fresh) {
-      fresh = false;
-      if (a.parents) {
-        __syncthreads();  // every warp is done with the last unit's bits
-        for (int k = threadIdx.x; k < C::M * (kPagedMaxNodes / 32); k += C::kThreads) s_bits[k] = 0;
-        __syncthreads();
-        for (int t = cur.t0 + threadIdx.x; t < cur.t1; t += C::kThreads)
-          s_depth[t - cur.t0] = tree_bits(a, cur.s, cur.b, t, s_bits + (t - cur.t0) * (kPagedMaxNodes / 32));
-        __syncthreads();
-      }
+  while (true) {
+    const int in_unit = min(cur.u.tiles - cur.i, end - cur.at);  // of the unit, in this CTA
+    if (a.parents) {
+      for (int k = threadIdx.x; k < C::M * (kPagedMaxNodes / 32); k += C::kThreads) s_bits[k] = 0;
+      __syncthreads();
+      for (int t = cur.t0 + threadIdx.x; t < cur.t1; t += C::kThreads)
+        s_depth[t - cur.t0] = tree_bits(a, cur.s, cur.b, t, s_bits + (t - cur.t0) * (kPagedMaxNodes / 32));
+      __syncthreads();
+    }
+    {
       const int R = cur.s.c * a.group;
       const int64_t first = a.nr.cu ? a.nr.cu[cur.b] : 0;
       const char* qb = a.q + (a.nr.cu ? 0 : cur.b * a.q_sb);
@@ -367,318 +437,343 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
           for (int e = 0; e < 4; ++e) o[nt][t2][e] = 0.f;
       }
       unit_exp = kNoExp;
+      unit_scale = pow2(6 - kNoExp);
     }
 
-    cp_wait<C::kStages - 1>();
-    __syncwarp();
-    uint8_t* st = ring + stage * C::kStage;
-    const uint32_t st_s = ring_s + stage * C::kStage;
-    const uint2 word = *reinterpret_cast<const uint2*>(st + 2 * C::kHalf);
-    const bool unit_done = word.x & kLast;
-    if (word.x & 0xffffu) {
-      const uint32_t valid = word.x;
-      const int j0 = static_cast<int>(word.y);
-      const bool plain = word.x & kPlain;
-      float x[NT][4];  // S^T: key g of row 2 c, of row 2 c + 1, key g + 8 of both
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[nt][e] = 0.f;
-      // ---- scores
-      if constexpr (C::kWide) {
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          uint32_t k[4];
-          ldsm4(k, st_s + piece_at<C::kCpr>(lane & 15, ks * 2 + (lane >> 4)));
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma(x[nt], k, qf[nt][ks][0], qf[nt][ks][1], X{});
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < D / 64; ++i) {
-          const uint4 w0 = *reinterpret_cast<const uint4*>(st + piece_at<C::kCpr>(g, c + 4 * i));
-          const uint4 w1 = *reinterpret_cast<const uint4*>(st + piece_at<C::kCpr>(g + 8, c + 4 * i));
-          const uint32_t u0[4] = {w0.x, w0.y, w0.z, w0.w}, u1[4] = {w1.x, w1.y, w1.z, w1.w};
-#pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            const uint32_t k[4] = {widen<ST, 0, 1>(u0[s], u0[s]), widen<ST, 0, 1>(u1[s], u1[s]), widen<ST, 2, 3>(u0[s], u0[s]),
-                                   widen<ST, 2, 3>(u1[s], u1[s])};
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma(x[nt], k, qf[nt][i * 4 + s][0], qf[nt][i * 4 + s][1], X{});
-          }
-        }
-      }
-      // ---- softmax
-      float vsc[2] = {1.f, 1.f}, ksc[2] = {1.f, 1.f};
-      float regrade = 1.f;
-      if constexpr (!C::kWide) {
-        const float* sc = reinterpret_cast<const float*>(st + 2 * C::kHalf + 16);
-        ksc[0] = sc[g];
-        ksc[1] = sc[g + 8];
-        vsc[0] = sc[16 + g];
-        vsc[1] = sc[24 + g];
-        float top = fmaxf(vsc[0], vsc[1]);  // (0 for keys that were not fetched)
-        if (__any_sync(0xffffffffu, (__float_as_int(top) >> 23) - 126 > unit_exp)) {
-#pragma unroll
-          for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-          const int e = (__float_as_int(top) >> 23) - 126;  // top < 2^e
-          if (e > unit_exp) {
-            regrade = unit_exp == kNoExp ? 0.f : pow2(unit_exp - e);
-            unit_exp = e;
-          }
-        }
-        const float f = pow2(6 - unit_exp);
-        vsc[0] *= f;
-        vsc[1] *= f;
-      }
-      bool move = regrade != 1.f;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[nt][e] *= qscale[nt][e & 1] * ksc[e >> 1];
-          if (!plain) {
-            const int k = g + 8 * (e >> 1);
-            if (!((valid >> k) & 1u) || !sees(nt, e & 1, j0 + k)) x[nt][e] = -INFINITY;
-          }
-          move |= x[nt][e] > m[nt][e & 1] + 8.f;
-        }
-      // The running max moves only when a score exceeds it by 8 (log2 units), so
-      // the usual group needs no shuffles and no rescaling.
-      if (__any_sync(0xffffffffu, move)) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float alpha[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(m[nt][e], fmaxf(x[nt][e], x[nt][e + 2]));
-#pragma unroll
-            for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-            alpha[e] = ex2(m[nt][e] - (top == -INFINITY ? 0.f : top));
-            m[nt][e] = top;
-            l[nt][e] *= alpha[e];
-            alpha[e] *= regrade;
-          }
-#pragma unroll
-          for (int t = 0; t < D / 16; ++t) {
-            o[nt][t][0] *= alpha[0];
-            o[nt][t][1] *= alpha[1];
-            o[nt][t][2] *= alpha[0];
-            o[nt][t][3] *= alpha[1];
-          }
-        }
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float base = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
-          x[nt][e] = ex2(x[nt][e] - base);
-          x[nt][e + 2] = ex2(x[nt][e + 2] - base);
-          l[nt][e] += x[nt][e] + x[nt][e + 2];
-        }
-      // ---- a partly hidden group of 16-bit rows: 0 * infinity must not reach a row that does not see it
-      bool slow = false;
-      if constexpr (C::kWide) {
-        if (!plain) {
-          bool odd = false;
-          for (int it = lane; it < G * C::kCpr; it += 32) {
-            const uint4 w = *reinterpret_cast<const uint4*>(st + C::kHalf + it * 16);
-            constexpr uint32_t top = std::is_same_v<T, __half> ? 0x7c00u : 0x7f80u;
-            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) odd |= (ww[e] & top) == top || ((ww[e] >> 16) & top) == top;
-          }
-          slow = __any_sync(0xffffffffu, odd);
-        }
-      }
-      // ---- output rows
-      if (C::kWide && slow) {
-        // One key at a time on the CUDA cores.  The weights go over the K rows, which are done with.
-        float* w = reinterpret_cast<float*>(st);
-        static_assert(!C::kWide || C::M * G * 4 <= C::kHalf, "weights fit the K block");
-        __syncwarp();
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int k = g + 8 * (e >> 1);
-            const bool on = ((valid >> k) & 1u) && sees(nt, e & 1, j0 + k);
-            w[(nt * 8 + 2 * c + (e & 1)) * G + k] = on ? x[nt][e] : -1.f;
-          }
-        __syncwarp();
 #pragma unroll 1
-        for (int k = 0; k < G; ++k)
+    for (int done = 0; done < in_unit; ++done) {
+      uint8_t* st = ring + stage * C::kStage;
+      const uint32_t st_s = ring_s + stage * C::kStage;
+      cp_wait<C::kStages - 1>();
+      __syncwarp();
+      const uint2 word = *reinterpret_cast<const uint2*>(st + C::kOffWord);
+      if (word.x) {
+        const uint32_t valid = word.x;
+        const int j0 = static_cast<int>(word.y & ~kPlain);
+        const bool plain = word.y & kPlain;
+        float x[KB][NT][4];  // S^T of a block: key g of row 2 c, of row 2 c + 1, key g + 8 of both
 #pragma unroll
-          for (int t = 0; t < D / 16; ++t)
+        for (int b = 0; b < KB; ++b)
 #pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-              const float v = Cvt<T>::to_f(*(reinterpret_cast<const T*>(st + C::kHalf + piece_at<C::kCpr>(k, 2 * t + hh)) + g));
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const float p = w[(nt * 8 + 2 * c + e) * G + k];
-                  if (!(p < 0.f)) o[nt][t][2 * hh + e] = fmaf(p, v, o[nt][t][2 * hh + e]);
-                }
-            }
-      } else {
-        uint32_t pf[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            float p0 = x[nt][2 * hh], p1 = x[nt][2 * hh + 1];
-            if constexpr (!C::kWide) {
-              p0 *= vsc[hh];
-              p1 *= vsc[hh];
-              if (!plain) {  // a hidden key's weight is 0 whatever its scale
-                p0 = x[nt][2 * hh] == 0.f ? 0.f : p0;
-                p1 = x[nt][2 * hh + 1] == 0.f ? 0.f : p1;
-              }
-            }
-            pf[nt][hh] = transpose8(pack2(p0, p1, X{}));
-          }
+            for (int e = 0; e < 4; ++e) x[b][nt][e] = 0.f;
+        // ---- scores
         if constexpr (C::kWide) {
 #pragma unroll
-          for (int t = 0; t < D / 16; ++t) {
-            uint32_t v[4];
-            ldsm4t(v, st_s + C::kHalf + piece_at<C::kCpr>((lane & 7) + ((lane >> 4) << 3), t * 2 + ((lane >> 3) & 1)));
+          for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma(o[nt][t], v, pf[nt][0], pf[nt][1], X{});
-          }
+            for (int b = 0; b < KB; ++b) {
+              uint32_t k[4];
+              ldsm4(k, st_s + C::at(b * 16 + (lane & 15), ks * 2 + (lane >> 4)));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma(x[b][nt], k, qf[nt][ks][0], qf[nt][ks][1], X{});
+            }
         } else {
-          uint32_t w[4][D / 32];  // keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9: D / 8 values from g on
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int key = (k >> 1) * 8 + 2 * c + (k & 1);
-            if constexpr (D == 128) {
-              const uint4 r = *reinterpret_cast<const uint4*>(st + C::kHalf + piece_at<C::kCpr>(key, g));
-              w[k][0] = r.x;
-              w[k][1] = r.y;
-              w[k][2] = r.z;
-              w[k][3] = r.w;
-            } else {
-              const uint2 r = *reinterpret_cast<const uint2*>(st + C::kHalf + piece_at<C::kCpr>(key, g >> 1) + (g & 1) * 8);
-              w[k][0] = r.x;
-              w[k][1] = r.y;
+          for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+              const uint4 w0 = *reinterpret_cast<const uint4*>(st + C::at(b * 16 + g, c + 4 * i));
+              const uint4 w1 = *reinterpret_cast<const uint4*>(st + C::at(b * 16 + g + 8, c + 4 * i));
+              const uint32_t u0[4] = {w0.x, w0.y, w0.z, w0.w}, u1[4] = {w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+              for (int s = 0; s < 4; ++s) {
+                uint32_t k[4];
+                widen_word<ST>(u0[s], k[0], k[2]);
+                widen_word<ST>(u1[s], k[1], k[3]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma(x[b][nt], k, qf[nt][i * 4 + s][0], qf[nt][i * 4 + s][1], X{});
+              }
+            }
+        }
+        // ---- softmax
+        const float* sc = reinterpret_cast<const float*>(st + C::kOffWord + 16);
+        float vsc[KB][2];
+        float regrade = 1.f;
+        if constexpr (!C::kWide) {
+          float top = 0.f;
+#pragma unroll
+          for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+              vsc[b][hh] = sc[G + b * 16 + hh * 8 + g];  // (0 for keys that were not fetched)
+              top = fmaxf(top, vsc[b][hh]);
+            }
+          if (__any_sync(0xffffffffu, __float_as_int(top) >= (unit_exp + 126) << 23)) {
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+            const int e = (__float_as_int(top) >> 23) - 126;  // top < 2^e
+            if (e > unit_exp) {
+              regrade = unit_exp == kNoExp ? 0.f : pow2(unit_exp - e);
+              unit_exp = e;
+              unit_scale = pow2(6 - e);
             }
           }
+        }
+        bool move = regrade != 1.f;
 #pragma unroll
-          for (int q = 0; q < D / 32; ++q) {
-            const uint32_t v0[4] = {widen<ST, 0, 4>(w[0][q], w[1][q]), widen<ST, 1, 5>(w[0][q], w[1][q]), widen<ST, 0, 4>(w[2][q], w[3][q]),
-                                    widen<ST, 1, 5>(w[2][q], w[3][q])};
-            const uint32_t v1[4] = {widen<ST, 2, 6>(w[0][q], w[1][q]), widen<ST, 3, 7>(w[0][q], w[1][q]), widen<ST, 2, 6>(w[2][q], w[3][q]),
-                                    widen<ST, 3, 7>(w[2][q], w[3][q])};
+        for (int b = 0; b < KB; ++b) {
+          const float k0 = C::kWide ? 1.f : sc[b * 16 + g], k1 = C::kWide ? 1.f : sc[b * 16 + 8 + g];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma(o[nt][2 * q], v0, pf[nt][0], pf[nt][1], X{});
-              mma(o[nt][2 * q + 1], v1, pf[nt][0], pf[nt][1], X{});
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              x[b][nt][e] *= C::kWide ? qscale[nt][e & 1] : qscale[nt][e & 1] * (e < 2 ? k0 : k1);
+        }
+        uint32_t hidden[KB] = {};
+        if (!plain) {
+#pragma unroll
+          for (int b = 0; b < KB; ++b) {
+            const int k0 = b * 16 + g;
+            hidden[b] = hidden_scores(a, &cur, s_bits, s_depth, cur.qb * C::M + 2 * c, NT, j0 + k0, j0 + k0 + 8, (valid >> k0) & 1u,
+                                      (valid >> (k0 + 8)) & 1u);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if ((hidden[b] >> (4 * nt + e)) & 1u) x[b][nt][e] = -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = fmaxf(x[0][nt][e], x[0][nt][e + 2]);
+            if constexpr (KB == 2) top = fmaxf(top, fmaxf(x[KB - 1][nt][e], x[KB - 1][nt][e + 2]));
+            move |= top > m[nt][e] + 8.f;
+          }
+        // The running max moves only when a score exceeds it by 8 (log2 units), so
+        // the usual group needs no shuffles and no rescaling.
+        if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float alpha[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float top = m[nt][e];
+#pragma unroll
+              for (int b = 0; b < KB; ++b) top = fmaxf(top, fmaxf(x[b][nt][e], x[b][nt][e + 2]));
+#pragma unroll
+              for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+              alpha[e] = ex2(m[nt][e] - (top == -INFINITY ? 0.f : top));
+              m[nt][e] = top;
+              l[nt][e] *= alpha[e];
+              alpha[e] *= regrade;
+            }
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) {
+              o[nt][t][0] *= alpha[0];
+              o[nt][t][1] *= alpha[1];
+              o[nt][t][2] *= alpha[0];
+              o[nt][t][3] *= alpha[1];
+            }
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float base = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+              x[b][nt][e] = ex2(x[b][nt][e] - base);
+              x[b][nt][e + 2] = ex2(x[b][nt][e + 2] - base);
+              l[nt][e] += x[b][nt][e] + x[b][nt][e + 2];
+            }
+          }
+        // ---- a partly hidden group of 16-bit rows: 0 * infinity must not reach a row that does not see it
+        bool slow = false;
+        if constexpr (C::kWide) {
+          if (!plain) {
+            bool odd = false;
+            for (int it = lane; it < G * C::kCpr; it += 32) {
+              const uint4 w = *reinterpret_cast<const uint4*>(st + C::kHalf + it * 16);
+              constexpr uint32_t top = std::is_same_v<T, __half> ? 0x7c00u : 0x7f80u;
+              const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) odd |= (ww[e] & top) == top || ((ww[e] >> 16) & top) == top;
+            }
+            slow = __any_sync(0xffffffffu, odd);
+          }
+        }
+        // ---- output rows
+        if (C::kWide && slow) {
+          // One key at a time on the CUDA cores.  The weights go over the K rows, which are done with.
+          float* w = reinterpret_cast<float*>(st);
+          static_assert(!C::kWide || C::M * G * 4 <= C::kHalf, "weights fit the K block");
+          __syncwarp();
+#pragma unroll
+          for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[(nt * 8 + 2 * c + (e & 1)) * G + b * 16 + g + 8 * (e >> 1)] =
+                    (hidden[b] >> (4 * nt + e)) & 1u ? -1.f : x[b][nt][e];
+          __syncwarp();
+#pragma unroll 1
+          for (int k = 0; k < G; ++k)
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+              for (int hh = 0; hh < 2; ++hh) {
+                const float v = Cvt<T>::to_f(*(reinterpret_cast<const T*>(st + C::kHalf + C::at(k, 2 * t + hh)) + g));
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    const float p = w[(nt * 8 + 2 * c + e) * G + k];
+                    if (!(p < 0.f)) o[nt][t][2 * hh + e] = fmaf(p, v, o[nt][t][2 * hh + e]);
+                  }
+              }
+        } else {
+#pragma unroll
+          for (int b = 0; b < KB; ++b) {
+            uint32_t pf[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int hh = 0; hh < 2; ++hh) {
+                float p0 = x[b][nt][2 * hh], p1 = x[b][nt][2 * hh + 1];
+                if constexpr (!C::kWide) {
+                  const float f = vsc[b][hh] * unit_scale;
+                  // (a hidden key's weight is 0 whatever its scale)
+                  p0 = !plain && p0 == 0.f ? 0.f : p0 * f;
+                  p1 = !plain && p1 == 0.f ? 0.f : p1 * f;
+                }
+                pf[nt][hh] = transpose8(pack2(p0, p1, X{}));
+              }
+            if constexpr (C::kWide) {
+#pragma unroll
+              for (int t = 0; t < D / 16; ++t) {
+                uint32_t v[4];
+                ldsm4t(v, st_s + C::kHalf + C::at(b * 16 + (lane & 7) + ((lane >> 4) << 3), t * 2 + ((lane >> 3) & 1)));
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma(o[nt][t], v, pf[nt][0], pf[nt][1], X{});
+              }
+            } else {
+              uint32_t w[4][D / 32];  // keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9: D / 8 values from g on
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const int key = b * 16 + (k >> 1) * 8 + 2 * c + (k & 1);
+                if constexpr (D == 128) {
+                  const uint4 r = *reinterpret_cast<const uint4*>(st + C::kHalf + C::at(key, g));
+                  w[k][0] = r.x;
+                  w[k][1] = r.y;
+                  w[k][2] = r.z;
+                  w[k][3] = r.w;
+                } else {
+                  const uint2 r = *reinterpret_cast<const uint2*>(st + C::kHalf + C::at(key, g >> 1) + (g & 1) * 8);
+                  w[k][0] = r.x;
+                  w[k][1] = r.y;
+                }
+              }
+#pragma unroll
+              for (int q = 0; q < D / 32; ++q) {
+                const uint32_t v0[4] = {widen<ST, 0, 4>(w[0][q], w[1][q]), widen<ST, 1, 5>(w[0][q], w[1][q]),
+                                        widen<ST, 0, 4>(w[2][q], w[3][q]), widen<ST, 1, 5>(w[2][q], w[3][q])};
+                const uint32_t v1[4] = {widen<ST, 2, 6>(w[0][q], w[1][q]), widen<ST, 3, 7>(w[0][q], w[1][q]),
+                                        widen<ST, 2, 6>(w[2][q], w[3][q]), widen<ST, 3, 7>(w[2][q], w[3][q])};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  mma(o[nt][2 * q], v0, pf[nt][0], pf[nt][1], X{});
+                  mma(o[nt][2 * q + 1], v1, pf[nt][0], pf[nt][1], X{});
+                }
+              }
             }
           }
         }
       }
+      __syncwarp();  // every lane is done with the stage
+      issue(stage);
+      stage = stage + 1 == C::kStages ? 0 : stage + 1;
     }
-    __syncwarp();  // every lane is done with the stage
-    issue(stage);
-    stage = stage + 1 == C::kStages ? 0 : stage + 1;
 
     // ---- the end of the unit, or of the CTA's part of it
-    ++tiles_done;
-    if (unit_done || tiles_done == in_unit) {
-      const bool whole = unit_done && !cut_start;
-      const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (first_unit ? 0 : 1);
-      const int R = cur.s.c * a.group;
-      const int64_t first = a.nr.cu ? a.nr.cu[cur.b] : 0;
+    const bool unit_done = cur.i + in_unit == cur.u.tiles;
+    const bool whole = unit_done && !cut_start;
+    const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (first_unit ? 0 : 1);
+    const int R = cur.s.c * a.group;
+    const int64_t first = a.nr.cu ? a.nr.cu[cur.b] : 0;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < 2; ++e) {
 #pragma unroll
-          for (int w = 4; w < 32; w <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], w);
-          if (g == 0) s_ml[warp * C::M + nt * 8 + 2 * c + e] = make_float2(m[nt][e], l[nt][e]);
-        }
-      __syncthreads();
-      if (threadIdx.x < C::M) {
-        float top = -INFINITY, L = 0.f;
-#pragma unroll
-        for (int w = 0; w < C::kWarps; ++w) top = fmaxf(top, s_ml[w * C::M + threadIdx.x].x);
-#pragma unroll
-        for (int w = 0; w < C::kWarps; ++w) {
-          const float2 y = s_ml[w * C::M + threadIdx.x];
-          L += y.x == -INFINITY ? y.y : y.y * ex2(y.x - top);  // (a warp that met only NaN has its sum alone)
-        }
-        s_row[threadIdx.x] = make_float2(top, L);
+        for (int w = 4; w < 32; w <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], w);
+        if (g == 0) s_ml[warp * C::M + nt * 8 + 2 * c + e] = make_float2(m[nt][e], l[nt][e]);
       }
-      __syncthreads();
+    __syncthreads();
+    if (threadIdx.x < C::M) {
+      float top = -INFINITY, L = 0.f;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int rows = min(8, R - cur.qb * C::M - nt * 8);
-        if (rows <= 0) break;
+      for (int w = 0; w < C::kWarps; ++w) top = fmaxf(top, s_ml[w * C::M + threadIdx.x].x);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float f = ex2(m[nt][e] - s_row[nt * 8 + 2 * c + e].x);
-          if constexpr (!C::kWide) f *= pow2(unit_exp - 6);
+      for (int w = 0; w < C::kWarps; ++w) {
+        const float2 y = s_ml[w * C::M + threadIdx.x];
+        L += y.x == -INFINITY ? y.y : y.y * ex2(y.x - top);  // (a warp that met only NaN has its sum alone)
+      }
+      s_row[threadIdx.x] = make_float2(top, L);
+    }
+    __syncthreads();
 #pragma unroll
-          for (int t = 0; t < D / 16; ++t) {
-            o[nt][t][e] = m[nt][e] == -INFINITY ? 0.f : o[nt][t][e] * f;  // (nothing seen: weight 0)
-            o[nt][t][e + 2] = m[nt][e] == -INFINITY ? 0.f : o[nt][t][e + 2] * f;
-          }
-        }
-        // as many tiles of 16 columns per pass as fit the buffer for the rows in use
-        const int rp = rows <= 4 ? 4 : 8;
-        const int tiles = min(D / 16, (kRedFloats / (C::kWarps * rp) - 4) / 16);
-        const int pitch = tiles * 16 + 4;
-        for (int p0 = 0; p0 < D / 16; p0 += tiles) {
+    for (int nt = 0; nt < NT; ++nt) {
+      const int rows = min(8, R - cur.qb * C::M - nt * 8);
+      if (rows <= 0) break;
 #pragma unroll
-          for (int t = 0; t < D / 16; ++t) {
-            if (t < p0 || t >= p0 + tiles || 2 * c >= rp) continue;
-            float* at = s_red + (warp * rp + 2 * c) * pitch + (t - p0) * 16 + g;
-            at[0] = o[nt][t][0];
-            at[pitch] = o[nt][t][1];
-            at[8] = o[nt][t][2];
-            at[pitch + 8] = o[nt][t][3];
-          }
-          __syncthreads();
-          const int cols = min(tiles, D / 16 - p0) * 16;
-          for (int e = threadIdx.x; e < rows * cols; e += C::kThreads) {
-            const int r = e / cols, v = e - r * cols;
-            float sum = 0.f;
+      for (int e = 0; e < 2; ++e) {
+        float f = ex2(m[nt][e] - s_row[nt * 8 + 2 * c + e].x);
+        if constexpr (!C::kWide) f *= pow2(unit_exp - 6);
 #pragma unroll
-            for (int w = 0; w < C::kWarps; ++w) sum += s_red[(w * rp + r) * pitch + v];
-            const int t = p0 + (v >> 4);
-            const int d = C::kWide ? t * 16 + (v & 15) : (v & 7) * (D / 8) + 2 * t + ((v >> 3) & 1);
-            const int row = nt * 8 + r;
-            const float top = s_row[row].x, L = s_row[row].y;
-            if (whole) {
-              const int pr = cur.qb * C::M + row, tt = pr / a.group, h = cur.kvh * a.group + pr - tt * a.group;
-              T* out = reinterpret_cast<T*>(a.out) + (a.nr.cu ? 0 : cur.b * a.o_sb) + h * a.o_sh + (first + tt) * a.o_sn;
-              out[d] = Cvt<T>::from_f(sum * (1.f / L));
-              if (a.lse && d == 0)
-                a.lse[(a.nr.cu ? 0 : cur.b * a.l_sb) + h * a.l_sh + (first + tt) * a.l_sn] = (top + log2f(L)) * 0.6931471805599453f;
-            } else {
-              a.part_o[(slot * C::M + row) * D + d] = sum;
-              if (d == 0) a.part_ml[slot * C::M + row] = make_float2(top, L);
-            }
-          }
-          __syncthreads();
+        for (int t = 0; t < D / 16; ++t) {
+          o[nt][t][e] = m[nt][e] == -INFINITY ? 0.f : o[nt][t][e] * f;  // (nothing seen: weight 0)
+          o[nt][t][e + 2] = m[nt][e] == -INFINITY ? 0.f : o[nt][t][e + 2] * f;
         }
       }
-      __syncthreads();  // s_ml and s_row are read by every warp before the next unit writes them
-      fresh = true;
-      first_unit = cut_start = false;
-      TileCursor n = cur;
-      n.at += n.u.tiles - 1 - n.i;
-      n.i = n.u.tiles - 1;
-      more_tiles = unit_done && n.next(a, end);
-      __syncwarp();
-      if (more_tiles && lane == 0) cur = n;
-      __syncwarp();
-      if (more_tiles) {
-        tiles_done = 0;
-        in_unit = min(cur.u.tiles, end - cur.at);
+      // as many tiles of 16 columns per pass as fit the buffer for the rows in use
+      const int rp = rows <= 4 ? 4 : 8;
+      const int tiles = min(D / 16, (kRedFloats / (C::kWarps * rp) - 4) / 16);
+      const int pitch = tiles * 16 + 4;
+      for (int p0 = 0; p0 < D / 16; p0 += tiles) {
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) {
+          if (t < p0 || t >= p0 + tiles || 2 * c >= rp) continue;
+          float* at = s_red + (warp * rp + 2 * c) * pitch + (t - p0) * 16 + g;
+          at[0] = o[nt][t][0];
+          at[pitch] = o[nt][t][1];
+          at[8] = o[nt][t][2];
+          at[pitch + 8] = o[nt][t][3];
+        }
+        __syncthreads();
+        const int cols = min(tiles, D / 16 - p0) * 16;
+        for (int e = threadIdx.x; e < rows * cols; e += C::kThreads) {
+          const int r = e / cols, v = e - r * cols;
+          float sum = 0.f;
+#pragma unroll
+          for (int w = 0; w < C::kWarps; ++w) sum += s_red[(w * rp + r) * pitch + v];
+          const int t = p0 + (v >> 4);
+          const int d = C::kWide ? t * 16 + (v & 15) : (v & 7) * (D / 8) + 2 * t + ((v >> 3) & 1);
+          const int row = nt * 8 + r;
+          const float top = s_row[row].x, L = s_row[row].y;
+          if (whole) {
+            const int pr = cur.qb * C::M + row, tt = pr / a.group, h = cur.kvh * a.group + pr - tt * a.group;
+            T* out = reinterpret_cast<T*>(a.out) + (a.nr.cu ? 0 : cur.b * a.o_sb) + h * a.o_sh + (first + tt) * a.o_sn;
+            out[d] = Cvt<T>::from_f(sum * (1.f / L));
+            if (a.lse && d == 0)
+              a.lse[(a.nr.cu ? 0 : cur.b * a.l_sb) + h * a.l_sh + (first + tt) * a.l_sn] = (top + log2f(L)) * 0.6931471805599453f;
+          } else {
+            a.part_o[(slot * C::M + row) * D + d] = sum;
+            if (d == 0) a.part_ml[slot * C::M + row] = make_float2(top, L);
+          }
+        }
+        __syncthreads();
       }
     }
+    first_unit = cut_start = false;
+    if (threadIdx.x == 0) step_unit(a, &cur, end);
+    __syncthreads();  // (the rows' maxima and sums, too, are read before the next unit writes them)
+    if (cur.at >= end) break;
   }
   cp_wait<0>();
 }
@@ -686,7 +781,7 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
 template <typename T, int ST, int D, int NT>
 int launch_t(const PagedAttn& a, cudaStream_t st) {
   using C = Cfg<T, ST, D, NT>;
-  static_assert(C::kSmem <= 233472 / kCtasPerSm - 1024 - 288, "shared memory per block");
+  static_assert(C::kSmem <= 233472 / kCtasPerSm - 1024, "shared memory per block");
   auto kern = paged_mma_kernel<T, ST, D, NT>;
   int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem),
                       "gorgon_paged_attn smem attribute");
