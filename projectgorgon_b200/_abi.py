@@ -33,7 +33,7 @@ ERR_CAND_CAPACITY = 1 << 5
 ERR_BAD_PAGE = 1 << 6
 
 KV_NATIVE, KV_INT8, KV_E4M3 = 0, 1, 2
-PAGED_AUTO, PAGED_SIMT, PAGED_MMA = 0, 1, 2
+PAGED_AUTO, PAGED_SIMT, PAGED_MMA, PAGED_TCGEN05 = 0, 1, 2, 3
 
 
 class TreeAttnParams(Structure):

@@ -22,7 +22,7 @@ INCLUDE = PKG.parent / "include"
 
 SOURCES = ["abi.cu", "tree_mask.cu", "attn_api.cu", "attn_simt.cu", "attn_tc.cu", "attn_pair.cu",
            "verify.cu", "kv_trim.cu", "cand_tree.cu", "paged_cache.cu", "paged_attn_api.cu", "paged_attn_simt.cu",
-           "paged_attn_mma.cu"]
+           "paged_attn_mma.cu", "paged_attn_tc.cu"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--expt-relaxed-constexpr",

@@ -295,5 +295,9 @@ int launch_paged_merge(const PagedAttn& a, cudaStream_t st);
 bool paged_mma_supported(const PagedAttn& a);
 void paged_mma_plan(PagedAttn* a);
 int launch_paged_mma(const PagedAttn& a, cudaStream_t st);
+// tcgen05 kernel for many.
+bool paged_tc_supported(const PagedAttn& a);
+void paged_tc_plan(PagedAttn* a);
+int launch_paged_tc(const PagedAttn& a, cudaStream_t st);
 
 }  // namespace gorgon

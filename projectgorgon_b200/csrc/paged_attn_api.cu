@@ -25,7 +25,7 @@ int make_args(const gorgon_paged_attn_params* p, PagedAttn* a) {
     return set_error(GORGON_ERR_UNSUPPORTED, "gorgon_paged_attn: a tree needs n rows in every sequence (no cu_q)");
   if (p->cu_q && (p->rows < 0 || p->rows > INT32_MAX))
     return set_error(GORGON_ERR_INVALID, "gorgon_paged_attn: bad count of packed rows");
-  if (p->backend < GORGON_PAGED_AUTO || p->backend > GORGON_PAGED_MMA)
+  if (p->backend < GORGON_PAGED_AUTO || p->backend > GORGON_PAGED_TCGEN05)
     return set_error(GORGON_ERR_INVALID, "gorgon_paged_attn: unknown backend");
   if (p->kv.batch * p->heads_q * p->n * p->kv.head_dim > 0 && (!p->q || !p->out || !p->kv.seq_lens))
     return set_error(GORGON_ERR_INVALID, "gorgon_paged_attn: null q, out or seq_lens");
@@ -54,14 +54,18 @@ int make_args(const gorgon_paged_attn_params* p, PagedAttn* a) {
 
 bool empty(const PagedAttn& a) { return static_cast<int64_t>(a.pool.batch) * a.hq * a.n * a.pool.d == 0; }
 
-enum class Kernel { kSimt, kMma, kNone };
+enum class Kernel { kSimt, kMma, kTc, kNone };
 
 Kernel choose(const gorgon_paged_attn_params* p, const PagedAttn& a) {
   const bool mma = paged_mma_supported(a);
   switch (p->backend) {
     case GORGON_PAGED_SIMT: return Kernel::kSimt;
     case GORGON_PAGED_MMA: return mma ? Kernel::kMma : Kernel::kNone;
-    default: return mma ? Kernel::kMma : Kernel::kSimt;
+    case GORGON_PAGED_TCGEN05: return paged_tc_supported(a) ? Kernel::kTc : Kernel::kNone;
+    default:
+      // up to 16 packed rows fill one tile of the warp-level kernel
+      if (static_cast<int64_t>(a.n) * a.group > 16 && paged_tc_supported(a)) return Kernel::kTc;
+      return mma ? Kernel::kMma : Kernel::kSimt;
   }
 }
 
@@ -92,6 +96,9 @@ extern "C" size_t gorgon_paged_attn_workspace_size(const gorgon_paged_attn_param
     case Kernel::kMma:
       paged_mma_plan(&a);
       return cut_workspace(a);
+    case Kernel::kTc:
+      paged_tc_plan(&a);
+      return cut_workspace(a);
     default: return 0;
   }
 }
@@ -104,17 +111,19 @@ extern "C" int gorgon_paged_attn(const gorgon_paged_attn_params* p, void* worksp
   if (rc) return rc;
   if (empty(a)) return GORGON_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  switch (choose(p, a)) {
+  const Kernel k = choose(p, a);
+  switch (k) {
     case Kernel::kSimt: return launch_paged_simt(a, st);
     case Kernel::kMma: paged_mma_plan(&a); break;
+    case Kernel::kTc: paged_tc_plan(&a); break;
     default:
       return set_error(GORGON_ERR_UNSUPPORTED, "gorgon_paged_attn: the requested kernel needs a 16-bit dtype, head_dim 64 or "
-                                               "128 and rows of whole 16-byte pieces");
+                                               "128, rows of whole 16-byte pieces and (tcgen05) trees of at most 256 rows");
   }
   if (!workspace || workspace_bytes < cut_workspace(a))
     return set_error(GORGON_ERR_WORKSPACE, "gorgon_paged_attn: workspace smaller than gorgon_paged_attn_workspace_size()");
   place_workspace(&a, workspace);
-  rc = launch_paged_mma(a, st);
+  rc = k == Kernel::kTc ? launch_paged_tc(a, st) : launch_paged_mma(a, st);
   if (rc) return rc;
   return launch_paged_merge(a, st);
 }

@@ -1,0 +1,807 @@
+// Paged attention for many packed rows per (sequence, kv head): prompt chunks,
+// draft trees.  tcgen05 products with TMEM accumulators.
+//
+// A unit is MT x 128 packed rows of one (sequence, kv head), row t * group + g;
+// a tile is 64 positions of its cache.  One CTA per SM walks its share of the
+// tile list (paged_attn.cuh).  Warp roles:
+//   warp 0        Q K^T issuer (one thread)
+//   warp 1        P V issuer (one thread); the warp allocates TMEM
+//   warps 2, 3    idle (they fill a warpgroup: registers go to the others)
+//   warps 4, 5    K producers, 32 rows of every tile each
+//   warps 6, 7    V producers
+//   warps 8 - 11  softmax and epilogue of M-tile 0, a thread per row
+//   warps 12 - 15 (MT = 2) of M-tile 1
+// The producers gather rows one by one (pages of any size and stride) with
+// 16-byte cp.async copies into the SW128 tiles that the products read; 8-bit
+// rows go to a ring of raw bytes first, and each producer widens its 32 rows
+// from there to f16, exactly (paged_widen.cuh), so that the products see the
+// stored numbers and the scales are applied in fp32: K's to the scores, V's to
+// the weights.  Rows that no row of the unit sees are not read; they are zeros.
+//
+// Softmax per row is owned by one thread (TMEM lane = row): no shuffles.  The
+// running max moves only when a tile's max exceeds it by more than 8 (log2
+// units), which bounds weights by 2^8 and makes corrections of O rare.  Tiles
+// that every row of the unit sees whole run a loop without masks.  In the
+// others a 64-bit word per row says which columns it sees, and their V rows
+// are searched for infinities and NaN (0 times those would reach every row):
+// the search replaces them by zeros, and the epilogue adds them to the rows
+// that do see them.
+//
+// Every mbarrier wait is bounded; a wait that runs out raises kErrTimeout, and
+// the CTA drains its copies and products, frees TMEM and returns.
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_tc_common.cuh"
+#include "paged_attn.cuh"
+#include "paged_widen.cuh"
+
+namespace gorgon {
+namespace {
+using namespace sm100;
+
+constexpr int kTile = 64;  // positions per tile
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kColS = 0;    // + (buf * MT + mt) * kTile
+constexpr uint32_t kColO = 256;  // + mt * D
+constexpr int kMaxTree = 256;    // tree rows (8 words of ancestor bits)
+
+template <typename T, int ST, int D_, int MT_>
+struct TcCfg {
+  static constexpr int D = D_, MT = MT_;
+  static constexpr bool kWide = ST == GORGON_KV_NATIVE;
+  using X = std::conditional_t<kWide, T, __half>;
+  static constexpr int kHalves = D / 64;                 // 128-byte column blocks of a row
+  static constexpr int M = MT * 128;
+  static constexpr int kThreads = 256 + MT * 128;
+  static constexpr uint32_t kQTile = kHalves * kQHalf;   // one M-tile of Q
+  static constexpr uint32_t kBlock = kTile * 128;        // 64 rows of one column block
+  static constexpr uint32_t kTileBytes = kHalves * kBlock;
+  static constexpr int kStages = kWide ? (MT == 2 ? 4 : 5) : 3;
+  static constexpr int kRawStages = kWide ? 0 : (MT == 2 ? 3 : 5);
+  static constexpr uint32_t kRawBytes = 32 * D;          // a producer's rows of a tile
+  static constexpr int kLag = kWide ? kStages - 2 : 0;   // tiles in flight behind the newest
+  static constexpr uint32_t kOffK = MT * kQTile;
+  static constexpr uint32_t kOffV = kOffK + kStages * kTileBytes;
+  static constexpr uint32_t kOffRaw = kOffV + kStages * kTileBytes;         // [4 producers][stages]
+  static constexpr uint32_t kOffMeta = kOffRaw + 4 * kRawStages * kRawBytes;  // [stages] Meta
+  static constexpr uint32_t kMetaBytes = kWide ? 16 : 16 + 8 * kTile;       // 2 words of valid keys, max V scale x 2; K and V scales
+  static constexpr uint32_t kOffBits = kOffMeta + kStages * kMetaBytes;     // [M][8] ancestor words
+  static constexpr uint32_t kOffQs = kOffBits + M * (kMaxTree / 32) * 4;    // [M] undoes Q's power of two
+  static constexpr uint32_t kOffBar = (kOffQs + M * 4 + 15) / 16 * 16;
+  static constexpr uint32_t kSmem = kOffBar + 512 + 1024;                   // + alignment slack
+  static_assert(kSmem <= 232448, "shared memory per block");
+};
+
+template <typename C>
+struct TcBars {
+  uint64_t k_full[C::kStages], k_empty[C::kStages], v_full[C::kStages], v_empty[C::kStages];
+  uint64_t q_full;
+  uint64_t s_full[2 * C::MT], p_full[2 * C::MT];  // buf * MT + mt
+  uint64_t p_free[2];
+  uint64_t drain[2];
+  uint32_t tmem_base;
+  int abort;
+  int odd;  // bit 0: infinities or NaN were taken out of partly hidden V rows, bit 1: of a tile with a bad page
+  ShareScratch sh;
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {
+  const int n = take ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <int N>
+struct Slot {  // ring position
+  uint32_t stage = 0, phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == N) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
+// The unit's positions that every row sees: [all_lo, all_hi], and the sinks.
+struct Common {
+  int all_hi, all_lo;
+  __device__ __forceinline__ Common(const PagedAttn& a, const TileCursor& c) {
+    all_hi = a.parents ? c.s.P - 1 : c.s.P + c.t0;
+    const int last = c.s.P + (a.parents ? c.s.c : c.t1) - 1;
+    all_lo = a.window ? max(0, last - a.window + 1) : 0;
+  }
+  __device__ __forceinline__ bool plain(const PagedAttn& a, int j0) const {
+    return j0 + kTile - 1 <= all_hi && (j0 >= all_lo || j0 + kTile <= a.sinks);
+  }
+};
+
+// Bits [lo, hi) of a 64-bit word, clipped to it.
+__device__ __forceinline__ uint64_t bit_range(int lo, int hi) {
+  lo = max(0, min(64, lo));
+  hi = max(0, min(64, hi));
+  if (lo >= hi) return 0;
+  const uint64_t up = hi == 64 ? ~0ull : (1ull << hi) - 1;
+  return up & ~((1ull << lo) - 1);
+}
+
+// ------------------------------------------------------------ producers
+// One of the two warps that fetch K (is_v 0) or V rows; `half` picks its 32 of a tile's rows.
+template <typename T, int ST, typename C>
+__device__ void produce(const PagedAttn& a, TileCursor cur, int end, uint8_t* smem, TcBars<C>* bars, int is_v, int half) {
+  const int lane = threadIdx.x & 31;
+  volatile int* abort = &bars->abort;
+  uint64_t* full = is_v ? bars->v_full : bars->k_full;
+  uint64_t* empty = is_v ? bars->v_empty : bars->k_empty;
+  uint8_t* ring = smem + (is_v ? C::kOffV : C::kOffK);
+  uint8_t* raw = smem + C::kOffRaw + (is_v * 2 + half) * C::kRawStages * C::kRawBytes;
+  const int64_t sp = is_v ? a.pool.v_sp : a.pool.k_sp, ss = is_v ? a.pool.v_ss : a.pool.k_ss, sh = is_v ? a.pool.v_sh : a.pool.k_sh;
+  const char* pages = is_v ? a.pool.v : a.pool.k;
+  constexpr int kRow = C::kWide ? C::D * 2 : C::D;       // bytes of a row
+  constexpr int kCpr = kRow / 16, kRpi = 32 / kCpr;
+  const int piece = lane % kCpr, rsub = lane / kCpr;
+
+  // The fetch runs ahead of the hand-over by kLag tiles (16-bit) or by the raw ring (8-bit).
+  constexpr int kAhead = C::kWide ? C::kLag : C::kRawStages - 1;
+  struct Held {  // of a fetched tile
+    uint32_t valid;
+    float ks, vs;
+    bool plain;
+  };
+  Held held[C::kWide ? C::kLag + 1 : C::kRawStages];
+  TileCursor f = cur;
+  bool more = true;
+  int f_tile = 0;             // tiles fetched
+  Slot<C::kStages> fs;        // (16-bit) the stage fetched into
+  auto fetch = [&](Held& h) -> bool {
+    if constexpr (C::kWide) {
+      if (!warp_wait(&empty[fs.stage], fs.phase ^ 1u, abort, a.wait_ns)) return false;
+    }
+    const int j0 = f.tile() * kTile + half * 32;
+    const int j = j0 + lane;
+    int page = -1, prow = 0;
+    if (f.u.wanted(j)) {
+      int col;
+      a.pool.split(j, col, prow);
+      page = __ldg(a.pool.table + static_cast<int64_t>(f.b) * a.pool.table_sb + col);
+      if (page < 0 || page >= a.pool.num_pages) {
+        raise_device_error(a.pool.err, kErrBadPage);
+        page = -1;
+      }
+    }
+    h.valid = __ballot_sync(0xffffffffu, page >= 0);
+    h.plain = Common(a, f).plain(a, f.tile() * kTile);
+    const int64_t off = page >= 0 ? page * sp + prow * ss : 0;
+    const char* base = pages + f.kvh * sh + piece * 16;
+#pragma unroll
+    for (int it = 0; it < 32 / kRpi; ++it) {
+      const int r = it * kRpi + rsub;
+      const int64_t o = __shfl_sync(0xffffffffu, off, r);
+      uint32_t at;
+      if constexpr (C::kWide)
+        at = smem_u32(ring + fs.stage * C::kTileBytes + (piece >> 3) * C::kBlock) + sw128(half * 32 + r, piece & 7);
+      else
+        at = smem_u32(raw + (f_tile % C::kRawStages) * C::kRawBytes) + r * kRow + piece * 16;
+      cp16(at, base + o, (h.valid >> r) & 1u);
+    }
+    cp_commit();
+    if constexpr (!C::kWide) {
+      h.ks = h.vs = 0.f;
+      if (is_v && page >= 0) {
+        h.ks = __ldg(a.pool.ks + page * a.pool.ks_sp + f.kvh * a.pool.ks_sh + prow * a.pool.ks_ss);
+        h.vs = __ldg(a.pool.vs + page * a.pool.vs_sp + f.kvh * a.pool.vs_sh + prow * a.pool.vs_ss);
+      }
+    }
+    if constexpr (C::kWide) fs.next();
+    ++f_tile;
+    more = f.next(a, end);
+    return true;
+  };
+  Slot<C::kStages> hs;  // the stage handed over
+  int done = 0;
+  // Hands tile `done` over: its copies have landed.
+  auto hand_over = [&](const Held& h) -> bool {
+    uint8_t* st = ring + hs.stage * C::kTileBytes;
+    __syncwarp();  // every lane's copies
+    if constexpr (!C::kWide) {
+      if (!warp_wait(&empty[hs.stage], hs.phase ^ 1u, abort, a.wait_ns)) return false;
+      const uint8_t* src = raw + (done % C::kRawStages) * C::kRawBytes;
+#pragma unroll
+      for (int it = 0; it < 32 / kRpi; ++it) {
+        const int r = it * kRpi + rsub;
+        const uint4 w = *reinterpret_cast<const uint4*>(src + r * kRow + piece * 16);
+        uint32_t x[8];
+        widen_word<ST>(w.x, x[0], x[1]);
+        widen_word<ST>(w.y, x[2], x[3]);
+        widen_word<ST>(w.z, x[4], x[5]);
+        widen_word<ST>(w.w, x[6], x[7]);
+        uint8_t* blk = st + (piece >> 2) * C::kBlock;
+        *reinterpret_cast<uint4*>(blk + sw128(half * 32 + r, (2 * piece) & 7)) = make_uint4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<uint4*>(blk + sw128(half * 32 + r, (2 * piece + 1) & 7)) = make_uint4(x[4], x[5], x[6], x[7]);
+      }
+    }
+    if (is_v) {
+      uint8_t* meta = smem + C::kOffMeta + hs.stage * C::kMetaBytes;
+      if (lane == 0) reinterpret_cast<uint32_t*>(meta)[half] = h.valid;
+      if constexpr (!C::kWide) {
+        float top = h.vs;  // (NaN never wins)
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (lane == 0) reinterpret_cast<float*>(meta)[2 + half] = top;
+        reinterpret_cast<float*>(meta + 16)[half * 32 + lane] = h.ks;
+        reinterpret_cast<float*>(meta + 16)[kTile + half * 32 + lane] = h.vs;
+      } else if (!(h.plain && h.valid == 0xffffffffu)) {
+        bool odd = false;
+#pragma unroll 1
+        for (int it = 0; it < 32 / kRpi; ++it) {
+          const int r = half * 32 + it * kRpi + rsub;
+          uint4* w = reinterpret_cast<uint4*>(st + (piece >> 3) * C::kBlock + sw128(r, piece & 7));
+          uint32_t x[4] = {w->x, w->y, w->z, w->w};
+          constexpr uint32_t top = std::is_same_v<T, __half> ? 0x7c00u : 0x7f80u;
+          bool here = false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if ((x[e] & top) == top) {
+              x[e] &= 0xffff0000u;
+              here = true;
+            }
+            if (((x[e] >> 16) & top) == top) {
+              x[e] &= 0xffffu;
+              here = true;
+            }
+          }
+          if (here) *w = make_uint4(x[0], x[1], x[2], x[3]);
+          odd |= here;
+        }
+        if (odd) atomicOr(&bars->odd, h.plain ? 2 : 1);
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&full[hs.stage]);
+    hs.next();
+    ++done;
+    return true;
+  };
+  bool ok = true;
+  while (ok && more && f_tile < kAhead) ok = fetch(held[f_tile % (kAhead + 1)]);
+  while (ok && more) {
+    ok = fetch(held[f_tile % (kAhead + 1)]);
+    if (!ok) break;
+    cp_wait<kAhead>();
+    ok = hand_over(held[done % (kAhead + 1)]);
+  }
+  cp_wait<0>();
+  while (ok && done < f_tile) ok = hand_over(held[done % (kAhead + 1)]);
+}
+
+// ------------------------------------------------------------ issuers
+template <typename C>
+__device__ void issue_scores(const PagedAttn& a, TileCursor cur, int end, uint8_t* smem, TcBars<C>* bars, uint32_t tmem, uint32_t fmt) {
+  volatile int* abort = &bars->abort;
+  const uint64_t q0 = umma_desc_sw128(smem_u32(smem), 16, 1024);
+  const uint64_t k0 = umma_desc_sw128(smem_u32(smem + C::kOffK), 16, 1024);
+  const uint32_t idesc = umma_idesc_f16(fmt, 128, kTile, 0, 0);
+  Slot<C::kStages> kr;
+  uint32_t i = 0, unit = 0;
+  bool ok = true;
+  while (ok) {
+    if (!spin_wait(&bars->q_full, unit & 1u, abort, a.wait_ns)) break;
+    ++unit;
+    const int n = min(cur.u.tiles - cur.i, end - cur.at);
+    for (int t = 0; t < n; ++t, ++i) {
+      if (!spin_wait(&bars->k_full[kr.stage], kr.phase, abort, a.wait_ns) ||
+          (i >= 2 && !spin_wait(&bars->p_free[i & 1u], ((i - 2) >> 1) & 1u, abort, a.wait_ns))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+#pragma unroll
+      for (int mt = 0; mt < C::MT; ++mt) {
+#pragma unroll
+        for (int ks = 0; ks < C::D / 16; ++ks)
+          umma_f16_ss(tmem + kColS + ((i & 1u) * C::MT + mt) * kTile,
+                      q0 + static_cast<uint64_t>((mt * C::kHalves + (ks >> 2)) * (kQHalf >> 4) + (ks & 3) * 2),
+                      k0 + static_cast<uint64_t>(kr.stage * (C::kTileBytes >> 4) + (ks >> 2) * (C::kBlock >> 4) + (ks & 3) * 2), idesc,
+                      ks > 0 ? 1u : 0u);
+        umma_commit(&bars->s_full[(i & 1u) * C::MT + mt]);
+      }
+      umma_commit(&bars->k_empty[kr.stage]);
+      kr.next();
+    }
+    cur.at += n - 1;
+    cur.i += n - 1;
+    if (!ok || !cur.next(a, end)) break;
+  }
+  umma_commit(&bars->drain[0]);
+  drain_wait(&bars->drain[0], 0);
+}
+
+template <typename C>
+__device__ void issue_outputs(const PagedAttn& a, TileCursor cur, int end, uint8_t* smem, TcBars<C>* bars, uint32_t tmem, uint32_t fmt) {
+  volatile int* abort = &bars->abort;
+  const uint64_t v0 = umma_desc_sw128(smem_u32(smem + C::kOffV), C::kBlock, 1024);
+  const uint32_t idesc = umma_idesc_f16(fmt, 128, C::D, 0, 1);
+  Slot<C::kStages> vr;
+  uint32_t i = 0;
+  bool ok = true;
+  while (ok) {
+    const int n = min(cur.u.tiles - cur.i, end - cur.at);
+    for (int t = 0; t < n && ok; ++t, ++i) {
+      const uint32_t buf = i & 1u;
+      if (!spin_wait(&bars->v_full[vr.stage], vr.phase, abort, a.wait_ns)) {
+        ok = false;
+        break;
+      }
+      for (int mt = 0; mt < C::MT; ++mt) {
+        if (!spin_wait(&bars->p_full[buf * C::MT + mt], (i >> 1) & 1u, abort, a.wait_ns)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int ks = 0; ks < kTile / 16; ++ks)
+          umma_f16_ts(tmem + kColO + mt * C::D, tmem + kColS + (buf * C::MT + mt) * kTile + ks * 8,
+                      v0 + static_cast<uint64_t>(vr.stage * (C::kTileBytes >> 4) + ks * (2048 >> 4)), idesc, (ks > 0 || t > 0) ? 1u : 0u);
+      }
+      if (!ok) break;
+      umma_commit(&bars->p_free[buf]);
+      umma_commit(&bars->v_empty[vr.stage]);
+      vr.next();
+    }
+    cur.at += n - 1;
+    cur.i += n - 1;
+    if (!ok || !cur.next(a, end)) break;
+  }
+  umma_commit(&bars->drain[1]);
+  drain_wait(&bars->drain[1], 0);
+}
+
+// ------------------------------------------------------------ softmax
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
+constexpr int kNoExp = -116;
+
+// Which columns of the tile at j0 the row sees.
+__device__ __forceinline__ uint64_t row_word(const PagedAttn& a, const TileCursor& c, int pos, bool ok, const uint32_t* bits, int j0) {
+  if (!ok) return 0;
+  const int P = c.s.P;
+  const int hi = a.parents ? P - 1 : pos;
+  uint64_t w = bit_range(0, hi - j0 + 1);
+  if (a.window) w &= bit_range(pos - a.window + 1 - j0, 64) | bit_range(0, a.sinks - j0);
+  if (a.parents && j0 + 64 > P) {  // its own tree's columns by its ancestor bits
+    const int o = j0 - P;          // the tile's first tree row (negative: the tree starts inside the tile)
+    const int words = (c.s.c + 31) >> 5;
+    auto word = [&](int k) -> uint64_t { return k >= 0 && k < words ? bits[k] : 0u; };
+    const int k = o >> 5, sh = o & 31;  // floor
+    uint64_t t = (word(k) | (word(k + 1) << 32)) >> sh;
+    if (sh) t |= word(k + 2) << (64 - sh);
+    w |= t;
+  }
+  return w;
+}
+
+template <typename T, int ST, typename C>
+__device__ void softmax(const PagedAttn& a, TileCursor cur, int end, uint8_t* smem, TcBars<C>* bars, uint32_t tmem) {
+  using X = typename C::X;
+  constexpr bool kScaleQ = !C::kWide && std::is_same_v<T, __nv_bfloat16>;
+  constexpr int MT = C::MT, D = C::D;
+  constexpr int kChunks = D / 8;          // 16-byte pieces of a 16-bit row
+  constexpr int kRows = 32 / kChunks;     // rows that a warp instruction covers
+  volatile int* abort = &bars->abort;
+  const int wg = (threadIdx.x >> 7) - 2;  // M-tile
+  const int wq = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
+  const int r = threadIdx.x & 127, qrow = wg * 128 + r;
+  const uint32_t lane_base = tmem + (static_cast<uint32_t>(wq * 32) << 16);
+  uint8_t* q_tile = smem + wg * C::kQTile;
+  uint32_t* s_bits = reinterpret_cast<uint32_t*>(smem + C::kOffBits);
+  float* s_qs = reinterpret_cast<float*>(smem + C::kOffQs);
+  constexpr int kWords = kMaxTree / 32;
+  const int chunk = lane % kChunks, rsub = lane / kChunks;
+  // a row of the warp's 32: 16-byte pieces in the SW128 order of Q
+  auto stage_row = [&](int rr, int j) -> uint8_t* {
+    return q_tile + (j >> 3) * kQHalf + sw128(static_cast<uint32_t>(wq * 32 + rr), static_cast<uint32_t>(j & 7));
+  };
+  const bool vec_out = (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0 && ((a.o_sb | a.o_sh | a.o_sn) & 7) == 0;
+  int64_t i = 0;
+  Slot<C::kStages> vr;
+  bool first_unit = true;
+  bool cut_start = cur.i > 0;
+  while (true) {
+    const int n = min(cur.u.tiles - cur.i, end - cur.at);
+    const int R = cur.s.c * a.group;
+    const int64_t first = a.nr.cu ? a.nr.cu[cur.b] : 0;
+    const int pr = cur.qb * C::M + qrow;
+    const bool row_ok = pr < R;
+    const int t = row_ok ? pr / a.group : cur.t0;
+    const int h = cur.kvh * a.group + (row_ok ? pr - t * a.group : 0);
+    // ---- Q rows -> shared memory; the previous unit's last product is complete
+    {
+      const char* qb = a.q + (a.nr.cu ? 0 : cur.b * a.q_sb) + first * a.q_sn + static_cast<int64_t>(cur.kvh) * a.group * a.q_sh;
+      const int p0 = cur.qb * C::M + wg * 128 + wq * 32;
+      constexpr int kBatch = 8;
+#pragma unroll 1
+      for (int k0 = 0; k0 < 32; k0 += kBatch * kRows) {
+        uint4 qv[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const int p = p0 + k0 + k * kRows + rsub;
+          const int tt = p / a.group, gg = p - tt * a.group;
+          qv[k] = p < R ? __ldg(reinterpret_cast<const uint4*>(qb + tt * a.q_sn + gg * a.q_sh) + chunk) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const int rr = k0 + k * kRows + rsub;
+          if constexpr (kScaleQ) {
+            uint32_t x[4] = {qv[k].x, qv[k].y, qv[k].z, qv[k].w};
+            uint32_t top = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = max(top, max((x[e] << 16) & 0x7f800000u, x[e] & 0x7f800000u));
+#pragma unroll
+            for (int o = 1; o < kChunks; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const int e2 = max(static_cast<int>(top >> 23) - 127, -100);
+            const float f = pow2i(8 - e2);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              x[e] = pack16x2(__uint_as_float(x[e] << 16) * f, __uint_as_float(x[e] & 0xffff0000u) * f, false);
+            qv[k] = make_uint4(x[0], x[1], x[2], x[3]);
+            if (chunk == 0) s_qs[wg * 128 + wq * 32 + rr] = pow2i(e2 - 8);
+          }
+          *reinterpret_cast<uint4*>(stage_row(rr, chunk)) = qv[k];
+        }
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->q_full);
+    }
+    // ---- this row's ancestor bits (each thread its own: rows of one node repeat the
+    // walk, but no barrier stands between warps that may give up a wait)
+    int pos = cur.s.P + t;
+    uint32_t* bits = s_bits + qrow * kWords;
+    if (a.parents && row_ok) {
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) bits[w] = 0;
+      pos = cur.s.P + tree_bits(a, cur.s, cur.b, t, bits);
+    }
+    const Common common(a, cur);
+    const float qs = a.scale_log2 * (kScaleQ ? s_qs[qrow] : 1.f);
+    float m_used = -INFINITY, l = 0.f;
+    int unit_exp = kNoExp;
+    float unit = pow2i(6 - kNoExp);
+    // One tile of this row: scores to weights against the lazy running max.
+    auto tile = [&](auto mask_tag, int j0, bool fresh) -> bool {
+      constexpr bool kMask = decltype(mask_tag)::value;
+      const uint32_t bi = static_cast<uint32_t>(i & 1) * MT + wg;
+      const uint8_t* meta = smem + C::kOffMeta + vr.stage * C::kMetaBytes;
+      if (!warp_wait(&bars->v_full[vr.stage], vr.phase, abort, a.wait_ns)) return false;
+      uint64_t vw = ~0ull;
+      if (kMask) vw = row_word(a, cur, pos, row_ok, bits, j0) & *reinterpret_cast<const uint64_t*>(meta);
+      if (!warp_wait(&bars->s_full[bi], static_cast<uint32_t>(i >> 1) & 1u, abort, a.wait_ns)) return false;
+      tc_fence_after();
+      const uint32_t s_addr = lane_base + kColS + bi * kTile;
+      float x[kTile];
+      {
+        uint32_t rr[2][32];
+        tmem_ld32(s_addr, rr[0]);
+        tmem_ld32(s_addr + 32, rr[1]);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < kTile; ++c) x[c] = __uint_as_float(rr[c >> 5][c & 31]);
+      }
+      if constexpr (!C::kWide) {
+        const float4* ks = reinterpret_cast<const float4*>(meta + 16);
+#pragma unroll
+        for (int c = 0; c < kTile / 4; ++c) {
+          const float4 f = ks[c];
+          x[4 * c] *= f.x;
+          x[4 * c + 1] *= f.y;
+          x[4 * c + 2] *= f.z;
+          x[4 * c + 3] *= f.w;
+        }
+      }
+      if (kMask) {
+        const uint32_t w[2] = {static_cast<uint32_t>(vw), static_cast<uint32_t>(vw >> 32)};
+#pragma unroll
+        for (int c = 0; c < kTile; ++c) x[c] = ((w[c >> 5] >> (c & 31)) & 1u) ? x[c] : -INFINITY;
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < kTile; c += 2) mx[(c >> 1) & 3] = fmax3(mx[(c >> 1) & 3], x[c], x[c + 1]);
+      const float tmax = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]) * qs;
+      float alpha = 1.f;
+      bool need = false;
+      if (fresh) {
+        m_used = tmax;
+      } else if (tmax > m_used + 8.f) {
+        alpha = ex2_approx(m_used - tmax);
+        m_used = tmax;
+        need = true;
+      }
+      l *= alpha;
+      if constexpr (!C::kWide) {
+        const float2 top2 = *reinterpret_cast<const float2*>(meta + 8);
+        const int e = (__float_as_int(fmaxf(top2.x, top2.y)) >> 23) - 126;
+        if (e > unit_exp) {
+          alpha *= unit_exp == kNoExp ? 0.f : pow2i(unit_exp - e);
+          unit_exp = e;
+          unit = pow2i(6 - e);
+          need = !fresh;
+        }
+      }
+      const float nmb = m_used == -INFINITY ? 0.f : -m_used;
+      const uint64_t qs2 = f2_pack(qs, qs), nmb2 = f2_pack(nmb, nmb);
+      uint64_t acc[4] = {0, 0, 0, 0};
+      uint32_t packed[kTile / 2];
+      const float4* vs = reinterpret_cast<const float4*>(meta + 16 + 4 * kTile);
+      const uint64_t unit2 = f2_pack(unit, unit);
+#pragma unroll
+      for (int c = 0; c < kTile; c += 4) {
+        float y[4];
+        f2_unpack(f2_fma(f2_pack(x[c], x[c + 1]), qs2, nmb2), y[0], y[1]);
+        f2_unpack(f2_fma(f2_pack(x[c + 2], x[c + 3]), qs2, nmb2), y[2], y[3]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = ex2_approx(y[e]);
+        uint64_t p0 = f2_pack(y[0], y[1]), p1 = f2_pack(y[2], y[3]);
+        acc[(c >> 1) & 3] = f2_add(acc[(c >> 1) & 3], p0);
+        acc[((c >> 1) + 1) & 3] = f2_add(acc[((c >> 1) + 1) & 3], p1);
+        if constexpr (!C::kWide) {
+          const float4 f = vs[c >> 2];
+          p0 = f2_mul(p0, f2_mul(f2_pack(f.x, f.y), unit2));
+          p1 = f2_mul(p1, f2_mul(f2_pack(f.z, f.w), unit2));
+          float z[4];
+          f2_unpack(p0, z[0], z[1]);
+          f2_unpack(p1, z[2], z[3]);
+          if (kMask) {  // a hidden key's weight is 0 whatever its scale
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[e] = y[e] == 0.f ? 0.f : z[e];
+          }
+          packed[c >> 1] = pack16x2(z[0], z[1], false);
+          packed[(c >> 1) + 1] = pack16x2(z[2], z[3], false);
+        } else {
+          packed[c >> 1] = pack16x2(y[0], y[1], std::is_same_v<X, __nv_bfloat16>);
+          packed[(c >> 1) + 1] = pack16x2(y[2], y[3], std::is_same_v<X, __nv_bfloat16>);
+        }
+      }
+      {
+        float s0, s1;
+        f2_unpack(f2_add(f2_add(acc[0], acc[1]), f2_add(acc[2], acc[3])), s0, s1);
+        l += s0 + s1;
+      }
+      if (__any_sync(0xffffffffu, need)) {
+        const int64_t pv = i - 1;
+        if (!warp_wait(&bars->p_free[pv & 1], static_cast<uint32_t>(pv >> 1) & 1u, abort, a.wait_ns)) return false;
+        tc_fence_after();
+        const uint32_t o_addr = lane_base + kColO + wg * D;
+#pragma unroll
+        for (int ch = 0; ch < D / 32; ++ch) {
+          uint32_t ov[32];
+          tmem_ld32(o_addr + ch * 32, ov);
+          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
+          tmem_st32(o_addr + ch * 32, ov);
+        }
+        tmem_wait_st();
+      }
+      tmem_st32(s_addr, packed);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->p_full[bi]);
+      vr.next();
+      return true;
+    };
+    for (int k = 0; k < n; ++k, ++i) {
+      const int j0 = cur.u.tile(cur.i + k) * kTile;
+      const bool plain = common.plain(a, j0);
+      bool whole_tile = plain;
+      if (plain) {
+        // (the valid words are read again under the mask; a plain tile lacks keys only where a page is bad)
+        if (!warp_wait(&bars->v_full[vr.stage], vr.phase, abort, a.wait_ns)) return;
+        whole_tile = *reinterpret_cast<const uint64_t*>(smem + C::kOffMeta + vr.stage * C::kMetaBytes) == ~0ull;
+      }
+      if (!(whole_tile ? tile(std::false_type(), j0, k == 0) : tile(std::true_type(), j0, k == 0))) return;
+    }
+    // ---- epilogue
+    const int64_t lastv = i - 1;
+    if (!warp_wait(&bars->p_free[lastv & 1], static_cast<uint32_t>(lastv >> 1) & 1u, abort, a.wait_ns)) return;
+    tc_fence_after();
+    const bool whole = cur.i + n == cur.u.tiles && !cut_start;
+    const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (first_unit ? 0 : 1);
+    const uint32_t o_addr = lane_base + kColO + wg * D;
+    const float back = C::kWide ? 1.f : pow2i(unit_exp - 6);
+    const float f = whole ? back / l : (m_used == -INFINITY ? 0.f : back);
+    const int odd = C::kWide ? *reinterpret_cast<volatile int*>(&bars->odd) : 0;
+    // Adds what the producers took out of partly hidden V rows to a row that sees
+    // it: columns [c0, c0 + 32), key by key from the pages.
+    auto put_back = [&](int c0, float (&v)[32]) {
+      for (int k = 0; k < n; ++k) {
+        const int j0 = cur.u.tile(cur.i + k) * kTile;
+        if (!(odd & 2) && common.plain(a, j0)) continue;
+        const uint64_t see = row_word(a, cur, pos, row_ok, bits, j0);
+        for (int j = j0; j < j0 + kTile; ++j) {
+          if (!((see >> (j - j0)) & 1ull) || !cur.u.wanted(j)) continue;
+          int col, prow;
+          a.pool.split(j, col, prow);
+          const int page = a.pool.page(cur.b, col);
+          if (page < 0) continue;
+          const T* src = reinterpret_cast<const T*>(a.pool.v + page * a.pool.v_sp + cur.kvh * a.pool.v_sh + prow * a.pool.v_ss) + c0;
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const float y = Cvt<T>::to_f(src[c]);
+            if (!(fabsf(y) < INFINITY)) v[c] += y;
+          }
+        }
+      }
+    };
+    T* out = reinterpret_cast<T*>(a.out) + (a.nr.cu ? 0 : cur.b * a.o_sb);
+    float* part = a.part_o + (slot * C::M + qrow) * D;
+#pragma unroll
+    for (int ch = 0; ch < D / 32; ++ch) {
+      uint32_t ov[32];
+      tmem_ld32(o_addr + ch * 32, ov);
+      tmem_wait_ld();
+      float v[32];
+#pragma unroll
+      for (int c = 0; c < 32; ++c) v[c] = m_used == -INFINITY && !whole ? 0.f : __uint_as_float(ov[c]) * f;
+      if (odd) put_back(ch * 32, v);
+      if (!whole) {
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) *reinterpret_cast<float4*>(part + ch * 32 + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+      } else if (vec_out) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = pack16x2(v[8 * u + 2 * e], v[8 * u + 2 * e + 1], std::is_same_v<T, __nv_bfloat16>);
+          *reinterpret_cast<uint4*>(stage_row(lane, ch * 4 + u)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      } else if (row_ok) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) out[h * a.o_sh + (first + t) * a.o_sn + ch * 32 + c] = Cvt<T>::from_f(v[c]);
+      }
+    }
+    if (whole) {
+      if (vec_out) {
+        __syncwarp();
+        const int p0 = cur.qb * C::M + wg * 128 + wq * 32;
+        T* ob = out + first * a.o_sn + static_cast<int64_t>(cur.kvh) * a.group * a.o_sh + chunk * 8;
+#pragma unroll 4
+        for (int k = 0; k < 32; k += kRows) {
+          const int p = p0 + k + rsub;
+          const int tt = p / a.group, gg = p - tt * a.group;
+          const uint4 w = *reinterpret_cast<const uint4*>(stage_row(k + rsub, chunk));
+          if (p < R) *reinterpret_cast<uint4*>(ob + tt * a.o_sn + gg * a.o_sh) = w;
+        }
+        __syncwarp();
+      }
+      if (row_ok && a.lse)
+        a.lse[(a.nr.cu ? 0 : cur.b * a.l_sb) + h * a.l_sh + (first + t) * a.l_sn] = (m_used + log2f(l)) * 0.6931471805599453f;
+    } else {
+      a.part_ml[slot * C::M + qrow] = make_float2(m_used, l);
+    }
+    first_unit = cut_start = false;
+    cur.at += n - 1;
+    cur.i += n - 1;
+    if (!cur.next(a, end)) return;
+  }
+}
+
+template <typename T, int ST, int D, int MT>
+__global__ void __launch_bounds__(TcCfg<T, ST, D, MT>::kThreads, 1) paged_tc_kernel(const __grid_constant__ PagedAttn a) {
+  using C = TcCfg<T, ST, D, MT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  TcBars<C>* bars = reinterpret_cast<TcBars<C>*>(smem + C::kOffBar);
+  static_assert(sizeof(TcBars<C>) <= 1024, "barrier block");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&bars->k_full[s], 2);   // the two producer warps
+      mbar_init(&bars->k_empty[s], 1);
+      mbar_init(&bars->v_full[s], 2);
+      mbar_init(&bars->v_empty[s], 1);
+    }
+    mbar_init(&bars->q_full, 4 * MT);
+    for (int b = 0; b < 2 * MT; ++b) {
+      mbar_init(&bars->s_full[b], 1);
+      mbar_init(&bars->p_full[b], 4);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&bars->p_free[b], 1);
+      mbar_init(&bars->drain[b], 1);
+    }
+    bars->abort = 0;
+    bars->odd = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&bars->tmem_base, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  Share share;
+  TileCursor cur;
+  const bool work = cta_share<C::kThreads>(a, &bars->sh, share, cur);
+  if (threadIdx.x == 0) note_cut(a, work, cur, share);
+  clear_unused<T, C::kThreads>(a);
+  const int end = static_cast<int>(share.g1 - share.g0);
+  constexpr uint32_t fmt = std::is_same_v<typename C::X, __nv_bfloat16> ? 1u : 0u;
+  // Registers: the launch's 512 x 128 (MT = 2) go 168 to a softmax thread, 88 to the others.
+  if (warp < 8) {
+    if constexpr (MT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (work) {
+      if (warp == 0) {
+        if (lane == 0) issue_scores<C>(a, cur, end, smem, bars, tmem, fmt);
+      } else if (warp == 1) {
+        if (lane == 0) issue_outputs<C>(a, cur, end, smem, bars, tmem, fmt);
+      } else if (warp >= 4) {
+        produce<T, ST, C>(a, cur, end, smem, bars, (warp - 4) >> 1, warp & 1);
+      }
+    }
+  } else {
+    if constexpr (MT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    if (work) softmax<T, ST, C>(a, cur, end, smem, bars, tmem);
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (bars->abort && threadIdx.x == 0) raise_device_error(a.pool.err, kErrTimeout);
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+template <typename F>
+int by_config(const PagedAttn& a, F&& f) {
+  auto rows = [&](auto t, auto s, auto d) {
+    return a.m == 128 ? f(t, s, d, std::integral_constant<int, 1>()) : f(t, s, d, std::integral_constant<int, 2>());
+  };
+  auto dims = [&](auto t, auto s) {
+    return a.pool.d == 128 ? rows(t, s, std::integral_constant<int, 128>()) : rows(t, s, std::integral_constant<int, 64>());
+  };
+  auto store = [&](auto t) {
+    switch (a.pool.storage) {
+      case GORGON_KV_NATIVE: return dims(t, std::integral_constant<int, GORGON_KV_NATIVE>());
+      case GORGON_KV_INT8: return dims(t, std::integral_constant<int, GORGON_KV_INT8>());
+      default: return dims(t, std::integral_constant<int, GORGON_KV_E4M3>());
+    }
+  };
+  return a.pool.dtype == GORGON_BF16 ? store(__nv_bfloat16{}) : store(__half{});
+}
+
+}  // namespace
+
+bool paged_tc_supported(const PagedAttn& a) { return paged_mma_supported(a) && !(a.parents && a.n > kMaxTree); }
+
+void paged_tc_plan(PagedAttn* a) {
+  const int64_t rows = static_cast<int64_t>(a->n) * a->group;
+  a->m = rows <= 128 ? 128 : 256;
+  a->bn = kTile;
+  a->qblocks = static_cast<int>(ceil_div(rows, a->m));
+  a->unit_cost = 4;
+  const int64_t keys = static_cast<int64_t>(a->pool.table_cols) * a->pool.page_size;
+  const int64_t tiles = static_cast<int64_t>(a->pool.batch) * a->pool.hkv * a->qblocks * std::max<int64_t>(1, ceil_div(keys, kTile));
+  a->grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sm_count(), tiles)));
+}
+
+int launch_paged_tc(const PagedAttn& a, cudaStream_t st) {
+  return by_config(a, [&](auto t, auto s, auto d, auto mt) {
+    using C = TcCfg<decltype(t), decltype(s)::value, decltype(d)::value, decltype(mt)::value>;
+    auto kern = paged_tc_kernel<decltype(t), decltype(s)::value, decltype(d)::value, decltype(mt)::value>;
+    constexpr int smem = C::kSmem + 512;
+    static_assert(smem <= 232448, "shared memory per block");
+    int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "gorgon_paged_attn smem attribute");
+    if (rc) return rc;
+    kern<<<a.grid, C::kThreads, smem, st>>>(a);
+    return check_cuda(cudaGetLastError(), "gorgon_paged_attn launch");
+  });
+}
+
+}  // namespace gorgon

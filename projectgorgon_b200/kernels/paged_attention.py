@@ -17,7 +17,8 @@ from .._paged import compute_dtype, device_index, int32, packer, pool_fields
 from .._util import on_device, parents_tensor, stream_ptr, workspace
 
 _ATTN = packer("qqq" + "Pqqq" * 3 + "PPqiqqfi")
-_BACKENDS = {"auto": _abi.PAGED_AUTO, "simt": _abi.PAGED_SIMT, "mma": _abi.PAGED_MMA}
+_BACKENDS = {"auto": _abi.PAGED_AUTO, "simt": _abi.PAGED_SIMT, "mma": _abi.PAGED_MMA,
+             "tcgen05": _abi.PAGED_TCGEN05}
 
 
 def paged_attention(

@@ -73,7 +73,7 @@ def check(p: Paged, new, Hq, *, packed=False, parents=None, max_depth=None, wind
 STORES = ["native", "int8", "fp8"]
 
 
-@pytest.mark.parametrize("backend", ["auto", "mma", "simt"])
+@pytest.mark.parametrize("backend", ["auto", "mma", "tcgen05", "simt"])
 @pytest.mark.parametrize("storage", STORES)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("Hq,Hkv,D,ps", [(8, 2, 128, 16), (5, 1, 64, 12), (4, 4, 128, 1), (14, 2, 128, 7), (16, 1, 64, 64), (20, 1, 128, 16)])
