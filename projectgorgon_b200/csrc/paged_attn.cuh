@@ -42,7 +42,9 @@ struct PagedAttn {
   int rows;           // packed rows of q and out (with nr.cu)
   float scale_log2;   // softmax scale * log2(e)
   // tensor-core schedule
-  int m, bn;          // packed rows per unit, positions per tile
+  int m, bn_shift;    // packed rows per unit, log2 of the positions per tile
+  uint32_t group_m;   // with group_s: division by `group` (group_div)
+  int group_s;
   int qblocks;        // units per (sequence, kv head) at most
   int unit_cost;      // places in the list that a unit's start and end take
   int grid;
@@ -51,6 +53,18 @@ struct PagedAttn {
   struct CutUnit* cut;  // [grid]
   uint64_t wait_ns;
 };
+
+// n / group for 0 <= n < 2^31, by a multiplication (m = floor(2^32 (2^s - group)
+// / group) + 1, s = ceil(log2 group)).
+__device__ __forceinline__ int group_div(const PagedAttn& a, int n) {
+  return static_cast<int>((__umulhi(static_cast<uint32_t>(n), a.group_m) + static_cast<uint32_t>(n)) >> a.group_s);
+}
+inline void set_group_div(PagedAttn* a) {
+  int s = 0;
+  while ((1 << s) < a->group) ++s;
+  a->group_s = s;
+  a->group_m = static_cast<uint32_t>((((uint64_t(1) << s) - a->group) << 32) / a->group + 1);
+}
 
 // What CTA c leaves for the merge: the unit that its range starts inside of.
 // pieces == 0: none, or an earlier CTA's entry names the unit.
@@ -98,9 +112,10 @@ __device__ __forceinline__ UnitKeys unit_keys(const PagedAttn& a, const Seq& s, 
   const int first = s.P + (a.parents ? 0 : t0);  // the smallest position of the unit's rows, at least
   u.lo = a.window ? max(0, first - a.window + 1) : 0;
   u.s_end = min(a.sinks, u.lo);
-  u.lo_tile = u.lo / a.bn;
-  u.s_tiles = min((u.s_end + a.bn - 1) / a.bn, u.lo_tile);
-  u.tiles = u.s_tiles + (u.hi + a.bn - 1) / a.bn - u.lo_tile;
+  const int up = (1 << a.bn_shift) - 1;
+  u.lo_tile = u.lo >> a.bn_shift;
+  u.s_tiles = min((u.s_end + up) >> a.bn_shift, u.lo_tile);
+  u.tiles = u.s_tiles + ((u.hi + up) >> a.bn_shift) - u.lo_tile;
   return u;
 }
 
@@ -108,14 +123,14 @@ __device__ __forceinline__ UnitKeys unit_keys(const PagedAttn& a, const Seq& s, 
 __device__ __forceinline__ bool block_rows(const PagedAttn& a, const Seq& s, int qb, int& t0, int& t1) {
   const int r0 = qb * a.m, R = s.c * a.group;
   if (r0 >= R) return false;
-  t0 = r0 / a.group;
-  t1 = min(s.c, (min(r0 + a.m, R) - 1) / a.group + 1);
+  t0 = qb == 0 ? 0 : group_div(a, r0);
+  t1 = r0 + a.m >= R ? s.c : group_div(a, r0 + a.m - 1) + 1;
   return true;
 }
 
 // Places of every row block of one (sequence, kv head).
-__device__ __forceinline__ int64_t head_places(const PagedAttn& a, const Seq& s) {
-  int64_t n = 0;
+__device__ __forceinline__ int head_places(const PagedAttn& a, const Seq& s) {
+  int n = 0;
   int t0, t1;
   if (!s.ok) return 0;
   for (int qb = 0; block_rows(a, s, qb, t0, t1); ++qb) n += unit_keys(a, s, t0, t1).tiles + a.unit_cost;
@@ -150,6 +165,8 @@ struct TileCursor {
     u = unit_keys(a, s, t0, t1);
     return true;
   }
+  // Whether the CTA, whose share ends at place `end`, has a tile after this unit.
+  __device__ __forceinline__ bool more(const PagedAttn& a, int end) const { return at + u.tiles - i + a.unit_cost < end; }
   // To the next tile before place `end`; false when there is none.
   __device__ __forceinline__ bool next(const PagedAttn& a, int end) {
     if (i + 1 < u.tiles) {
@@ -157,7 +174,7 @@ struct TileCursor {
       ++at;
       return at < end;
     }
-    return at + 1 + a.unit_cost < end && next_unit(a) && at < end;
+    return more(a, end) && next_unit(a) && at < end;
   }
 };
 
@@ -167,59 +184,73 @@ struct TileCursor {
 // [t * per, (t + 1) * per), a block scan places them, and the thread that
 // owns g0 names its sequence.
 struct ShareScratch {
-  int64_t warp_sum[32];
-  int64_t rem;
-  int b;
+  int warp_sum[32];
+  int rem, b;
+  Seq s;
 };
 struct Share {
-  int64_t g0, g1, T, G;
+  int g0, g1, T, G;  // (the planner keeps T below 2^31)
+  // The first place of CTA c: c T / G, in 32 bits.
+  __device__ __forceinline__ int start(int c) const {
+    const uint32_t q = static_cast<uint32_t>(T) / static_cast<uint32_t>(G), r = static_cast<uint32_t>(T) - q * G;
+    return static_cast<int>(c * q + c * r / static_cast<uint32_t>(G));  // (c r < G^2)
+  }
 };
 template <int THREADS>
 __device__ __forceinline__ bool cta_share(const PagedAttn& a, ShareScratch* sh, Share& r, TileCursor& cur) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (a.pool.batch + THREADS - 1) / THREADS;
   const int b0 = min(tid * per, a.pool.batch), b1 = min(b0 + per, a.pool.batch);
-  int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += head_places(a, sequence(a, b, blockIdx.x == 0)) * a.pool.hkv;
-  int64_t incl = mine;
+  int mine = 0;
+  Seq last{};
+  for (int b = b0; b < b1; ++b) {
+    last = sequence(a, b, blockIdx.x == 0);
+    mine += head_places(a, last) * a.pool.hkv;
+  }
+  int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+    const int up = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += up;
   }
   if (lane == 31) sh->warp_sum[warp] = incl;
   __syncthreads();
-  int64_t before = 0, T = 0;
+  int before = 0, T = 0;
+#pragma unroll
   for (int w = 0; w < THREADS / 32; ++w) {
-    const int64_t x = sh->warp_sum[w];
+    const int x = sh->warp_sum[w];
     if (w < warp) before += x;
     T += x;
   }
   r.T = T;
-  r.G = min(static_cast<int64_t>(a.grid), T);
-  const bool work = static_cast<int64_t>(blockIdx.x) < r.G;
-  r.g0 = work ? static_cast<int64_t>(blockIdx.x) * T / r.G : T;
-  r.g1 = work ? static_cast<int64_t>(blockIdx.x + 1) * T / r.G : T;
-  const int64_t g0 = r.g0;
-  const int64_t start = before + incl - mine;
+  r.G = min(a.grid, T);
+  const bool work = static_cast<int>(blockIdx.x) < r.G;
+  r.g0 = work ? r.start(blockIdx.x) : T;
+  r.g1 = work ? r.start(blockIdx.x + 1) : T;
+  const int g0 = r.g0;
+  const int start = before + incl - mine;
   if (work && g0 >= start && g0 < start + mine) {
-    int64_t rem = g0 - start;
-    int b = b0;
-    for (; b < b1 - 1; ++b) {
-      const int64_t n = head_places(a, sequence(a, b, false)) * a.pool.hkv;
-      if (rem < n) break;
-      rem -= n;
+    int rem = g0 - start;
+    int b = b1 - 1;
+    if (per > 1) {
+      for (b = b0; b < b1 - 1; ++b) {
+        const int n = head_places(a, sequence(a, b, false)) * a.pool.hkv;
+        if (rem < n) break;
+        rem -= n;
+      }
+      last = sequence(a, b, false);
     }
     sh->b = b;
     sh->rem = rem;
+    sh->s = last;
   }
   __syncthreads();
   if (!work) return false;
   cur.b = sh->b;
-  cur.s = sequence(a, cur.b, false);
-  const int64_t per_head = head_places(a, cur.s);
-  cur.kvh = static_cast<int>(sh->rem / per_head);
-  int rem = static_cast<int>(sh->rem - cur.kvh * per_head);
+  cur.s = sh->s;
+  const uint32_t per_head = head_places(a, cur.s);
+  cur.kvh = static_cast<int>(static_cast<uint32_t>(sh->rem) / per_head);
+  int rem = sh->rem - cur.kvh * per_head;
   for (cur.qb = 0;; ++cur.qb) {
     block_rows(a, cur.s, cur.qb, cur.t0, cur.t1);
     cur.u = unit_keys(a, cur.s, cur.t0, cur.t1);
@@ -239,10 +270,11 @@ __device__ __forceinline__ void note_cut(const PagedAttn& a, bool work, const Ti
   CutUnit n{};
   if (work && cur.i > 0) {
     const int c = blockIdx.x;
-    const int64_t first = r.g0 - cur.i, end = first + cur.u.tiles;  // places of the unit's tiles
-    const int64_t prev = static_cast<int64_t>(c - 1) * r.T / r.G;
+    const int first = r.g0 - cur.i, end = first + cur.u.tiles;  // places of the unit's tiles
+    const int prev = r.start(c - 1);
     if (first >= prev) {
-      const int last = static_cast<int>((end * r.G - 1) / r.T);  // the CTA of place end - 1
+      int last = c;  // the CTA of place end - 1
+      if (r.g1 < end) last = static_cast<int>((static_cast<int64_t>(end) * r.G - 1) / r.T);
       n = CutUnit{cur.b, cur.kvh, cur.qb, last - c + 2, prev >= first - a.unit_cost ? 0 : 1};
     }
   }
@@ -287,6 +319,23 @@ __device__ __forceinline__ int tree_bits(const PagedAttn& a, const Seq& s, int b
     cur = up;
   }
   return hop;
+}
+
+// Launches a kernel so that it may start while the one before it in the stream
+// ends (it waits for that itself, by griddepcontrol.wait).
+template <typename K>
+int launch_early(K kern, const PagedAttn& a, int threads, int smem, cudaStream_t st, int grid_y = 1) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.grid), static_cast<unsigned>(grid_y));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, a), "gorgon_paged_attn launch");
 }
 
 int launch_paged_simt(const PagedAttn& a, cudaStream_t st);

@@ -45,6 +45,7 @@ int make_args(const gorgon_paged_attn_params* p, PagedAttn* a) {
   x.hq = static_cast<int>(p->heads_q);
   x.group = x.hq / x.pool.hkv;
   x.n = static_cast<int>(p->n);
+  if (x.group > 0) set_group_div(&x);
   x.rows = p->cu_q ? static_cast<int>(p->rows) : 0;
   const float scale = p->scale != 0.f ? p->scale : (x.pool.d > 0 ? 1.f / std::sqrt(static_cast<float>(x.pool.d)) : 1.f);
   x.scale_log2 = scale * 1.4426950408889634f;
@@ -56,15 +57,22 @@ bool empty(const PagedAttn& a) { return static_cast<int64_t>(a.pool.batch) * a.h
 
 enum class Kernel { kSimt, kMma, kTc, kNone };
 
+// The schedule's places fit 32 bits (it counts them per 64 positions or more).
+bool short_list(const PagedAttn& a) {
+  const int64_t blocks = static_cast<int64_t>(a.n) * a.group / 8 + 1;
+  const int64_t tiles = static_cast<int64_t>(a.pool.table_cols) * a.pool.page_size / 64 + 6;
+  return blocks * tiles < (int64_t(1) << 31) / (static_cast<int64_t>(a.pool.batch) * a.pool.hkv + 1);
+}
+
 Kernel choose(const gorgon_paged_attn_params* p, const PagedAttn& a) {
-  const bool mma = paged_mma_supported(a);
+  const bool mma = paged_mma_supported(a) && short_list(a);
   switch (p->backend) {
     case GORGON_PAGED_SIMT: return Kernel::kSimt;
     case GORGON_PAGED_MMA: return mma ? Kernel::kMma : Kernel::kNone;
-    case GORGON_PAGED_TCGEN05: return paged_tc_supported(a) ? Kernel::kTc : Kernel::kNone;
+    case GORGON_PAGED_TCGEN05: return mma && paged_tc_supported(a) ? Kernel::kTc : Kernel::kNone;
     default:
       // up to 16 packed rows fill one tile of the warp-level kernel
-      if (static_cast<int64_t>(a.n) * a.group > 16 && paged_tc_supported(a)) return Kernel::kTc;
+      if (static_cast<int64_t>(a.n) * a.group > 16 && mma && paged_tc_supported(a)) return Kernel::kTc;
       return mma ? Kernel::kMma : Kernel::kSimt;
   }
 }

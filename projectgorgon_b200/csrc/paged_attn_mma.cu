@@ -51,9 +51,9 @@ struct Cfg {
   static constexpr int kStage = kOffWord + (kWide ? 16 : 16 + 8 * G);
   // Two CTAs an SM, so that one's unit ends (barriers, the next unit's Q) pass
   // under the other's loads.
-  static constexpr int kWarps = kRowBytes == 64 ? 6 : 4;
+  static constexpr int kWarps = 4;
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kStages = kRowBytes == 64 ? 4 : 3;
+  static constexpr int kStages = kRowBytes == 64 ? 6 : 3;
   static constexpr int BN = G * kWarps;
   static constexpr int M = 8 * NT;
   // 16-byte pieces: kCpr to a row, kRpi rows to a copy instruction.  Piece p of
@@ -148,7 +148,7 @@ __device__ __noinline__ uint32_t hidden_scores(const PagedAttn& a, const TileCur
     const int pr = row + (k >> 2) * 8 + (k & 1), j = k & 2 ? j1 : j0;
     bool see = (k & 2 ? held1 : held0) && pr < R;
     if (see) {
-      const int t = pr / a.group;
+      const int t = group_div(a, pr);
       if (a.parents && j >= P) {
         see = j - P < cur->s.c && ((bits[(t - cur->t0) * (kPagedMaxNodes / 32) + ((j - P) >> 5)] >> ((j - P) & 31)) & 1u);
       } else {
@@ -181,6 +181,8 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
   extern __shared__ __align__(128) uint8_t smem[];
   static_assert(sizeof(ShareScratch) <= kRedFloats * 4, "scratch");
   ShareScratch* sh = reinterpret_cast<ShareScratch*>(smem + C::kOffRed);
+  // Launched while the kernel before it ends; nothing is read before that has.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
@@ -216,6 +218,7 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
   const int end = static_cast<int>(share.g1 - share.g0);
   UnitKeys u;              // of `ahead`
   int tile = 0, left = 0;  // the tile to fetch, and how many of the unit's are left to fetch with it
+  bool more = false;       // the CTA has tiles of a later unit
   int page = -2, prow = 0;
   const bool in_pages = a.pool.page_size % 16 == 0;  // 16 keys from a multiple of 16 on lie in one page
   const int piece = lane % C::kCpr, rsub = lane / C::kCpr;
@@ -234,6 +237,7 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
     u = ahead.u;
     tile = ahead.i;
     left = min(u.tiles - tile, end - ahead.at);
+    more = ahead.more(a, end);
     kb = a.pool.k + ahead.kvh * a.pool.k_sh + piece * 16;
     vb = a.pool.v + ahead.kvh * a.pool.v_sh + piece * 16;
     if constexpr (!C::kWide) {
@@ -314,9 +318,10 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
         }
       }
       ++tile;
-      if (--left == 0) {
+      if (--left == 0 && more) {
         if (lane == 0) step_unit(a, &ahead, end);
         __syncwarp();
+        more = false;
         if (ahead.at < end) enter();
         __syncwarp();
       }
@@ -355,7 +360,7 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
       for (int nt = 0; nt < NT; ++nt) {
         const int pr = cur.qb * C::M + nt * 8 + g;
         const bool ok = pr < R;
-        const int t = ok ? pr / a.group : 0;
+        const int t = ok ? group_div(a, pr) : 0;
         const int h = cur.kvh * a.group + (ok ? pr - t * a.group : 0);
         const char* row = qb + (first + t) * a.q_sn + static_cast<int64_t>(h) * a.q_sh;
 #pragma unroll
@@ -722,7 +727,7 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
           const int row = nt * 8 + r;
           const float top = s_row[row].x, L = s_row[row].y;
           if (whole) {
-            const int pr = cur.qb * C::M + row, tt = pr / a.group, h = cur.kvh * a.group + pr - tt * a.group;
+            const int pr = cur.qb * C::M + row, tt = group_div(a, pr), h = cur.kvh * a.group + pr - tt * a.group;
             T* out = reinterpret_cast<T*>(a.out) + (a.nr.cu ? 0 : cur.b * a.o_sb) + h * a.o_sh + (first + tt) * a.o_sn;
             out[d] = Cvt<T>::from_f(sum * (1.f / L));
             if (a.lse && d == 0)
@@ -736,6 +741,8 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
       }
     }
     first_unit = cut_start = false;
+    if (!cur.more(a, end)) break;
+    __syncthreads();
     if (threadIdx.x == 0) step_unit(a, &cur, end);
     __syncthreads();  // (the rows' maxima and sums, too, are read before the next unit writes them)
     if (cur.at >= end) break;
@@ -751,8 +758,7 @@ int launch_t(const PagedAttn& a, cudaStream_t st) {
   int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem),
                       "gorgon_paged_attn smem attribute");
   if (rc) return rc;
-  kern<<<a.grid, C::kThreads, C::kSmem, st>>>(a);
-  return check_cuda(cudaGetLastError(), "gorgon_paged_attn launch");
+  return launch_early(kern, a, C::kThreads, C::kSmem, st);
 }
 
 // Calls f with the configuration's constants as types.
@@ -791,14 +797,17 @@ void paged_mma_plan(PagedAttn* a) {
   const int64_t rows = static_cast<int64_t>(a->n) * a->group;
   a->m = rows <= 8 ? 8 : 16;
   by_config(*a, [&](auto t, auto s, auto d, auto nt) {
-    a->bn = Cfg<decltype(t), decltype(s)::value, decltype(d)::value, decltype(nt)::value>::BN;
+    constexpr int bn = Cfg<decltype(t), decltype(s)::value, decltype(d)::value, decltype(nt)::value>::BN;
+    static_assert((bn & (bn - 1)) == 0, "tiles of a power of two");
+    for (a->bn_shift = 0; (1 << a->bn_shift) < bn; ++a->bn_shift) {
+    }
     return 0;
   });
   a->qblocks = static_cast<int>(ceil_div(rows, a->m));
   a->unit_cost = 2;
   // no more CTAs than there can be tiles
   const int64_t keys = static_cast<int64_t>(a->pool.table_cols) * a->pool.page_size;
-  const int64_t tiles = static_cast<int64_t>(a->pool.batch) * a->pool.hkv * a->qblocks * std::max<int64_t>(1, ceil_div(keys, a->bn));
+  const int64_t tiles = static_cast<int64_t>(a->pool.batch) * a->pool.hkv * a->qblocks * std::max<int64_t>(1, ceil_div(keys, int64_t(1) << a->bn_shift));
   a->grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(static_cast<int64_t>(kCtasPerSm) * sm_count(), tiles)));
 }
 

@@ -138,6 +138,7 @@ int launch_t(const PagedAttn& a, cudaStream_t st) {
 constexpr int kMergeWarps = 8;
 template <typename T, int D>
 __global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __grid_constant__ PagedAttn a) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   __shared__ float s_acc[kMergeWarps][D];
   __shared__ float s_l[kMergeWarps];
@@ -159,22 +160,31 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __g
   M = warp_max(M);
   const float base = M == -INFINITY ? 0.f : M;
   float L = 0.f, acc[V] = {};
-#pragma unroll 8
-  for (int p = sub; p < n.pieces; p += per) {
-    const float2 ml = __ldcg(&a.part_ml[slot(p) * a.m + row]);
-    const float f = exp2f(ml.x - base);
-    const float* o = a.part_o + (slot(p) * a.m + row) * D + lane * V;
-    L = fmaf(f, ml.y, L);
-    if constexpr (V == 4) {
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(o));
-      acc[0] = fmaf(f, x.x, acc[0]);
-      acc[1] = fmaf(f, x.y, acc[1]);
-      acc[2] = fmaf(f, x.z, acc[2]);
-      acc[3] = fmaf(f, x.w, acc[3]);
-    } else {
-      const float2 x = __ldcg(reinterpret_cast<const float2*>(o));
-      acc[0] = fmaf(f, x.x, acc[0]);
-      acc[1] = fmaf(f, x.y, acc[1]);
+  constexpr int kInFlight = 8;
+#pragma unroll 1
+  for (int p0 = sub; p0 < n.pieces; p0 += per * kInFlight) {
+    float2 ml[kInFlight];
+    float x[kInFlight][V];
+#pragma unroll
+    for (int k = 0; k < kInFlight; ++k) {
+      const int p = p0 + k * per;
+      ml[k] = make_float2(-INFINITY, 0.f);
+      if (p < n.pieces) {
+        ml[k] = __ldcg(&a.part_ml[slot(p) * a.m + row]);
+        const float* o = a.part_o + (slot(p) * a.m + row) * D + lane * V;
+        if constexpr (V == 4)
+          *reinterpret_cast<float4*>(x[k]) = __ldcg(reinterpret_cast<const float4*>(o));
+        else
+          *reinterpret_cast<float2*>(x[k]) = __ldcg(reinterpret_cast<const float2*>(o));
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kInFlight; ++k) {
+      if (p0 + k * per >= n.pieces) break;
+      const float f = exp2f(ml[k].x - base);
+      L = fmaf(f, ml[k].y, L);
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] = fmaf(f, x[k][v], acc[v]);
     }
   }
   if (per > 1) {
@@ -204,23 +214,12 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __g
 }  // namespace
 
 int launch_paged_merge(const PagedAttn& a, cudaStream_t st) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.grid), static_cast<unsigned>(ceil_div(a.m, 8)));
-  cfg.blockDim = dim3(kMergeWarps * 32);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  cudaError_t e;
+  const int y = static_cast<int>(ceil_div(a.m, 8));
   if (a.pool.dtype == GORGON_BF16)
-    e = a.pool.d == 128 ? cudaLaunchKernelEx(&cfg, paged_merge_kernel<__nv_bfloat16, 128>, a)
-                        : cudaLaunchKernelEx(&cfg, paged_merge_kernel<__nv_bfloat16, 64>, a);
-  else
-    e = a.pool.d == 128 ? cudaLaunchKernelEx(&cfg, paged_merge_kernel<__half, 128>, a)
-                        : cudaLaunchKernelEx(&cfg, paged_merge_kernel<__half, 64>, a);
-  return check_cuda(e, "gorgon_paged_attn merge launch");
+    return a.pool.d == 128 ? launch_early(paged_merge_kernel<__nv_bfloat16, 128>, a, kMergeWarps * 32, 0, st, y)
+                           : launch_early(paged_merge_kernel<__nv_bfloat16, 64>, a, kMergeWarps * 32, 0, st, y);
+  return a.pool.d == 128 ? launch_early(paged_merge_kernel<__half, 128>, a, kMergeWarps * 32, 0, st, y)
+                         : launch_early(paged_merge_kernel<__half, 64>, a, kMergeWarps * 32, 0, st, y);
 }
 
 int launch_paged_simt(const PagedAttn& a, cudaStream_t st) {

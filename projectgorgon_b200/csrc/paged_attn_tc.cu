@@ -413,7 +413,7 @@ __device__ void softmax(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
     const int64_t first = a.nr.cu ? a.nr.cu[cur.b] : 0;
     const int pr = cur.qb * C::M + qrow;
     const bool row_ok = pr < R;
-    const int t = row_ok ? pr / a.group : cur.t0;
+    const int t = row_ok ? group_div(a, pr) : cur.t0;
     const int h = cur.kvh * a.group + (row_ok ? pr - t * a.group : 0);
     // ---- Q rows -> shared memory; the previous unit's last product is complete
     {
@@ -426,7 +426,7 @@ __device__ void softmax(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
           const int p = p0 + k0 + k * kRows + rsub;
-          const int tt = p / a.group, gg = p - tt * a.group;
+          const int tt = group_div(a, p), gg = p - tt * a.group;
           qv[k] = p < R ? __ldg(reinterpret_cast<const uint4*>(qb + tt * a.q_sn + gg * a.q_sh) + chunk) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
@@ -533,7 +533,7 @@ __device__ void softmax(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
       const uint64_t qs2 = f2_pack(qs, qs), nmb2 = f2_pack(nmb, nmb);
       uint64_t acc[4] = {0, 0, 0, 0};
       uint32_t packed[kTile / 2];
-      const float4* vs = reinterpret_cast<const float4*>(meta + 16 + 4 * kTile);
+      [[maybe_unused]] const float4* vs = reinterpret_cast<const float4*>(meta + 16 + 4 * kTile);
       const uint64_t unit2 = f2_pack(unit, unit);
 #pragma unroll
       for (int c = 0; c < kTile; c += 4) {
@@ -670,7 +670,7 @@ __device__ void softmax(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
 #pragma unroll 4
         for (int k = 0; k < 32; k += kRows) {
           const int p = p0 + k + rsub;
-          const int tt = p / a.group, gg = p - tt * a.group;
+          const int tt = group_div(a, p), gg = p - tt * a.group;
           const uint4 w = *reinterpret_cast<const uint4*>(stage_row(k + rsub, chunk));
           if (p < R) *reinterpret_cast<uint4*>(ob + tt * a.o_sn + gg * a.o_sh) = w;
         }
@@ -695,7 +695,6 @@ __global__ void __launch_bounds__(TcCfg<T, ST, D, MT>::kThreads, 1) paged_tc_ker
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   TcBars<C>* bars = reinterpret_cast<TcBars<C>*>(smem + C::kOffBar);
   static_assert(sizeof(TcBars<C>) <= 1024, "barrier block");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
@@ -725,6 +724,9 @@ __global__ void __launch_bounds__(TcCfg<T, ST, D, MT>::kThreads, 1) paged_tc_ker
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
+  // Launched while the kernel before it ends; nothing is read before that has.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   Share share;
   TileCursor cur;
   const bool work = cta_share<C::kThreads>(a, &bars->sh, share, cur);
@@ -783,7 +785,7 @@ bool paged_tc_supported(const PagedAttn& a) { return paged_mma_supported(a) && !
 void paged_tc_plan(PagedAttn* a) {
   const int64_t rows = static_cast<int64_t>(a->n) * a->group;
   a->m = rows <= 128 ? 128 : 256;
-  a->bn = kTile;
+  a->bn_shift = 6;
   a->qblocks = static_cast<int>(ceil_div(rows, a->m));
   a->unit_cost = 4;
   const int64_t keys = static_cast<int64_t>(a->pool.table_cols) * a->pool.page_size;
@@ -799,8 +801,7 @@ int launch_paged_tc(const PagedAttn& a, cudaStream_t st) {
     static_assert(smem <= 232448, "shared memory per block");
     int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "gorgon_paged_attn smem attribute");
     if (rc) return rc;
-    kern<<<a.grid, C::kThreads, smem, st>>>(a);
-    return check_cuda(cudaGetLastError(), "gorgon_paged_attn launch");
+    return launch_early(kern, a, C::kThreads, smem, st);
   });
 }
 

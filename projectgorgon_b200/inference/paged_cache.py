@@ -16,8 +16,8 @@ from typing import Optional, Tuple, Union
 import torch
 
 from .. import _abi
-from .._paged import compute_dtype, device_index, int32, packer, pool_fields
-from .._util import gorgon_dtype, on_device, stream_ptr
+from .._paged import call, compute_dtype, device_index, int32, packer, pool_fields
+from .._util import gorgon_dtype
 from ..kernels.paged_attention import paged_attention
 
 _APPEND = packer("PqqqPqqqqqP")
@@ -39,8 +39,8 @@ def paged_cache_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, 
     12 significant bits (``largest`` 127 for int8, 448 for e4m3); a row with an
     infinity or a NaN reads back as NaN.  Two sequences of one call must not
     share the page row that they write."""
-    device_index("k, v, pages, block_table and seq_lens", k, v, k_pages, v_pages, block_table, seq_lens, k_scale,
-                 v_scale, cu_q)
+    dev = device_index("k, v, pages, block_table and seq_lens", k, v, k_pages, v_pages, block_table, seq_lens, k_scale,
+                       v_scale, cu_q)
     dtype = compute_dtype(k.dtype, "k")
     if v.dtype is not dtype or v.shape != k.shape:
         raise RuntimeError(f"k and v must have one shape and dtype, got {tuple(k.shape)} {k.dtype} and "
@@ -74,9 +74,7 @@ def paged_cache_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, 
         raise RuntimeError(f"k has {heads} heads of {d}, the pages {pool[4]} of {pool[5]}")
     params = _APPEND.pack(*pool, k.data_ptr(), k_sb, k_sh, k_sn, v.data_ptr(), v_sb, v_sh, v_sn, n, rows,
                           0 if cu is None else cu.data_ptr())
-    dev = k.device
-    with on_device(dev):
-        rc = _abi.lib().gorgon_paged_append(params, stream_ptr(dev))
+    rc = call(dev, _abi.lib().gorgon_paged_append, params)
     if rc:
         _abi.check(rc, "gorgon_paged_append")
 
@@ -92,8 +90,8 @@ def paged_cache_read(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: 
     ``D`` contiguous, keeps them).  ``dtype`` is the result's: default the pages'
     own, or bfloat16 for 8-bit pages.  8-bit values are multiplied by their scale
     in fp32 and rounded once, to the type's largest finite value at most."""
-    device_index("pages, block_table and cu_rows", k_pages, v_pages, block_table, cu_rows, starts, k_scale, v_scale,
-                 *(out or ()))
+    dev = device_index("pages, block_table and cu_rows", k_pages, v_pages, block_table, cu_rows, starts, k_scale,
+                       v_scale, *(out or ()))
     native = k_pages.dtype not in (torch.int8, torch.float8_e4m3fn)
     if out is not None:
         dtype = out[0].dtype if dtype is None else dtype
@@ -114,9 +112,9 @@ def paged_cache_read(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: 
         raise RuntimeError("rows must not be negative")
     pool = pool_fields(held, k_pages, v_pages, table, None, batch, k_scale, v_scale)
     shape = (rows, pool[4], pool[5])
-    dev = k_pages.device
     if out is None:
-        k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
+        on = k_pages.device
+        k, v = torch.empty(shape, dtype=dtype, device=on), torch.empty(shape, dtype=dtype, device=on)
     else:
         k, v = out
         for x in out:
@@ -125,8 +123,7 @@ def paged_cache_read(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: 
     (k_sn, k_sh, _), (v_sn, v_sh, _) = k.stride(), v.stride()
     params = _READ.pack(*pool, gorgon_dtype(dtype), k.data_ptr(), k_sn, k_sh, v.data_ptr(), v_sn, v_sh, rows,
                         cu.data_ptr(), 0 if starts is None else starts.data_ptr())
-    with on_device(dev):
-        rc = _abi.lib().gorgon_paged_read(params, stream_ptr(dev))
+    rc = call(dev, _abi.lib().gorgon_paged_read, params)
     if rc:
         _abi.check(rc, "gorgon_paged_read")
     return k, v
@@ -142,24 +139,23 @@ def paged_cache_trim(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: 
     (or one layer's ``[pages, Hkv, page_size, D]``); ``dst_start`` ``[B]``, an int, or
     None for 0.  At most 256 rows per sequence.  A bad index sets the device
     error bits and leaves its sequence as it is."""
-    device_index("pages, block_table, src_idx and lens", k_pages, v_pages, block_table, src_idx, lens, k_scale, v_scale,
-                 dst_start if isinstance(dst_start, torch.Tensor) else None)
+    dev = device_index("pages, block_table, src_idx and lens", k_pages, v_pages, block_table, src_idx, lens, k_scale,
+                       v_scale, dst_start if isinstance(dst_start, torch.Tensor) else None)
     lead = 1 if k_pages.dim() == 5 else 0
     native = k_pages.dtype not in (torch.int8, torch.float8_e4m3fn)
     held = compute_dtype(k_pages.dtype, "k_pages") if native else torch.bfloat16
     table = int32(block_table, "block_table", 2)
     idx = int32(src_idx.unsqueeze(0) if src_idx.dim() == 1 else src_idx, "src_idx", 2)
-    ln = int32(lens.reshape(-1), "lens", 1)
+    ln = int32(lens if lens.dim() == 1 else lens.reshape(-1), "lens", 1)
     batch = table.shape[0]
     if idx.shape[0] != batch or ln.shape[0] != batch:
         raise RuntimeError("src_idx and lens need one row per sequence")
-    dev = k_pages.device
     if dst_start is None:
         ds = None
     elif isinstance(dst_start, int):
-        ds = torch.full((batch,), dst_start, dtype=torch.int32, device=dev)
+        ds = torch.full((batch,), dst_start, dtype=torch.int32, device=k_pages.device)
     else:
-        ds = int32(dst_start.reshape(-1), "dst_start", 1)
+        ds = int32(dst_start if dst_start.dim() == 1 else dst_start.reshape(-1), "dst_start", 1)
         if ds.shape[0] != batch:
             raise RuntimeError("dst_start needs one entry per sequence")
     pool = pool_fields(held, k_pages, v_pages, table, None, batch, k_scale, v_scale, lead)
@@ -170,8 +166,7 @@ def paged_cache_trim(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: 
         layers, k_sl, v_sl, ks_sl, vs_sl = 1, 0, 0, 0, 0
     params = _TRIM.pack(*pool, layers, k_sl, v_sl, ks_sl, vs_sl, idx.data_ptr(), idx.stride(0), idx.shape[1],
                         ln.data_ptr(), 0 if ds is None else ds.data_ptr())
-    with on_device(dev):
-        rc = _abi.lib().gorgon_paged_trim(params, stream_ptr(dev))
+    rc = call(dev, _abi.lib().gorgon_paged_trim, params)
     if rc:
         _abi.check(rc, "gorgon_paged_trim")
 

@@ -13,12 +13,17 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from .. import _abi
-from .._paged import compute_dtype, device_index, int32, packer, pool_fields
-from .._util import on_device, parents_tensor, stream_ptr, workspace
+from .._paged import call, compute_dtype, device_index, int32, packer, pool_fields
+from .._util import parents_tensor
 
 _ATTN = packer("qqq" + "Pqqq" * 3 + "PPqiqqfi")
 _BACKENDS = {"auto": _abi.PAGED_AUTO, "simt": _abi.PAGED_SIMT, "mma": _abi.PAGED_MMA,
              "tcgen05": _abi.PAGED_TCGEN05}
+
+
+def _workspace_size_on(dev: int, params: bytes) -> int:
+    with torch.cuda.device(dev):  # the schedule counts the current device's SMs
+        return _abi.lib().gorgon_paged_attn_workspace_size(params)
 
 
 def paged_attention(
@@ -145,11 +150,10 @@ def paged_attention(
                         -1 if max_depth is None else int(max_depth), 0 if window is None else int(window), int(sinks),
                         0.0 if scale is None else float(scale), be)
     lib = _abi.lib()
-    device = q.device
-    with on_device(device):
-        nbytes = lib.gorgon_paged_attn_workspace_size(params)
-        ws = workspace(nbytes, device) if nbytes else None
-        rc = lib.gorgon_paged_attn(params, ws.data_ptr() if nbytes else 0, nbytes, stream_ptr(device))
+    nbytes = lib.gorgon_paged_attn_workspace_size(params) if dev == torch._C._cuda_getDevice() else \
+        _workspace_size_on(dev, params)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    rc = call(dev, lib.gorgon_paged_attn, params, ws.data_ptr() if nbytes else 0, nbytes)
     if rc:
         _abi.check(rc, "gorgon_paged_attn")
     return (out, lse) if return_lse else out
