@@ -6,7 +6,7 @@
 // tile list (paged_attn.cuh).  Warp roles:
 //   warp 0        Q K^T issuer (one thread)
 //   warp 1        P V issuer (one thread); the warp allocates TMEM
-//   warps 2, 3    idle (they fill a warpgroup: registers go to the others)
+//   warps 2, 3    idle
 //   warps 4, 5    K producers, 32 rows of every tile each
 //   warps 6, 7    V producers
 //   warps 8 - 11  softmax and epilogue of M-tile 0, a thread per row
@@ -59,7 +59,8 @@ struct TcCfg {
   static constexpr uint32_t kTileBytes = kHalves * kBlock;
   static constexpr int kStages = kWide ? (MT == 2 ? 4 : 5) : 3;
   static constexpr int kRawStages = kWide ? 0 : (MT == 2 ? 3 : 5);
-  static constexpr uint32_t kRawBytes = 32 * D;          // a producer's rows of a tile
+  static constexpr uint32_t kRawBytes = 32 * D + 256;    // a producer's rows of a tile, their K and V scales
+  static constexpr int kInfo = 8;                        // (more than the tiles a producer has in flight)
   static constexpr int kLag = kWide ? kStages - 2 : 0;   // tiles in flight behind the newest
   static constexpr uint32_t kOffK = MT * kQTile;
   static constexpr uint32_t kOffV = kOffK + kStages * kTileBytes;
@@ -68,7 +69,8 @@ struct TcCfg {
   static constexpr uint32_t kMetaBytes = kWide ? 16 : 16 + 8 * kTile;       // 2 words of valid keys, max V scale x 2; K and V scales
   static constexpr uint32_t kOffBits = kOffMeta + kStages * kMetaBytes;     // [M][8] ancestor words
   static constexpr uint32_t kOffQs = kOffBits + M * (kMaxTree / 32) * 4;    // [M] undoes Q's power of two
-  static constexpr uint32_t kOffBar = (kOffQs + M * 4 + 15) / 16 * 16;
+  static constexpr uint32_t kOffInfo = kOffQs + M * 4;                      // [4 producers][kInfo] valid keys, plain
+  static constexpr uint32_t kOffBar = (kOffInfo + 4 * kInfo * 8 + 15) / 16 * 16;
   static constexpr uint32_t kSmem = kOffBar + 512 + 1024;                   // + alignment slack
   static_assert(kSmem <= 232448, "shared memory per block");
 };
@@ -89,6 +91,10 @@ struct TcBars {
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {
   const int n = take ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool take) {
+  const int n = take ? 4 : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -144,34 +150,37 @@ __device__ void produce(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
 
   // The fetch runs ahead of the hand-over by kLag tiles (16-bit) or by the raw ring (8-bit).
   constexpr int kAhead = C::kWide ? C::kLag : C::kRawStages - 1;
-  struct Held {  // of a fetched tile
-    uint32_t valid;
-    float ks, vs;
-    bool plain;
-  };
-  Held held[C::kWide ? C::kLag + 1 : C::kRawStages];
+  // Of a fetched tile: which rows it has, and whether every row of the unit sees it whole.
+  uint2* info = reinterpret_cast<uint2*>(smem + C::kOffInfo) + (is_v * 2 + half) * C::kInfo;
+  static_assert(kAhead + 1 < C::kInfo, "info ring");
   TileCursor f = cur;
   bool more = true;
   int f_tile = 0;             // tiles fetched
   Slot<C::kStages> fs;        // (16-bit) the stage fetched into
-  auto fetch = [&](Held& h) -> bool {
+  // The page of this lane's row of the next tile (-2: not wanted), looked up a tile ahead.
+  int next_page = -2, next_row = 0;
+  auto look_up = [&]() {
+    next_page = -2;
+    const int j = f.tile() * kTile + half * 32 + lane;
+    if (f.u.wanted(j)) {
+      int col;
+      a.pool.split(j, col, next_row);
+      next_page = __ldg(a.pool.table + static_cast<int64_t>(f.b) * a.pool.table_sb + col);
+    }
+  };
+  look_up();
+  auto fetch = [&]() -> bool {
     if constexpr (C::kWide) {
       if (!warp_wait(&empty[fs.stage], fs.phase ^ 1u, abort, a.wait_ns)) return false;
     }
-    const int j0 = f.tile() * kTile + half * 32;
-    const int j = j0 + lane;
-    int page = -1, prow = 0;
-    if (f.u.wanted(j)) {
-      int col;
-      a.pool.split(j, col, prow);
-      page = __ldg(a.pool.table + static_cast<int64_t>(f.b) * a.pool.table_sb + col);
-      if (page < 0 || page >= a.pool.num_pages) {
-        raise_device_error(a.pool.err, kErrBadPage);
-        page = -1;
-      }
+    int page = next_page;
+    const int prow = next_row;
+    if (page != -2 && (page < 0 || page >= a.pool.num_pages)) {
+      raise_device_error(a.pool.err, kErrBadPage);
+      page = -2;
     }
-    h.valid = __ballot_sync(0xffffffffu, page >= 0);
-    h.plain = Common(a, f).plain(a, f.tile() * kTile);
+    const uint32_t valid = __ballot_sync(0xffffffffu, page >= 0);
+    if (lane == 0) info[f_tile % C::kInfo] = make_uint2(valid, Common(a, f).plain(a, f.tile() * kTile) ? 1u : 0u);
     const int64_t off = page >= 0 ? page * sp + prow * ss : 0;
     const char* base = pages + f.kvh * sh + piece * 16;
 #pragma unroll
@@ -183,25 +192,28 @@ __device__ void produce(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
         at = smem_u32(ring + fs.stage * C::kTileBytes + (piece >> 3) * C::kBlock) + sw128(half * 32 + r, piece & 7);
       else
         at = smem_u32(raw + (f_tile % C::kRawStages) * C::kRawBytes) + r * kRow + piece * 16;
-      cp16(at, base + o, (h.valid >> r) & 1u);
+      cp16(at, base + o, (valid >> r) & 1u);
     }
-    cp_commit();
     if constexpr (!C::kWide) {
-      h.ks = h.vs = 0.f;
-      if (is_v && page >= 0) {
-        h.ks = __ldg(a.pool.ks + page * a.pool.ks_sp + f.kvh * a.pool.ks_sh + prow * a.pool.ks_ss);
-        h.vs = __ldg(a.pool.vs + page * a.pool.vs_sp + f.kvh * a.pool.vs_sh + prow * a.pool.vs_ss);
+      if (is_v) {
+        const int64_t pg = page >= 0 ? page : 0, pr = page >= 0 ? prow : 0;
+        const uint32_t at = smem_u32(raw + (f_tile % C::kRawStages) * C::kRawBytes) + 32 * kRow + lane * 4;
+        cp4(at, a.pool.ks + pg * a.pool.ks_sp + f.kvh * a.pool.ks_sh + pr * a.pool.ks_ss, page >= 0);
+        cp4(at + 128, a.pool.vs + pg * a.pool.vs_sp + f.kvh * a.pool.vs_sh + pr * a.pool.vs_ss, page >= 0);
       }
     }
+    cp_commit();
     if constexpr (C::kWide) fs.next();
     ++f_tile;
     more = f.next(a, end);
+    if (more) look_up();
     return true;
   };
   Slot<C::kStages> hs;  // the stage handed over
   int done = 0;
   // Hands tile `done` over: its copies have landed.
-  auto hand_over = [&](const Held& h) -> bool {
+  auto hand_over = [&]() -> bool {
+    const uint2 h = info[done % C::kInfo];
     uint8_t* st = ring + hs.stage * C::kTileBytes;
     __syncwarp();  // every lane's copies
     if constexpr (!C::kWide) {
@@ -223,15 +235,17 @@ __device__ void produce(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
     }
     if (is_v) {
       uint8_t* meta = smem + C::kOffMeta + hs.stage * C::kMetaBytes;
-      if (lane == 0) reinterpret_cast<uint32_t*>(meta)[half] = h.valid;
+      if (lane == 0) reinterpret_cast<uint32_t*>(meta)[half] = h.x;
       if constexpr (!C::kWide) {
-        float top = h.vs;  // (NaN never wins)
+        const float* sc = reinterpret_cast<const float*>(raw + (done % C::kRawStages) * C::kRawBytes + 32 * kRow);
+        const float vs = sc[32 + lane];
+        float top = vs;  // (NaN never wins)
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         if (lane == 0) reinterpret_cast<float*>(meta)[2 + half] = top;
-        reinterpret_cast<float*>(meta + 16)[half * 32 + lane] = h.ks;
-        reinterpret_cast<float*>(meta + 16)[kTile + half * 32 + lane] = h.vs;
-      } else if (!(h.plain && h.valid == 0xffffffffu)) {
+        reinterpret_cast<float*>(meta + 16)[half * 32 + lane] = sc[lane];
+        reinterpret_cast<float*>(meta + 16)[kTile + half * 32 + lane] = vs;
+      } else if (!(h.y && h.x == 0xffffffffu)) {
         bool odd = false;
 #pragma unroll 1
         for (int it = 0; it < 32 / kRpi; ++it) {
@@ -254,7 +268,7 @@ __device__ void produce(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
           if (here) *w = make_uint4(x[0], x[1], x[2], x[3]);
           odd |= here;
         }
-        if (odd) atomicOr(&bars->odd, h.plain ? 2 : 1);
+        if (odd) atomicOr(&bars->odd, h.y ? 2 : 1);
       }
     }
     fence_proxy_async_smem();
@@ -265,15 +279,15 @@ __device__ void produce(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
     return true;
   };
   bool ok = true;
-  while (ok && more && f_tile < kAhead) ok = fetch(held[f_tile % (kAhead + 1)]);
+  while (ok && more && f_tile < kAhead) ok = fetch();
   while (ok && more) {
-    ok = fetch(held[f_tile % (kAhead + 1)]);
+    ok = fetch();
     if (!ok) break;
     cp_wait<kAhead>();
-    ok = hand_over(held[done % (kAhead + 1)]);
+    ok = hand_over();
   }
   cp_wait<0>();
-  while (ok && done < f_tile) ok = hand_over(held[done % (kAhead + 1)]);
+  while (ok && done < f_tile) ok = hand_over();
 }
 
 // ------------------------------------------------------------ issuers
@@ -532,11 +546,15 @@ __device__ void softmax(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
       const float nmb = m_used == -INFINITY ? 0.f : -m_used;
       const uint64_t qs2 = f2_pack(qs, qs), nmb2 = f2_pack(nmb, nmb);
       uint64_t acc[4] = {0, 0, 0, 0};
-      uint32_t packed[kTile / 2];
       [[maybe_unused]] const float4* vs = reinterpret_cast<const float4*>(meta + 16 + 4 * kTile);
       const uint64_t unit2 = f2_pack(unit, unit);
+      // Weights go to TMEM 32 columns at a time (over this tile's scores, which are in
+      // registers), so that few are held beside them.
 #pragma unroll
-      for (int c = 0; c < kTile; c += 4) {
+      for (int c0 = 0; c0 < kTile; c0 += 32) {
+      uint32_t packed[16];
+#pragma unroll
+      for (int c = c0; c < c0 + 32; c += 4) {
         float y[4];
         f2_unpack(f2_fma(f2_pack(x[c], x[c + 1]), qs2, nmb2), y[0], y[1]);
         f2_unpack(f2_fma(f2_pack(x[c + 2], x[c + 3]), qs2, nmb2), y[2], y[3]);
@@ -556,12 +574,14 @@ __device__ void softmax(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
 #pragma unroll
             for (int e = 0; e < 4; ++e) z[e] = y[e] == 0.f ? 0.f : z[e];
           }
-          packed[c >> 1] = pack16x2(z[0], z[1], false);
-          packed[(c >> 1) + 1] = pack16x2(z[2], z[3], false);
+          packed[(c - c0) >> 1] = pack16x2(z[0], z[1], false);
+          packed[((c - c0) >> 1) + 1] = pack16x2(z[2], z[3], false);
         } else {
-          packed[c >> 1] = pack16x2(y[0], y[1], std::is_same_v<X, __nv_bfloat16>);
-          packed[(c >> 1) + 1] = pack16x2(y[2], y[3], std::is_same_v<X, __nv_bfloat16>);
+          packed[(c - c0) >> 1] = pack16x2(y[0], y[1], std::is_same_v<X, __nv_bfloat16>);
+          packed[((c - c0) >> 1) + 1] = pack16x2(y[2], y[3], std::is_same_v<X, __nv_bfloat16>);
         }
+      }
+      tmem_st16(s_addr + (c0 >> 1), packed);
       }
       {
         float s0, s1;
@@ -584,7 +604,6 @@ __device__ void softmax(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
         }
         tmem_wait_st();
       }
-      tmem_st32(s_addr, packed);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -734,9 +753,7 @@ __global__ void __launch_bounds__(TcCfg<T, ST, D, MT>::kThreads, 1) paged_tc_ker
   clear_unused<T, C::kThreads>(a);
   const int end = static_cast<int>(share.g1 - share.g0);
   constexpr uint32_t fmt = std::is_same_v<typename C::X, __nv_bfloat16> ? 1u : 0u;
-  // Registers: the launch's 512 x 128 (MT = 2) go 168 to a softmax thread, 88 to the others.
   if (warp < 8) {
-    if constexpr (MT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (work) {
       if (warp == 0) {
         if (lane == 0) issue_scores<C>(a, cur, end, smem, bars, tmem, fmt);
@@ -747,7 +764,6 @@ __global__ void __launch_bounds__(TcCfg<T, ST, D, MT>::kThreads, 1) paged_tc_ker
       }
     }
   } else {
-    if constexpr (MT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     if (work) softmax<T, ST, C>(a, cur, end, smem, bars, tmem);
   }
   __syncwarp();
