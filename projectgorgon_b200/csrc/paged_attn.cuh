@@ -52,6 +52,7 @@ struct PagedAttn {
   float2* part_ml;    // [grid * 2][m]  running max (log2 units) and sum
   struct CutUnit* cut;  // [grid]
   uint64_t wait_ns;
+  int tma;            // (tcgen05) pages come by TMA
 };
 
 // n / group for 0 <= n < 2^31, by a multiplication (m = floor(2^32 (2^s - group)
@@ -323,8 +324,8 @@ __device__ __forceinline__ int tree_bits(const PagedAttn& a, const Seq& s, int b
 
 // Launches a kernel so that it may start while the one before it in the stream
 // ends (it waits for that itself, by griddepcontrol.wait).
-template <typename K>
-int launch_early(K kern, const PagedAttn& a, int threads, int smem, cudaStream_t st, int grid_y = 1) {
+template <typename K, typename... More>
+int launch_early(K kern, const PagedAttn& a, int threads, int smem, cudaStream_t st, int grid_y = 1, const More&... more) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(a.grid), static_cast<unsigned>(grid_y));
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
@@ -335,7 +336,7 @@ int launch_early(K kern, const PagedAttn& a, int threads, int smem, cudaStream_t
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, kern, a), "gorgon_paged_attn launch");
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, a, more...), "gorgon_paged_attn launch");
 }
 
 int launch_paged_simt(const PagedAttn& a, cudaStream_t st);

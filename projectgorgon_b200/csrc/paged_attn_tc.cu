@@ -6,17 +6,20 @@
 // tile list (paged_attn.cuh).  Warp roles:
 //   warp 0        Q K^T issuer (one thread)
 //   warp 1        P V issuer (one thread); the warp allocates TMEM
-//   warps 2, 3    idle
-//   warps 4, 5    K producers, 32 rows of every tile each
-//   warps 6, 7    V producers
+//   warps 2, 3    TMA loads of K and V tiles (one thread each)
+//   warps 4, 5    K, 32 rows of every tile each
+//   warps 6, 7    V
 //   warps 8 - 11  softmax and epilogue of M-tile 0, a thread per row
 //   warps 12 - 15 (MT = 2) of M-tile 1
-// The producers gather rows one by one (pages of any size and stride) with
-// 16-byte cp.async copies into the SW128 tiles that the products read; 8-bit
-// rows go to a ring of raw bytes first, and each producer widens its 32 rows
-// from there to f16, exactly (paged_widen.cuh), so that the products see the
-// stored numbers and the scales are applied in fp32: K's to the scores, V's to
-// the weights.  Rows that no row of the unit sees are not read; they are zeros.
+// Pages of 8, 16, 32 rows or a multiple of 64 come by TMA, a box per page (or
+// per 64 rows of one) and 128-byte column block.  16-bit rows land in the SW128
+// tiles that the products read.  8-bit rows land in a ring of raw bytes, and
+// warps 4 to 7 widen their 32 rows from there to f16, exactly (paged_widen.cuh),
+// so that the products see the stored numbers and the scales are applied in
+// fp32: K's to the scores, V's to the weights.  Pages of other sizes are
+// gathered row by row by warps 4 to 7 with 16-byte cp.async copies (which took
+// 1700 cycles a tile of 2300, most of them waiting for issue slots, so TMA is
+// used where it can be).  V rows that no row of the unit sees are made zeros.
 //
 // Softmax per row is owned by one thread (TMEM lane = row): no shuffles.  The
 // running max moves only when a tile's max exceeds it by more than 8 (log2
@@ -31,6 +34,10 @@
 // the CTA drains its copies and products, frees TMEM and returns.
 #include <algorithm>
 #include <type_traits>
+
+#include <cuda.h>
+
+#include <mutex>
 
 #include "attn_tc_common.cuh"
 #include "paged_attn.cuh"
@@ -59,13 +66,14 @@ struct TcCfg {
   static constexpr uint32_t kTileBytes = kHalves * kBlock;
   static constexpr int kStages = kWide ? (MT == 2 ? 4 : 5) : 3;
   static constexpr int kRawStages = kWide ? 0 : (MT == 2 ? 3 : 5);
-  static constexpr uint32_t kRawBytes = 32 * D + 256;    // a producer's rows of a tile, their K and V scales
+  static constexpr uint32_t kRawRows = 32 * D;           // bytes of a producer's 32 rows
+  static constexpr uint32_t kRawBytes = 2 * kRawRows + 512;  // a tile of K or V, and (cp.async) its K and V scales
   static constexpr int kInfo = 8;                        // (more than the tiles a producer has in flight)
   static constexpr int kLag = kWide ? kStages - 2 : 0;   // tiles in flight behind the newest
   static constexpr uint32_t kOffK = MT * kQTile;
   static constexpr uint32_t kOffV = kOffK + kStages * kTileBytes;
-  static constexpr uint32_t kOffRaw = kOffV + kStages * kTileBytes;         // [4 producers][stages]
-  static constexpr uint32_t kOffMeta = kOffRaw + 4 * kRawStages * kRawBytes;  // [stages] Meta
+  static constexpr uint32_t kOffRaw = kOffV + kStages * kTileBytes;         // [K, V][stages]
+  static constexpr uint32_t kOffMeta = kOffRaw + 2 * kRawStages * kRawBytes;  // [stages] Meta
   static constexpr uint32_t kMetaBytes = kWide ? 16 : 16 + 8 * kTile;       // 2 words of valid keys, max V scale x 2; K and V scales
   static constexpr uint32_t kOffBits = kOffMeta + kStages * kMetaBytes;     // [M][8] ancestor words
   static constexpr uint32_t kOffQs = kOffBits + M * (kMaxTree / 32) * 4;    // [M] undoes Q's power of two
@@ -78,6 +86,8 @@ struct TcCfg {
 template <typename C>
 struct TcBars {
   uint64_t k_full[C::kStages], k_empty[C::kStages], v_full[C::kStages], v_empty[C::kStages];
+  // TMA: 16-bit V tiles land, 8-bit K and V tiles land, and their raw bytes are done with
+  uint64_t land[2][C::kWide ? C::kStages : C::kRawStages], raw_empty[2][C::kWide ? 1 : C::kRawStages];
   uint64_t q_full;
   uint64_t s_full[2 * C::MT], p_full[2 * C::MT];  // buf * MT + mt
   uint64_t p_free[2];
@@ -132,7 +142,222 @@ __device__ __forceinline__ uint64_t bit_range(int lo, int hi) {
   return up & ~((1ull << lo) - 1);
 }
 
-// ------------------------------------------------------------ producers
+// ------------------------------------------------------------ tiles
+// A producer's 32 rows of raw bytes (row-major at src) to the f16 tile at st;
+// rows without their bit in `keep` become zeros.
+template <int ST, typename C>
+__device__ __forceinline__ void widen_rows(const uint8_t* src, uint8_t* st, int half, uint32_t keep) {
+  constexpr int kRow = C::D, kCpr = kRow / 16, kRpi = 32 / kCpr;
+  const int lane = threadIdx.x & 31, piece = lane % kCpr, rsub = lane / kCpr;
+  uint8_t* blk = st + (piece >> 2) * C::kBlock;
+#pragma unroll 4
+  for (int it = 0; it < 32 / kRpi; ++it) {
+    const int r = it * kRpi + rsub;
+    uint4 w = *reinterpret_cast<const uint4*>(src + r * kRow + piece * 16);
+    if (!((keep >> r) & 1u)) w = make_uint4(0, 0, 0, 0);
+    uint32_t x[8];
+    widen_word<ST>(w.x, x[0], x[1]);
+    widen_word<ST>(w.y, x[2], x[3]);
+    widen_word<ST>(w.z, x[4], x[5]);
+    widen_word<ST>(w.w, x[6], x[7]);
+    *reinterpret_cast<uint4*>(blk + sw128(half * 32 + r, (2 * piece) & 7)) = make_uint4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<uint4*>(blk + sw128(half * 32 + r, (2 * piece + 1) & 7)) = make_uint4(x[4], x[5], x[6], x[7]);
+  }
+}
+
+// Takes infinities and NaN out of 32 rows of a 16-bit V tile (rows without their
+// bit in `keep` become zeros); true on lanes that found some in kept rows.
+template <typename T, typename C>
+__device__ __forceinline__ bool strip_rows(uint8_t* st, int half, uint32_t keep) {
+  constexpr int kCpr = C::D / 8, kRpi = 32 / kCpr;
+  const int lane = threadIdx.x & 31, piece = lane % kCpr, rsub = lane / kCpr;
+  bool odd = false;
+#pragma unroll 1
+  for (int it = 0; it < 32 / kRpi; ++it) {
+    const int r = it * kRpi + rsub;
+    uint4* w = reinterpret_cast<uint4*>(st + (piece >> 3) * C::kBlock + sw128(half * 32 + r, piece & 7));
+    uint32_t x[4] = {w->x, w->y, w->z, w->w};
+    constexpr uint32_t top = std::is_same_v<T, __half> ? 0x7c00u : 0x7f80u;
+    const bool kept = (keep >> r) & 1u;
+    bool here = !kept;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (!kept) x[e] = 0;
+      if ((x[e] & top) == top) {
+        x[e] &= 0xffff0000u;
+        odd = here = true;
+      }
+      if (((x[e] >> 16) & top) == top) {
+        x[e] &= 0xffffu;
+        odd = here = true;
+      }
+    }
+    if (here) *w = make_uint4(x[0], x[1], x[2], x[3]);
+  }
+  return odd;
+}
+
+// The half's valid word and (8-bit) scales for the softmax.
+template <typename C>
+__device__ __forceinline__ void write_meta(uint8_t* smem, uint32_t stage, int half, uint32_t valid, float ks, float vs) {
+  const int lane = threadIdx.x & 31;
+  uint8_t* meta = smem + C::kOffMeta + stage * C::kMetaBytes;
+  if (lane == 0) reinterpret_cast<uint32_t*>(meta)[half] = valid;
+  if constexpr (!C::kWide) {
+    float top = vs;  // (NaN never wins)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) reinterpret_cast<float*>(meta)[2 + half] = top;
+    reinterpret_cast<float*>(meta + 16)[half * 32 + lane] = ks;
+    reinterpret_cast<float*>(meta + 16)[kTile + half * 32 + lane] = vs;
+  }
+}
+
+// Rows of a page that one TMA box covers, 0 when pages of this size go row by row.
+__host__ __device__ __forceinline__ int box_rows(int page_size) {
+  return page_size % kTile == 0 ? kTile : page_size >= 8 && kTile % page_size == 0 ? page_size : 0;
+}
+
+// ------------------------------------------------------------ TMA loads
+template <typename C>
+__device__ void load_tiles(const PagedAttn& a, const CUtensorMap* map, TileCursor f, int end, uint8_t* smem, TcBars<C>* bars, int is_v) {
+  constexpr int kSlots = C::kWide ? C::kStages : C::kRawStages;
+  const int lane = threadIdx.x & 31;
+  volatile int* abort = &bars->abort;
+  uint64_t* full = C::kWide && !is_v ? bars->k_full : bars->land[is_v];
+  uint64_t* empty = C::kWide ? (is_v ? bars->v_empty : bars->k_empty) : bars->raw_empty[is_v];
+  uint8_t* ring = smem + (C::kWide ? (is_v ? C::kOffV : C::kOffK) : C::kOffRaw + is_v * C::kRawStages * C::kRawBytes);
+  constexpr uint32_t kSlotBytes = C::kWide ? C::kTileBytes : C::kRawBytes;
+  const int R = box_rows(a.pool.page_size), boxes = kTile / R;
+  const uint32_t box_bytes = static_cast<uint32_t>(R) * (C::kWide ? C::D * 2 : C::D);
+  int page = -2, row = 0;  // of box `lane` of the next tile
+  auto look_up = [&]() {
+    page = -2;
+    const int p = f.tile() * kTile + lane * R;
+    if (lane < boxes && p < f.u.hi && (p + R > f.u.lo || p < f.u.s_end)) {
+      int col;
+      a.pool.split(p, col, row);
+      page = __ldg(a.pool.table + static_cast<int64_t>(f.b) * a.pool.table_sb + col);
+    }
+  };
+  look_up();
+  Slot<kSlots> s;
+  int64_t issued = 0;
+  bool more = true;
+  while (more) {
+    if (!warp_wait(&empty[s.stage], s.phase ^ 1u, abort, a.wait_ns)) break;
+    const uint32_t go = __ballot_sync(0xffffffffu, page >= 0 && page < a.pool.num_pages);  // (the row lookups report bad pages)
+    if (lane == 0) mbar_arrive_expect_tx(&full[s.stage], __popc(go) * box_bytes);
+    __syncwarp();
+    uint8_t* dst = ring + s.stage * kSlotBytes;
+    for (int x = 0; x < boxes; ++x) {
+      const int pg = __shfl_sync(0xffffffffu, page, x), r = __shfl_sync(0xffffffffu, row, x);
+      if (!((go >> x) & 1u)) continue;
+      if (lane == 0) {
+        if constexpr (C::kWide) {
+#pragma unroll
+          for (int h = 0; h < C::kHalves; ++h)
+            tma_load_4d(dst + h * C::kBlock + x * R * 128, map, &full[s.stage], h * 64, r, f.kvh, pg);
+        } else {
+          tma_load_4d(dst + x * R * C::D, map, &full[s.stage], 0, r, f.kvh, pg);
+        }
+      }
+    }
+    ++issued;
+    s.next();
+    more = f.next(a, end);
+    if (more) look_up();
+  }
+  // Every issued load must land before the CTA leaves.
+  if (lane == 0)
+    for (int64_t k = issued > kSlots ? issued - kSlots : 0; k < issued; ++k)
+      drain_wait(&full[k % kSlots], static_cast<uint32_t>(k / kSlots) & 1u);
+}
+
+// What is left to do for 32 rows of every tile that lands by TMA: their valid
+// word and scales, hidden rows of 16-bit V, widening of 8-bit rows.
+template <typename T, int ST, typename C>
+__device__ void finish_tiles(const PagedAttn& a, TileCursor f, int end, uint8_t* smem, TcBars<C>* bars, int is_v, int half) {
+  const int lane = threadIdx.x & 31;
+  volatile int* abort = &bars->abort;
+  uint64_t* full = is_v ? bars->v_full : bars->k_full;
+  uint64_t* empty = is_v ? bars->v_empty : bars->k_empty;
+  uint8_t* ring = smem + (is_v ? C::kOffV : C::kOffK);
+  // This lane's row: its page two tiles ahead, its scales one tile ahead, so that nothing waits for them.
+  int page = -2, row = 0, kvh = 0;
+  auto look_up = [&]() {
+    page = -2;
+    kvh = f.kvh;
+    const int j = f.tile() * kTile + half * 32 + lane;
+    if (f.u.wanted(j)) {
+      int col;
+      a.pool.split(j, col, row);
+      page = __ldg(a.pool.table + static_cast<int64_t>(f.b) * a.pool.table_sb + col);
+    }
+  };
+  bool held = false;
+  float ks = 0.f, vs = 0.f;
+  auto take = [&]() {  // the looked-up page's validity and scales
+    held = page >= 0 && page < a.pool.num_pages;
+    if (page != -2 && !held) raise_device_error(a.pool.err, kErrBadPage);
+    if constexpr (!C::kWide) {
+      ks = vs = 0.f;
+      if (is_v && held) {
+        ks = __ldg(a.pool.ks + page * a.pool.ks_sp + kvh * a.pool.ks_sh + row * a.pool.ks_ss);
+        vs = __ldg(a.pool.vs + page * a.pool.vs_sp + kvh * a.pool.vs_sh + row * a.pool.vs_ss);
+      }
+    }
+  };
+  bool plain = Common(a, f).plain(a, f.tile() * kTile), next_plain = false;
+  look_up();
+  take();
+  bool more = f.next(a, end);
+  if (more) {
+    next_plain = Common(a, f).plain(a, f.tile() * kTile);
+    look_up();
+  }
+  constexpr int kSlots = C::kWide ? C::kStages : C::kRawStages;
+  Slot<kSlots> ls;
+  Slot<C::kStages> hs;
+  while (true) {
+    const uint32_t valid = __ballot_sync(0xffffffffu, held);
+    const float k1 = ks, v1 = vs;
+    const bool p1 = plain, again = more;
+    if (more) {  // the next tile's scales, and the page of the one after
+      take();
+      plain = next_plain;
+      more = f.next(a, end);
+      if (more) {
+        next_plain = Common(a, f).plain(a, f.tile() * kTile);
+        look_up();
+      }
+    }
+    if (!warp_wait(&bars->land[is_v][ls.stage], ls.phase, abort, a.wait_ns)) return;
+    uint8_t* st = ring + hs.stage * C::kTileBytes;
+    if constexpr (C::kWide) {
+      if (!(p1 && valid == 0xffffffffu)) {
+        if (strip_rows<T, C>(st, half, valid)) atomicOr(&bars->odd, p1 ? 2 : 1);
+        fence_proxy_async_smem();
+      }
+    } else {
+      if (!warp_wait(&empty[hs.stage], hs.phase ^ 1u, abort, a.wait_ns)) return;
+      const uint8_t* src = smem + C::kOffRaw + (is_v * C::kRawStages + ls.stage) * C::kRawBytes + half * C::kRawRows;
+      widen_rows<ST, C>(src, st, half, is_v ? valid : 0xffffffffu);
+      fence_proxy_async_smem();
+    }
+    if (is_v) write_meta<C>(smem, hs.stage, half, valid, k1, v1);
+    __syncwarp();
+    if (lane == 0) {
+      if constexpr (!C::kWide) mbar_arrive(&bars->raw_empty[is_v][ls.stage]);
+      mbar_arrive(&full[hs.stage]);
+    }
+    ls.next();
+    hs.next();
+    if (!again) return;
+  }
+}
+
+// ------------------------------------------------------------ row by row
 // One of the two warps that fetch K (is_v 0) or V rows; `half` picks its 32 of a tile's rows.
 template <typename T, int ST, typename C>
 __device__ void produce(const PagedAttn& a, TileCursor cur, int end, uint8_t* smem, TcBars<C>* bars, int is_v, int half) {
@@ -141,7 +366,7 @@ __device__ void produce(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
   uint64_t* full = is_v ? bars->v_full : bars->k_full;
   uint64_t* empty = is_v ? bars->v_empty : bars->k_empty;
   uint8_t* ring = smem + (is_v ? C::kOffV : C::kOffK);
-  uint8_t* raw = smem + C::kOffRaw + (is_v * 2 + half) * C::kRawStages * C::kRawBytes;
+  uint8_t* raw = smem + C::kOffRaw + is_v * C::kRawStages * C::kRawBytes;
   const int64_t sp = is_v ? a.pool.v_sp : a.pool.k_sp, ss = is_v ? a.pool.v_ss : a.pool.k_ss, sh = is_v ? a.pool.v_sh : a.pool.k_sh;
   const char* pages = is_v ? a.pool.v : a.pool.k;
   constexpr int kRow = C::kWide ? C::D * 2 : C::D;       // bytes of a row
@@ -191,13 +416,13 @@ __device__ void produce(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
       if constexpr (C::kWide)
         at = smem_u32(ring + fs.stage * C::kTileBytes + (piece >> 3) * C::kBlock) + sw128(half * 32 + r, piece & 7);
       else
-        at = smem_u32(raw + (f_tile % C::kRawStages) * C::kRawBytes) + r * kRow + piece * 16;
+        at = smem_u32(raw + (f_tile % C::kRawStages) * C::kRawBytes) + half * C::kRawRows + r * kRow + piece * 16;
       cp16(at, base + o, (valid >> r) & 1u);
     }
     if constexpr (!C::kWide) {
       if (is_v) {
         const int64_t pg = page >= 0 ? page : 0, pr = page >= 0 ? prow : 0;
-        const uint32_t at = smem_u32(raw + (f_tile % C::kRawStages) * C::kRawBytes) + 32 * kRow + lane * 4;
+        const uint32_t at = smem_u32(raw + (f_tile % C::kRawStages) * C::kRawBytes) + 2 * C::kRawRows + half * 256 + lane * 4;
         cp4(at, a.pool.ks + pg * a.pool.ks_sp + f.kvh * a.pool.ks_sh + pr * a.pool.ks_ss, page >= 0);
         cp4(at + 128, a.pool.vs + pg * a.pool.vs_sp + f.kvh * a.pool.vs_sh + pr * a.pool.vs_ss, page >= 0);
       }
@@ -218,58 +443,18 @@ __device__ void produce(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
     __syncwarp();  // every lane's copies
     if constexpr (!C::kWide) {
       if (!warp_wait(&empty[hs.stage], hs.phase ^ 1u, abort, a.wait_ns)) return false;
-      const uint8_t* src = raw + (done % C::kRawStages) * C::kRawBytes;
-#pragma unroll
-      for (int it = 0; it < 32 / kRpi; ++it) {
-        const int r = it * kRpi + rsub;
-        const uint4 w = *reinterpret_cast<const uint4*>(src + r * kRow + piece * 16);
-        uint32_t x[8];
-        widen_word<ST>(w.x, x[0], x[1]);
-        widen_word<ST>(w.y, x[2], x[3]);
-        widen_word<ST>(w.z, x[4], x[5]);
-        widen_word<ST>(w.w, x[6], x[7]);
-        uint8_t* blk = st + (piece >> 2) * C::kBlock;
-        *reinterpret_cast<uint4*>(blk + sw128(half * 32 + r, (2 * piece) & 7)) = make_uint4(x[0], x[1], x[2], x[3]);
-        *reinterpret_cast<uint4*>(blk + sw128(half * 32 + r, (2 * piece + 1) & 7)) = make_uint4(x[4], x[5], x[6], x[7]);
-      }
+      widen_rows<ST, C>(raw + (done % C::kRawStages) * C::kRawBytes + half * C::kRawRows, st, half, h.x);
     }
     if (is_v) {
-      uint8_t* meta = smem + C::kOffMeta + hs.stage * C::kMetaBytes;
-      if (lane == 0) reinterpret_cast<uint32_t*>(meta)[half] = h.x;
+      float ks = 0.f, vs = 0.f;
       if constexpr (!C::kWide) {
-        const float* sc = reinterpret_cast<const float*>(raw + (done % C::kRawStages) * C::kRawBytes + 32 * kRow);
-        const float vs = sc[32 + lane];
-        float top = vs;  // (NaN never wins)
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (lane == 0) reinterpret_cast<float*>(meta)[2 + half] = top;
-        reinterpret_cast<float*>(meta + 16)[half * 32 + lane] = sc[lane];
-        reinterpret_cast<float*>(meta + 16)[kTile + half * 32 + lane] = vs;
+        const float* sc = reinterpret_cast<const float*>(raw + (done % C::kRawStages) * C::kRawBytes + 2 * C::kRawRows + half * 256);
+        ks = sc[lane];
+        vs = sc[32 + lane];
       } else if (!(h.y && h.x == 0xffffffffu)) {
-        bool odd = false;
-#pragma unroll 1
-        for (int it = 0; it < 32 / kRpi; ++it) {
-          const int r = half * 32 + it * kRpi + rsub;
-          uint4* w = reinterpret_cast<uint4*>(st + (piece >> 3) * C::kBlock + sw128(r, piece & 7));
-          uint32_t x[4] = {w->x, w->y, w->z, w->w};
-          constexpr uint32_t top = std::is_same_v<T, __half> ? 0x7c00u : 0x7f80u;
-          bool here = false;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if ((x[e] & top) == top) {
-              x[e] &= 0xffff0000u;
-              here = true;
-            }
-            if (((x[e] >> 16) & top) == top) {
-              x[e] &= 0xffffu;
-              here = true;
-            }
-          }
-          if (here) *w = make_uint4(x[0], x[1], x[2], x[3]);
-          odd |= here;
-        }
-        if (odd) atomicOr(&bars->odd, h.y ? 2 : 1);
+        if (strip_rows<T, C>(st, half, h.x)) atomicOr(&bars->odd, h.y ? 2 : 1);
       }
+      write_meta<C>(smem, hs.stage, half, h.x, ks, vs);
     }
     fence_proxy_async_smem();
     __syncwarp();
@@ -708,20 +893,27 @@ __device__ void softmax(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
 }
 
 template <typename T, int ST, int D, int MT>
-__global__ void __launch_bounds__(TcCfg<T, ST, D, MT>::kThreads, 1) paged_tc_kernel(const __grid_constant__ PagedAttn a) {
+__global__ void __launch_bounds__(TcCfg<T, ST, D, MT>::kThreads, 1) paged_tc_kernel(const __grid_constant__ PagedAttn a,
+                const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using C = TcCfg<T, ST, D, MT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   TcBars<C>* bars = reinterpret_cast<TcBars<C>*>(smem + C::kOffBar);
   static_assert(sizeof(TcBars<C>) <= 1024, "barrier block");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (a.tma && (warp == 2 || warp == 3) && lane == 0) prefetch_tensormap(warp == 3 ? &vmap : &kmap);
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(&bars->k_full[s], 2);   // the two producer warps
+      mbar_init(&bars->k_full[s], a.tma && C::kWide ? 1 : 2);  // the TMA thread, or the two warps of its rows
       mbar_init(&bars->k_empty[s], 1);
       mbar_init(&bars->v_full[s], 2);
       mbar_init(&bars->v_empty[s], 1);
     }
+    for (int v = 0; v < 2; ++v)
+      for (int s = 0; s < (C::kWide ? C::kStages : C::kRawStages); ++s) {
+        mbar_init(&bars->land[v][s], 1);
+        if (!C::kWide) mbar_init(&bars->raw_empty[v][s], 2);
+      }
     mbar_init(&bars->q_full, 4 * MT);
     for (int b = 0; b < 2 * MT; ++b) {
       mbar_init(&bars->s_full[b], 1);
@@ -759,7 +951,11 @@ __global__ void __launch_bounds__(TcCfg<T, ST, D, MT>::kThreads, 1) paged_tc_ker
         if (lane == 0) issue_scores<C>(a, cur, end, smem, bars, tmem, fmt);
       } else if (warp == 1) {
         if (lane == 0) issue_outputs<C>(a, cur, end, smem, bars, tmem, fmt);
-      } else if (warp >= 4) {
+      } else if (warp < 4) {
+        if (a.tma) load_tiles<C>(a, warp == 3 ? &vmap : &kmap, cur, end, smem, bars, warp - 2);
+      } else if (a.tma) {
+        if (!C::kWide || warp >= 6) finish_tiles<T, ST, C>(a, cur, end, smem, bars, (warp - 4) >> 1, warp & 1);
+      } else {
         produce<T, ST, C>(a, cur, end, smem, bars, (warp - 4) >> 1, warp & 1);
       }
     }
@@ -774,6 +970,41 @@ __global__ void __launch_bounds__(TcCfg<T, ST, D, MT>::kThreads, 1) paged_tc_ker
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
   }
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encoder() {
+  static EncodeFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeFn>(p);
+  });
+  return fn;
+}
+
+// The pages of K or V as a 4-D tensor (column, row in the page, head, page);
+// false where TMA does not take the layout, and rows are gathered instead.
+bool page_map(const PagedAttn& a, bool v, CUtensorMap* map) {
+  EncodeFn enc = encoder();
+  if (!enc || a.pool.num_pages < 1) return false;
+  const bool wide = a.pool.storage == GORGON_KV_NATIVE;
+  const int64_t sp = v ? a.pool.v_sp : a.pool.k_sp, sh = v ? a.pool.v_sh : a.pool.k_sh, ss = v ? a.pool.v_ss : a.pool.k_ss;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.pool.d), static_cast<cuuint64_t>(a.pool.page_size),
+                              static_cast<cuuint64_t>(a.pool.hkv), static_cast<cuuint64_t>(a.pool.num_pages)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(ss), static_cast<cuuint64_t>(sh), static_cast<cuuint64_t>(sp)};
+  const cuuint32_t box[4] = {wide ? 64u : static_cast<cuuint32_t>(a.pool.d), static_cast<cuuint32_t>(box_rows(a.pool.page_size)), 1, 1};
+  const cuuint32_t step[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType dt = !wide ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                 : a.pool.dtype == GORGON_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return enc(map, dt, 4, v ? a.pool.v : a.pool.k, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             wide ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename F>
@@ -809,7 +1040,10 @@ void paged_tc_plan(PagedAttn* a) {
   a->grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sm_count(), tiles)));
 }
 
-int launch_paged_tc(const PagedAttn& a, cudaStream_t st) {
+int launch_paged_tc(const PagedAttn& args, cudaStream_t st) {
+  PagedAttn a = args;
+  CUtensorMap kmap{}, vmap{};
+  a.tma = box_rows(a.pool.page_size) > 0 && page_map(a, false, &kmap) && page_map(a, true, &vmap);
   return by_config(a, [&](auto t, auto s, auto d, auto mt) {
     using C = TcCfg<decltype(t), decltype(s)::value, decltype(d)::value, decltype(mt)::value>;
     auto kern = paged_tc_kernel<decltype(t), decltype(s)::value, decltype(d)::value, decltype(mt)::value>;
@@ -817,7 +1051,7 @@ int launch_paged_tc(const PagedAttn& a, cudaStream_t st) {
     static_assert(smem <= 232448, "shared memory per block");
     int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "gorgon_paged_attn smem attribute");
     if (rc) return rc;
-    return launch_early(kern, a, C::kThreads, smem, st);
+    return launch_early(kern, a, C::kThreads, smem, st, 1, kmap, vmap);
   });
 }
 
