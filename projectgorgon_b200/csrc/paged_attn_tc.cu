@@ -70,6 +70,9 @@ struct TcCfg {
   static constexpr uint32_t kRawBytes = 2 * kRawRows + 512;  // a tile of K or V, and (cp.async) its K and V scales
   static constexpr int kInfo = 8;                        // (more than the tiles a producer has in flight)
   static constexpr int kLag = kWide ? kStages - 2 : 0;   // tiles in flight behind the newest
+  // With two M-tiles each softmax warpgroup frees a K stage once it has seen its
+  // scores, which takes a commit off the Q K^T issuer, the busiest thread.
+  static constexpr bool kSoftmaxFreesK = MT == 2;
   static constexpr uint32_t kOffK = MT * kQTile;
   static constexpr uint32_t kOffV = kOffK + kStages * kTileBytes;
   static constexpr uint32_t kOffRaw = kOffV + kStages * kTileBytes;         // [K, V][stages]
@@ -78,7 +81,8 @@ struct TcCfg {
   static constexpr uint32_t kOffBits = kOffMeta + kStages * kMetaBytes;     // [M][8] ancestor words
   static constexpr uint32_t kOffQs = kOffBits + M * (kMaxTree / 32) * 4;    // [M] undoes Q's power of two
   static constexpr uint32_t kOffInfo = kOffQs + M * 4;                      // [4 producers][kInfo] valid keys, plain
-  static constexpr uint32_t kOffBar = (kOffInfo + 4 * kInfo * 8 + 15) / 16 * 16;
+  static constexpr uint32_t kOffCur = kOffInfo + 4 * kInfo * 8;             // [softmax warps] TileCursor
+  static constexpr uint32_t kOffBar = (kOffCur + 4 * MT * static_cast<uint32_t>(sizeof(TileCursor)) + 15) / 16 * 16;
   static constexpr uint32_t kSmem = kOffBar + 512 + 1024;                   // + alignment slack
   static_assert(kSmem <= 232448, "shared memory per block");
 };
@@ -90,7 +94,8 @@ struct TcBars {
   uint64_t land[2][C::kWide ? C::kStages : C::kRawStages], raw_empty[2][C::kWide ? 1 : C::kRawStages];
   uint64_t q_full;
   uint64_t s_full[2 * C::MT], p_full[2 * C::MT];  // buf * MT + mt
-  uint64_t p_free[2];
+  uint64_t p_free[2];            // every M-tile's P V of the buffer has completed
+  int bad;   // a wanted page is out of the pool: tiles are checked for it
   uint64_t drain[2];
   uint32_t tmem_base;
   int abort;
@@ -246,7 +251,12 @@ __device__ void load_tiles(const PagedAttn& a, const CUtensorMap* map, TileCurso
   bool more = true;
   while (more) {
     if (!warp_wait(&empty[s.stage], s.phase ^ 1u, abort, a.wait_ns)) break;
-    const uint32_t go = __ballot_sync(0xffffffffu, page >= 0 && page < a.pool.num_pages);  // (the row lookups report bad pages)
+    const uint32_t go = __ballot_sync(0xffffffffu, page >= 0 && page < a.pool.num_pages);
+    if (page != -2 && !((go >> lane) & 1u)) {
+      raise_device_error(a.pool.err, kErrBadPage);
+      *reinterpret_cast<volatile int*>(&bars->bad) = 1;
+    }
+    __syncwarp();
     if (lane == 0) mbar_arrive_expect_tx(&full[s.stage], __popc(go) * box_bytes);
     __syncwarp();
     uint8_t* dst = ring + s.stage * kSlotBytes;
@@ -402,6 +412,7 @@ __device__ void produce(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
     const int prow = next_row;
     if (page != -2 && (page < 0 || page >= a.pool.num_pages)) {
       raise_device_error(a.pool.err, kErrBadPage);
+      *reinterpret_cast<volatile int*>(&bars->bad) = 1;  // before the tile is handed over
       page = -2;
     }
     const uint32_t valid = __ballot_sync(0xffffffffu, page >= 0);
@@ -489,9 +500,14 @@ __device__ void issue_scores(const PagedAttn& a, TileCursor cur, int end, uint8_
     if (!spin_wait(&bars->q_full, unit & 1u, abort, a.wait_ns)) break;
     ++unit;
     const int n = min(cur.u.tiles - cur.i, end - cur.at);
-    for (int t = 0; t < n; ++t, ++i) {
-      if (!spin_wait(&bars->k_full[kr.stage], kr.phase, abort, a.wait_ns) ||
-          (i >= 2 && !spin_wait(&bars->p_free[i & 1u], ((i - 2) >> 1) & 1u, abort, a.wait_ns))) {
+    for (int t = 0; t < n && ok; ++t, ++i) {
+      // Both probes before either result is used: the round trips overlap when the
+      // K tile and the S buffer (its weights of two tiles ago) are ready, as they usually are.
+      const uint32_t pf = ((i - 2) >> 1) & 1u;
+      const bool k_ready = mbar_test_wait(&bars->k_full[kr.stage], kr.phase);
+      const bool p_ready = i < 2 || mbar_test_wait(&bars->p_free[i & 1u], pf);
+      if (!(k_ready && p_ready) && (!spin_wait(&bars->k_full[kr.stage], kr.phase, abort, a.wait_ns) ||
+                                    (i >= 2 && !spin_wait(&bars->p_free[i & 1u], pf, abort, a.wait_ns)))) {
         ok = false;
         break;
       }
@@ -506,7 +522,7 @@ __device__ void issue_scores(const PagedAttn& a, TileCursor cur, int end, uint8_
                       ks > 0 ? 1u : 0u);
         umma_commit(&bars->s_full[(i & 1u) * C::MT + mt]);
       }
-      umma_commit(&bars->k_empty[kr.stage]);
+      if (!C::kSoftmaxFreesK) umma_commit(&bars->k_empty[kr.stage]);
       kr.next();
     }
     cur.at += n - 1;
@@ -581,7 +597,7 @@ __device__ __forceinline__ uint64_t row_word(const PagedAttn& a, const TileCurso
 }
 
 template <typename T, int ST, typename C>
-__device__ void softmax(const PagedAttn& a, TileCursor cur, int end, uint8_t* smem, TcBars<C>* bars, uint32_t tmem) {
+__device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, uint8_t* smem, TcBars<C>* bars, uint32_t tmem) {
   using X = typename C::X;
   constexpr bool kScaleQ = !C::kWide && std::is_same_v<T, __nv_bfloat16>;
   constexpr int MT = C::MT, D = C::D;
@@ -602,7 +618,11 @@ __device__ void softmax(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
     return q_tile + (j >> 3) * kQHalf + sw128(static_cast<uint32_t>(wq * 32 + rr), static_cast<uint32_t>(j & 7));
   };
   const bool vec_out = (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0 && ((a.o_sb | a.o_sh | a.o_sn) & 7) == 0;
-  int64_t i = 0;
+  // The warp's cursor lives in shared memory: the loop over tiles needs little of it.
+  TileCursor& cur = reinterpret_cast<TileCursor*>(smem + C::kOffCur)[(threadIdx.x >> 5) - 8];
+  if (lane == 0) cur = start;
+  __syncwarp();
+  uint32_t i = 0;
   Slot<C::kStages> vr;
   bool first_unit = true;
   bool cut_start = cur.i > 0;
@@ -671,12 +691,16 @@ __device__ void softmax(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
     // One tile of this row: scores to weights against the lazy running max.
     auto tile = [&](auto mask_tag, int j0, bool fresh) -> bool {
       constexpr bool kMask = decltype(mask_tag)::value;
-      const uint32_t bi = static_cast<uint32_t>(i & 1) * MT + wg;
-      const uint8_t* meta = smem + C::kOffMeta + vr.stage * C::kMetaBytes;
-      if (!warp_wait(&bars->v_full[vr.stage], vr.phase, abort, a.wait_ns)) return false;
+      const uint32_t bi = (i & 1u) * MT + wg;
+      [[maybe_unused]] const uint8_t* meta = smem + C::kOffMeta + vr.stage * C::kMetaBytes;
+      if (kMask || !C::kWide) {  // the tile's valid keys and scales
+        if (!warp_wait(&bars->v_full[vr.stage], vr.phase, abort, a.wait_ns)) return false;
+      }
       uint64_t vw = ~0ull;
       if (kMask) vw = row_word(a, cur, pos, row_ok, bits, j0) & *reinterpret_cast<const uint64_t*>(meta);
-      if (!warp_wait(&bars->s_full[bi], static_cast<uint32_t>(i >> 1) & 1u, abort, a.wait_ns)) return false;
+      if (!warp_wait(&bars->s_full[bi], (i >> 1) & 1u, abort, a.wait_ns)) return false;
+      if (!kMask && *reinterpret_cast<volatile int*>(&bars->bad)) return true;  // (the caller looks at it too)
+      if (C::kSoftmaxFreesK && wq == 0 && lane == 0) mbar_arrive(&bars->k_empty[i % C::kStages]);
       tc_fence_after();
       const uint32_t s_addr = lane_base + kColS + bi * kTile;
       float x[kTile];
@@ -774,8 +798,8 @@ __device__ void softmax(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
         l += s0 + s1;
       }
       if (__any_sync(0xffffffffu, need)) {
-        const int64_t pv = i - 1;
-        if (!warp_wait(&bars->p_free[pv & 1], static_cast<uint32_t>(pv >> 1) & 1u, abort, a.wait_ns)) return false;
+        const uint32_t pv = i - 1;
+        if (!warp_wait(&bars->p_free[pv & 1u], (pv >> 1) & 1u, abort, a.wait_ns)) return false;
         tc_fence_after();
         const uint32_t o_addr = lane_base + kColO + wg * D;
 #pragma unroll
@@ -796,20 +820,19 @@ __device__ void softmax(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
       vr.next();
       return true;
     };
+    const int first_tile = cur.i, sink_tiles = cur.u.s_tiles, to_window = cur.u.lo_tile - cur.u.s_tiles;
+#pragma unroll 1
     for (int k = 0; k < n; ++k, ++i) {
-      const int j0 = cur.u.tile(cur.i + k) * kTile;
-      const bool plain = common.plain(a, j0);
-      bool whole_tile = plain;
-      if (plain) {
-        // (the valid words are read again under the mask; a plain tile lacks keys only where a page is bad)
-        if (!warp_wait(&bars->v_full[vr.stage], vr.phase, abort, a.wait_ns)) return;
-        whole_tile = *reinterpret_cast<const uint64_t*>(smem + C::kOffMeta + vr.stage * C::kMetaBytes) == ~0ull;
-      }
-      if (!(whole_tile ? tile(std::false_type(), j0, k == 0) : tile(std::true_type(), j0, k == 0))) return;
+      const int at = first_tile + k;
+      const int j0 = (at < sink_tiles ? at : at + to_window) * kTile;
+      // (a plain tile lacks keys only where a page is bad, which is known before its scores are)
+      const uint32_t stage = vr.stage;
+      if (common.plain(a, j0) && !tile(std::false_type(), j0, k == 0)) return;
+      if (vr.stage == stage && !tile(std::true_type(), j0, k == 0)) return;
     }
     // ---- epilogue
-    const int64_t lastv = i - 1;
-    if (!warp_wait(&bars->p_free[lastv & 1], static_cast<uint32_t>(lastv >> 1) & 1u, abort, a.wait_ns)) return;
+    const uint32_t lastv = i - 1;
+    if (!warp_wait(&bars->p_free[lastv & 1u], (lastv >> 1) & 1u, abort, a.wait_ns)) return;
     tc_fence_after();
     const bool whole = cur.i + n == cur.u.tiles && !cut_start;
     const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (first_unit ? 0 : 1);
@@ -886,9 +909,17 @@ __device__ void softmax(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
       a.part_ml[slot * C::M + qrow] = make_float2(m_used, l);
     }
     first_unit = cut_start = false;
-    cur.at += n - 1;
-    cur.i += n - 1;
-    if (!cur.next(a, end)) return;
+    __syncwarp();
+    int more = 0;
+    if (lane == 0) {
+      TileCursor c = cur;
+      c.at += n - 1;
+      c.i += n - 1;
+      more = c.next(a, end);
+      cur = c;
+    }
+    if (!__shfl_sync(0xffffffffu, more, 0)) return;
+    __syncwarp();
   }
 }
 
@@ -905,7 +936,7 @@ __global__ void __launch_bounds__(TcCfg<T, ST, D, MT>::kThreads, 1) paged_tc_ker
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&bars->k_full[s], a.tma && C::kWide ? 1 : 2);  // the TMA thread, or the two warps of its rows
-      mbar_init(&bars->k_empty[s], 1);
+      mbar_init(&bars->k_empty[s], C::kSoftmaxFreesK ? MT : 1);
       mbar_init(&bars->v_full[s], 2);
       mbar_init(&bars->v_empty[s], 1);
     }
@@ -923,6 +954,7 @@ __global__ void __launch_bounds__(TcCfg<T, ST, D, MT>::kThreads, 1) paged_tc_ker
       mbar_init(&bars->p_free[b], 1);
       mbar_init(&bars->drain[b], 1);
     }
+    bars->bad = 0;
     bars->abort = 0;
     bars->odd = 0;
     fence_barrier_init();
