@@ -8,6 +8,8 @@
 // Bound by the latency of one key at a time per warp.
 #include <cuda_fp8.h>
 
+#include <algorithm>
+
 #include "paged_attn.cuh"
 
 namespace gorgon {
@@ -211,9 +213,106 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __g
     a.lse[(a.nr.cu ? 0 : n.b * a.l_sb) + h * a.l_sh + r * a.l_sn] = (M + log2f(L)) * 0.6931471805599453f;
 }
 
+// The same for units of many rows, most of them cut in two or three: a warp
+// takes eight rows, four pieces at a time; lane 4 r + p holds row r's max and
+// sum of piece p, and the eight rows of a piece are in flight together.
+constexpr int kRowsPerWarp = 8;
+constexpr int kMergeRows = kMergeWarps * kRowsPerWarp;
+template <typename T, int D>
+__global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_rows_kernel(const __grid_constant__ PagedAttn a) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int c = blockIdx.x;
+  const CutUnit n = a.cut[c];
+  if (n.pieces == 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int V = D / 32;
+  const Seq s = sequence(a, n.b, false);
+  const int r0 = blockIdx.y * kMergeRows + warp * kRowsPerWarp;
+  const int rows = min(kRowsPerWarp, min(a.m, s.c * a.group - n.qb * a.m) - r0);
+  if (rows <= 0) return;
+  auto slot = [&](int p) -> int64_t { return static_cast<int64_t>(c - 1 + p) * 2 + (p == 0 ? n.first_slot : 0); };
+  float acc[kRowsPerWarp][V] = {};
+  float M = -INFINITY, L = 0.f;  // of row lane / 4, the same on its four lanes
+  for (int p0 = 0; p0 < n.pieces; p0 += 4) {
+    const int p = p0 + (lane & 3), r = lane >> 2;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (p < n.pieces && r < rows) ml = __ldcg(&a.part_ml[slot(p) * a.m + r0 + r]);
+    float top = fmaxf(M, ml.x);
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const float base = top == -INFINITY ? 0.f : top;
+    const float old = exp2f(M - base), f = exp2f(ml.x - base);
+    float add = f * ml.y;
+    add += __shfl_xor_sync(0xffffffffu, add, 1);
+    add += __shfl_xor_sync(0xffffffffu, add, 2);
+    L = L * old + add;
+    M = top;
+    const int np = min(4, n.pieces - p0);
+    if (p0 > 0) {
+#pragma unroll
+      for (int k = 0; k < kRowsPerWarp; ++k) {
+        const float g = __shfl_sync(0xffffffffu, old, 4 * k);
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[k][v] *= g;
+      }
+    }
+    for (int q = 0; q < np; ++q) {
+      const float* o = a.part_o + (slot(p0 + q) * a.m + r0) * D + lane * V;
+      float x[kRowsPerWarp][V];
+#pragma unroll
+      for (int k = 0; k < kRowsPerWarp; ++k)
+        if (k < rows) {
+          if constexpr (V == 4)
+            *reinterpret_cast<float4*>(x[k]) = __ldcg(reinterpret_cast<const float4*>(o + k * D));
+          else
+            *reinterpret_cast<float2*>(x[k]) = __ldcg(reinterpret_cast<const float2*>(o + k * D));
+        }
+#pragma unroll
+      for (int k = 0; k < kRowsPerWarp; ++k) {
+        const float g = __shfl_sync(0xffffffffu, f, 4 * k + q);
+        if (k < rows) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) acc[k][v] = fmaf(g, x[k][v], acc[k][v]);
+        }
+      }
+    }
+  }
+  const int64_t first = a.nr.cu ? a.nr.cu[n.b] : 0;
+#pragma unroll
+  for (int k = 0; k < kRowsPerWarp; ++k) {
+    const float Lk = __shfl_sync(0xffffffffu, L, 4 * k), Mk = __shfl_sync(0xffffffffu, M, 4 * k);
+    if (k >= rows) continue;
+    const int pr = n.qb * a.m + r0 + k;
+    const int t = group_div(a, pr), h = n.kvh * a.group + pr - t * a.group;
+    T* out = reinterpret_cast<T*>(a.out) + (a.nr.cu ? 0 : n.b * a.o_sb) + h * a.o_sh + (first + t) * a.o_sn + lane * V;
+    const float inv = 1.f / Lk;
+    T y[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) y[v] = Cvt<T>::from_f(acc[k][v] * inv);
+    if (reinterpret_cast<uintptr_t>(out) % (V * sizeof(T)) == 0) {
+      if constexpr (V == 4) *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(y);
+      else *reinterpret_cast<uint32_t*>(out) = *reinterpret_cast<const uint32_t*>(y);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) out[v] = y[v];
+    }
+    if (a.lse && lane == 0)
+      a.lse[(a.nr.cu ? 0 : n.b * a.l_sb) + h * a.l_sh + (first + t) * a.l_sn] = (Mk + log2f(Lk)) * 0.6931471805599453f;
+  }
+}
+
 }  // namespace
 
 int launch_paged_merge(const PagedAttn& a, cudaStream_t st) {
+  if (a.m >= kMergeRows) {
+    const int rows = static_cast<int>(ceil_div(std::min<int64_t>(a.m, static_cast<int64_t>(a.n) * a.group), kMergeRows));
+    if (a.pool.dtype == GORGON_BF16)
+      return a.pool.d == 128 ? launch_early(paged_merge_rows_kernel<__nv_bfloat16, 128>, a, kMergeWarps * 32, 0, st, rows)
+                             : launch_early(paged_merge_rows_kernel<__nv_bfloat16, 64>, a, kMergeWarps * 32, 0, st, rows);
+    return a.pool.d == 128 ? launch_early(paged_merge_rows_kernel<__half, 128>, a, kMergeWarps * 32, 0, st, rows)
+                           : launch_early(paged_merge_rows_kernel<__half, 64>, a, kMergeWarps * 32, 0, st, rows);
+  }
   const int y = static_cast<int>(ceil_div(a.m, 8));
   if (a.pool.dtype == GORGON_BF16)
     return a.pool.d == 128 ? launch_early(paged_merge_kernel<__nv_bfloat16, 128>, a, kMergeWarps * 32, 0, st, y)

@@ -67,7 +67,7 @@ struct TcCfg {
   static constexpr int kStages = kWide ? (MT == 2 ? 4 : 5) : 3;
   static constexpr int kRawStages = kWide ? 0 : (MT == 2 ? 3 : 5);
   static constexpr uint32_t kRawRows = 32 * D;           // bytes of a producer's 32 rows
-  static constexpr uint32_t kRawBytes = 2 * kRawRows + 512;  // a tile of K or V, and (cp.async) its K and V scales
+  static constexpr uint32_t kRawBytes = 2 * kRawRows + 768;  // a tile of K or V, and (cp.async) its scales, for each half
   static constexpr int kInfo = 8;                        // (more than the tiles a producer has in flight)
   static constexpr int kLag = kWide ? kStages - 2 : 0;   // tiles in flight behind the newest
   // With two M-tiles each softmax warpgroup frees a K stage once it has seen its
@@ -77,7 +77,7 @@ struct TcCfg {
   static constexpr uint32_t kOffV = kOffK + kStages * kTileBytes;
   static constexpr uint32_t kOffRaw = kOffV + kStages * kTileBytes;         // [K, V][stages]
   static constexpr uint32_t kOffMeta = kOffRaw + 2 * kRawStages * kRawBytes;  // [stages] Meta
-  static constexpr uint32_t kMetaBytes = kWide ? 16 : 16 + 8 * kTile;       // 2 words of valid keys, max V scale x 2; K and V scales
+  static constexpr uint32_t kMetaBytes = kWide ? 16 : 16 + 8 * kTile;       // 2 words of valid keys, E; K and V factors
   static constexpr uint32_t kOffBits = kOffMeta + kStages * kMetaBytes;     // [M][8] ancestor words
   static constexpr uint32_t kOffQs = kOffBits + M * (kMaxTree / 32) * 4;    // [M] undoes Q's power of two
   static constexpr uint32_t kOffInfo = kOffQs + M * 4;                      // [4 producers][kInfo] valid keys, plain
@@ -202,19 +202,27 @@ __device__ __forceinline__ bool strip_rows(uint8_t* st, int half, uint32_t keep)
   return odd;
 }
 
-// The half's valid word and (8-bit) scales for the softmax.
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
+constexpr int kNoExp = -116;
+
+// What the softmax needs of a tile: the half's valid word, and (8-bit) K's scales
+// times the softmax scale and V's scales in units of 2^(E - 6), with 2^E above
+// every V scale of the unit so far, so that weights (at most 2^8) times them
+// stay in f16's range (see paged_attn_mma.cu).  Both halves know all 64 V
+// scales (`top`: their maximum), and so the same E.
 template <typename C>
-__device__ __forceinline__ void write_meta(uint8_t* smem, uint32_t stage, int half, uint32_t valid, float ks, float vs) {
+__device__ __forceinline__ void write_meta(const PagedAttn& a, uint8_t* smem, uint32_t stage, int half, uint32_t valid, float ks, float vs,
+                                           float top, bool first, int& unit_exp) {
   const int lane = threadIdx.x & 31;
   uint8_t* meta = smem + C::kOffMeta + stage * C::kMetaBytes;
   if (lane == 0) reinterpret_cast<uint32_t*>(meta)[half] = valid;
   if constexpr (!C::kWide) {
-    float top = vs;  // (NaN never wins)
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) reinterpret_cast<float*>(meta)[2 + half] = top;
-    reinterpret_cast<float*>(meta + 16)[half * 32 + lane] = ks;
-    reinterpret_cast<float*>(meta + 16)[kTile + half * 32 + lane] = vs;
+    unit_exp = max(first ? kNoExp : unit_exp, (__float_as_int(top) >> 23) - 126);
+    if (lane == 0 && half == 0) reinterpret_cast<int*>(meta)[2] = unit_exp;
+    reinterpret_cast<float*>(meta + 16)[half * 32 + lane] = ks * a.scale_log2;
+    reinterpret_cast<float*>(meta + 16)[kTile + half * 32 + lane] = vs * pow2i(6 - unit_exp);
   }
 }
 
@@ -293,37 +301,46 @@ __device__ void finish_tiles(const PagedAttn& a, TileCursor f, int end, uint8_t*
   uint64_t* full = is_v ? bars->v_full : bars->k_full;
   uint64_t* empty = is_v ? bars->v_empty : bars->k_empty;
   uint8_t* ring = smem + (is_v ? C::kOffV : C::kOffK);
-  // This lane's row: its page two tiles ahead, its scales one tile ahead, so that nothing waits for them.
-  int page = -2, row = 0, kvh = 0;
+  // This lane's row (and, for V's scales, the same row of the other half): its page
+  // two tiles ahead, its scales one tile ahead, so that nothing waits for them.
+  int page[2] = {-2, -2}, row[2] = {}, kvh = 0;
+  bool next_first = true;
   auto look_up = [&]() {
-    page = -2;
     kvh = f.kvh;
-    const int j = f.tile() * kTile + half * 32 + lane;
-    if (f.u.wanted(j)) {
-      int col;
-      a.pool.split(j, col, row);
-      page = __ldg(a.pool.table + static_cast<int64_t>(f.b) * a.pool.table_sb + col);
-    }
-  };
-  bool held = false;
-  float ks = 0.f, vs = 0.f;
-  auto take = [&]() {  // the looked-up page's validity and scales
-    held = page >= 0 && page < a.pool.num_pages;
-    if (page != -2 && !held) raise_device_error(a.pool.err, kErrBadPage);
-    if constexpr (!C::kWide) {
-      ks = vs = 0.f;
-      if (is_v && held) {
-        ks = __ldg(a.pool.ks + page * a.pool.ks_sp + kvh * a.pool.ks_sh + row * a.pool.ks_ss);
-        vs = __ldg(a.pool.vs + page * a.pool.vs_sp + kvh * a.pool.vs_sh + row * a.pool.vs_ss);
+#pragma unroll
+    for (int k = 0; k < (C::kWide ? 1 : 2); ++k) {
+      page[k] = -2;
+      const int j = f.tile() * kTile + (k ? 1 - half : half) * 32 + lane;
+      if (f.u.wanted(j)) {
+        int col;
+        a.pool.split(j, col, row[k]);
+        page[k] = __ldg(a.pool.table + static_cast<int64_t>(f.b) * a.pool.table_sb + col);
       }
     }
   };
+  bool held = false;
+  float ks = 0.f, vs = 0.f, vo = 0.f;
+  auto take = [&]() {  // the looked-up pages' validity and scales
+    held = page[0] >= 0 && page[0] < a.pool.num_pages;
+    if constexpr (!C::kWide) {
+      ks = vs = vo = 0.f;
+      if (is_v && held) {
+        ks = __ldg(a.pool.ks + page[0] * a.pool.ks_sp + kvh * a.pool.ks_sh + row[0] * a.pool.ks_ss);
+        vs = __ldg(a.pool.vs + page[0] * a.pool.vs_sp + kvh * a.pool.vs_sh + row[0] * a.pool.vs_ss);
+      }
+      if (is_v && page[1] >= 0 && page[1] < a.pool.num_pages)
+        vo = __ldg(a.pool.vs + page[1] * a.pool.vs_sp + kvh * a.pool.vs_sh + row[1] * a.pool.vs_ss);
+    }
+  };
+  int unit_exp = kNoExp;
+  bool first = true;  // the tile is the unit's first here
   bool plain = Common(a, f).plain(a, f.tile() * kTile), next_plain = false;
   look_up();
   take();
   bool more = f.next(a, end);
   if (more) {
     next_plain = Common(a, f).plain(a, f.tile() * kTile);
+    next_first = f.i == 0;
     look_up();
   }
   constexpr int kSlots = C::kWide ? C::kStages : C::kRawStages;
@@ -331,14 +348,16 @@ __device__ void finish_tiles(const PagedAttn& a, TileCursor f, int end, uint8_t*
   Slot<C::kStages> hs;
   while (true) {
     const uint32_t valid = __ballot_sync(0xffffffffu, held);
-    const float k1 = ks, v1 = vs;
-    const bool p1 = plain, again = more;
+    const float k1 = ks, v1 = vs, top = fmaxf(vs, vo);  // (NaN never wins)
+    const bool p1 = plain, f1 = first, again = more;
     if (more) {  // the next tile's scales, and the page of the one after
       take();
       plain = next_plain;
+      first = next_first;
       more = f.next(a, end);
       if (more) {
         next_plain = Common(a, f).plain(a, f.tile() * kTile);
+        next_first = f.i == 0;
         look_up();
       }
     }
@@ -355,7 +374,7 @@ __device__ void finish_tiles(const PagedAttn& a, TileCursor f, int end, uint8_t*
       widen_rows<ST, C>(src, st, half, is_v ? valid : 0xffffffffu);
       fence_proxy_async_smem();
     }
-    if (is_v) write_meta<C>(smem, hs.stage, half, valid, k1, v1);
+    if (is_v) write_meta<C>(a, smem, hs.stage, half, valid, k1, v1, top, f1, unit_exp);
     __syncwarp();
     if (lane == 0) {
       if constexpr (!C::kWide) mbar_arrive(&bars->raw_empty[is_v][ls.stage]);
@@ -393,15 +412,18 @@ __device__ void produce(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
   int f_tile = 0;             // tiles fetched
   Slot<C::kStages> fs;        // (16-bit) the stage fetched into
   // The page of this lane's row of the next tile (-2: not wanted), looked up a tile ahead.
-  int next_page = -2, next_row = 0;
+  int next_page = -2, next_row = 0, next_other = -2, next_other_row = 0;
   auto look_up = [&]() {
-    next_page = -2;
-    const int j = f.tile() * kTile + half * 32 + lane;
-    if (f.u.wanted(j)) {
-      int col;
-      a.pool.split(j, col, next_row);
-      next_page = __ldg(a.pool.table + static_cast<int64_t>(f.b) * a.pool.table_sb + col);
-    }
+    auto one = [&](int j, int& pg, int& rw) {
+      pg = -2;
+      if (f.u.wanted(j)) {
+        int col;
+        a.pool.split(j, col, rw);
+        pg = __ldg(a.pool.table + static_cast<int64_t>(f.b) * a.pool.table_sb + col);
+      }
+    };
+    one(f.tile() * kTile + half * 32 + lane, next_page, next_row);
+    if (!C::kWide && is_v) one(f.tile() * kTile + (1 - half) * 32 + lane, next_other, next_other_row);
   };
   look_up();
   auto fetch = [&]() -> bool {
@@ -410,13 +432,15 @@ __device__ void produce(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
     }
     int page = next_page;
     const int prow = next_row;
+    [[maybe_unused]] const int other = next_other, other_row = next_other_row;
     if (page != -2 && (page < 0 || page >= a.pool.num_pages)) {
       raise_device_error(a.pool.err, kErrBadPage);
       *reinterpret_cast<volatile int*>(&bars->bad) = 1;  // before the tile is handed over
       page = -2;
     }
     const uint32_t valid = __ballot_sync(0xffffffffu, page >= 0);
-    if (lane == 0) info[f_tile % C::kInfo] = make_uint2(valid, Common(a, f).plain(a, f.tile() * kTile) ? 1u : 0u);
+    if (lane == 0)
+      info[f_tile % C::kInfo] = make_uint2(valid, (Common(a, f).plain(a, f.tile() * kTile) ? 1u : 0u) | (f.i == 0 ? 2u : 0u));
     const int64_t off = page >= 0 ? page * sp + prow * ss : 0;
     const char* base = pages + f.kvh * sh + piece * 16;
 #pragma unroll
@@ -431,11 +455,14 @@ __device__ void produce(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
       cp16(at, base + o, (valid >> r) & 1u);
     }
     if constexpr (!C::kWide) {
-      if (is_v) {
+      if (is_v) {  // its rows' K and V scales, and the other half's V scales
         const int64_t pg = page >= 0 ? page : 0, pr = page >= 0 ? prow : 0;
-        const uint32_t at = smem_u32(raw + (f_tile % C::kRawStages) * C::kRawBytes) + 2 * C::kRawRows + half * 256 + lane * 4;
+        const bool other_held = other >= 0 && other < a.pool.num_pages;
+        const int64_t og = other_held ? other : 0, orow = other_held ? other_row : 0;
+        const uint32_t at = smem_u32(raw + (f_tile % C::kRawStages) * C::kRawBytes) + 2 * C::kRawRows + half * 384 + lane * 4;
         cp4(at, a.pool.ks + pg * a.pool.ks_sp + f.kvh * a.pool.ks_sh + pr * a.pool.ks_ss, page >= 0);
         cp4(at + 128, a.pool.vs + pg * a.pool.vs_sp + f.kvh * a.pool.vs_sh + pr * a.pool.vs_ss, page >= 0);
+        cp4(at + 256, a.pool.vs + og * a.pool.vs_sp + f.kvh * a.pool.vs_sh + orow * a.pool.vs_ss, other_held);
       }
     }
     cp_commit();
@@ -446,7 +473,7 @@ __device__ void produce(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
     return true;
   };
   Slot<C::kStages> hs;  // the stage handed over
-  int done = 0;
+  int done = 0, unit_exp = kNoExp;
   // Hands tile `done` over: its copies have landed.
   auto hand_over = [&]() -> bool {
     const uint2 h = info[done % C::kInfo];
@@ -457,15 +484,16 @@ __device__ void produce(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
       widen_rows<ST, C>(raw + (done % C::kRawStages) * C::kRawBytes + half * C::kRawRows, st, half, h.x);
     }
     if (is_v) {
-      float ks = 0.f, vs = 0.f;
+      float ks = 0.f, vs = 0.f, vo = 0.f;
       if constexpr (!C::kWide) {
-        const float* sc = reinterpret_cast<const float*>(raw + (done % C::kRawStages) * C::kRawBytes + 2 * C::kRawRows + half * 256);
+        const float* sc = reinterpret_cast<const float*>(raw + (done % C::kRawStages) * C::kRawBytes + 2 * C::kRawRows + half * 384);
         ks = sc[lane];
         vs = sc[32 + lane];
-      } else if (!(h.y && h.x == 0xffffffffu)) {
-        if (strip_rows<T, C>(st, half, h.x)) atomicOr(&bars->odd, h.y ? 2 : 1);
+        vo = sc[64 + lane];
+      } else if (!((h.y & 1u) && h.x == 0xffffffffu)) {
+        if (strip_rows<T, C>(st, half, h.x)) atomicOr(&bars->odd, h.y & 1u ? 2 : 1);
       }
-      write_meta<C>(smem, hs.stage, half, h.x, ks, vs);
+      write_meta<C>(a, smem, hs.stage, half, h.x, ks, vs, fmaxf(vs, vo), done == 0 || (h.y & 2u), unit_exp);
     }
     fence_proxy_async_smem();
     __syncwarp();
@@ -574,9 +602,6 @@ __device__ void issue_outputs(const PagedAttn& a, TileCursor cur, int end, uint8
 }
 
 // ------------------------------------------------------------ softmax
-__device__ __forceinline__ float pow2i(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
-constexpr int kNoExp = -116;
-
 // Which columns of the tile at j0 the row sees.
 __device__ __forceinline__ uint64_t row_word(const PagedAttn& a, const TileCursor& c, int pos, bool ok, const uint32_t* bits, int j0) {
   if (!ok) return 0;
@@ -684,10 +709,10 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
       pos = cur.s.P + tree_bits(a, cur.s, cur.b, t, bits);
     }
     const Common common(a, cur);
-    const float qs = a.scale_log2 * (kScaleQ ? s_qs[qrow] : 1.f);
+    // (8-bit: K's factors hold the softmax scale)
+    const float qs = C::kWide ? a.scale_log2 : kScaleQ ? s_qs[qrow] : 1.f;
     float m_used = -INFINITY, l = 0.f;
     int unit_exp = kNoExp;
-    float unit = pow2i(6 - kNoExp);
     // One tile of this row: scores to weights against the lazy running max.
     auto tile = [&](auto mask_tag, int j0, bool fresh) -> bool {
       constexpr bool kMask = decltype(mask_tag)::value;
@@ -712,15 +737,22 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
 #pragma unroll
         for (int c = 0; c < kTile; ++c) x[c] = __uint_as_float(rr[c >> 5][c & 31]);
       }
+      // Wide: x stays the raw score.  8-bit: x becomes the score (in log2 units) less
+      // the running max.
+      [[maybe_unused]] const float base = C::kWide || m_used == -INFINITY ? 0.f : m_used;
       if constexpr (!C::kWide) {
         const float4* ks = reinterpret_cast<const float4*>(meta + 16);
+        const uint64_t qb = f2_pack(qs, qs), nb = f2_pack(-base, -base);
 #pragma unroll
-        for (int c = 0; c < kTile / 4; ++c) {
-          const float4 f = ks[c];
-          x[4 * c] *= f.x;
-          x[4 * c + 1] *= f.y;
-          x[4 * c + 2] *= f.z;
-          x[4 * c + 3] *= f.w;
+        for (int c = 0; c < kTile; c += 4) {
+          const float4 f = ks[c >> 2];
+          uint64_t f0 = f2_pack(f.x, f.y), f1 = f2_pack(f.z, f.w);
+          if (kScaleQ) {
+            f0 = f2_mul(f0, qb);
+            f1 = f2_mul(f1, qb);
+          }
+          f2_unpack(f2_fma(f2_pack(x[c], x[c + 1]), f0, nb), x[c], x[c + 1]);
+          f2_unpack(f2_fma(f2_pack(x[c + 2], x[c + 3]), f1, nb), x[c + 2], x[c + 3]);
         }
       }
       if (kMask) {
@@ -731,32 +763,45 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int c = 0; c < kTile; c += 2) mx[(c >> 1) & 3] = fmax3(mx[(c >> 1) & 3], x[c], x[c + 1]);
-      const float tmax = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]) * qs;
+      const float top = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]);
       float alpha = 1.f;
       bool need = false;
-      if (fresh) {
-        m_used = tmax;
-      } else if (tmax > m_used + 8.f) {
-        alpha = ex2_approx(m_used - tmax);
-        m_used = tmax;
-        need = true;
+      if constexpr (C::kWide) {
+        const float tmax = top * qs;
+        if (fresh) {
+          m_used = tmax;
+        } else if (tmax > m_used + 8.f) {
+          alpha = ex2_approx(m_used - tmax);
+          m_used = tmax;
+          need = true;
+        }
+      } else {
+        const bool move = fresh || m_used == -INFINITY ? top > -INFINITY : top > 8.f;
+        if (__any_sync(0xffffffffu, move)) {
+          const float d = move ? top : 0.f;
+          if (move) {
+            alpha = m_used == -INFINITY ? 0.f : ex2_approx(-d);
+            m_used = base + d;
+            need = !fresh;
+          }
+          const uint64_t d2 = f2_pack(-d, -d);
+#pragma unroll
+          for (int c = 0; c < kTile; c += 2) f2_unpack(f2_add(f2_pack(x[c], x[c + 1]), d2), x[c], x[c + 1]);
+        }
       }
       l *= alpha;
       if constexpr (!C::kWide) {
-        const float2 top2 = *reinterpret_cast<const float2*>(meta + 8);
-        const int e = (__float_as_int(fmaxf(top2.x, top2.y)) >> 23) - 126;
+        const int e = reinterpret_cast<const int*>(meta)[2];
         if (e > unit_exp) {
           alpha *= unit_exp == kNoExp ? 0.f : pow2i(unit_exp - e);
           unit_exp = e;
-          unit = pow2i(6 - e);
           need = !fresh;
         }
       }
       const float nmb = m_used == -INFINITY ? 0.f : -m_used;
-      const uint64_t qs2 = f2_pack(qs, qs), nmb2 = f2_pack(nmb, nmb);
+      [[maybe_unused]] const uint64_t qs2 = f2_pack(qs, qs), nmb2 = f2_pack(nmb, nmb);
       uint64_t acc[4] = {0, 0, 0, 0};
       [[maybe_unused]] const float4* vs = reinterpret_cast<const float4*>(meta + 16 + 4 * kTile);
-      const uint64_t unit2 = f2_pack(unit, unit);
       // Weights go to TMEM 32 columns at a time (over this tile's scores, which are in
       // registers), so that few are held beside them.
 #pragma unroll
@@ -764,9 +809,11 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
       uint32_t packed[16];
 #pragma unroll
       for (int c = c0; c < c0 + 32; c += 4) {
-        float y[4];
-        f2_unpack(f2_fma(f2_pack(x[c], x[c + 1]), qs2, nmb2), y[0], y[1]);
-        f2_unpack(f2_fma(f2_pack(x[c + 2], x[c + 3]), qs2, nmb2), y[2], y[3]);
+        float y[4] = {x[c], x[c + 1], x[c + 2], x[c + 3]};
+        if constexpr (C::kWide) {
+          f2_unpack(f2_fma(f2_pack(x[c], x[c + 1]), qs2, nmb2), y[0], y[1]);
+          f2_unpack(f2_fma(f2_pack(x[c + 2], x[c + 3]), qs2, nmb2), y[2], y[3]);
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = ex2_approx(y[e]);
         uint64_t p0 = f2_pack(y[0], y[1]), p1 = f2_pack(y[2], y[3]);
@@ -774,8 +821,8 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
         acc[((c >> 1) + 1) & 3] = f2_add(acc[((c >> 1) + 1) & 3], p1);
         if constexpr (!C::kWide) {
           const float4 f = vs[c >> 2];
-          p0 = f2_mul(p0, f2_mul(f2_pack(f.x, f.y), unit2));
-          p1 = f2_mul(p1, f2_mul(f2_pack(f.z, f.w), unit2));
+          p0 = f2_mul(p0, f2_pack(f.x, f.y));
+          p1 = f2_mul(p1, f2_pack(f.z, f.w));
           float z[4];
           f2_unpack(p0, z[0], z[1]);
           f2_unpack(p1, z[2], z[3]);
@@ -863,7 +910,11 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
       }
     };
     T* out = reinterpret_cast<T*>(a.out) + (a.nr.cu ? 0 : cur.b * a.o_sb);
-    float* part = a.part_o + (slot * C::M + qrow) * D;
+    // Rows go out through the warp's staging rows (its slice of the Q tile, free
+    // now), so that a store instruction writes whole rows: 16-bit rows in one
+    // pass, the fp32 rows of a piece in two.
+    constexpr int kPass = kChunks * 4;  // fp32 columns that a staging row holds
+    float* part = a.part_o + (slot * C::M + wg * 128 + wq * 32) * D;
 #pragma unroll
     for (int ch = 0; ch < D / 32; ++ch) {
       uint32_t ov[32];
@@ -875,7 +926,16 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
       if (odd) put_back(ch * 32, v);
       if (!whole) {
 #pragma unroll
-        for (int c = 0; c < 32; c += 4) *reinterpret_cast<float4*>(part + ch * 32 + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+        for (int u = 0; u < 8; ++u)
+          *reinterpret_cast<float4*>(stage_row(lane, (ch * 32 % kPass) / 4 + u)) = make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+        if ((ch + 1) * 32 % kPass == 0) {
+          __syncwarp();
+#pragma unroll 4
+          for (int k = 0; k < 32; k += kRows)
+            *reinterpret_cast<float4*>(part + (k + rsub) * D + (ch * 32 / kPass) * kPass + chunk * 4) =
+                *reinterpret_cast<const float4*>(stage_row(k + rsub, chunk));
+          __syncwarp();
+        }
       } else if (vec_out) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
