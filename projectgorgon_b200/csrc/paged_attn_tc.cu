@@ -77,7 +77,7 @@ struct TcCfg {
   static constexpr uint32_t kOffV = kOffK + kStages * kTileBytes;
   static constexpr uint32_t kOffRaw = kOffV + kStages * kTileBytes;         // [K, V][stages]
   static constexpr uint32_t kOffMeta = kOffRaw + 2 * kRawStages * kRawBytes;  // [stages] Meta
-  static constexpr uint32_t kMetaBytes = kWide ? 16 : 16 + 8 * kTile;       // 2 words of valid keys, E; K and V factors
+  static constexpr uint32_t kMetaBytes = kWide ? 16 : 16 + 8 * kTile;       // 2 words of valid keys, E, partly hidden; K and V factors
   static constexpr uint32_t kOffBits = kOffMeta + kStages * kMetaBytes;     // [M][8] ancestor words
   static constexpr uint32_t kOffQs = kOffBits + M * (kMaxTree / 32) * 4;    // [M] undoes Q's power of two
   static constexpr uint32_t kOffInfo = kOffQs + M * 4;                      // [4 producers][kInfo] valid keys, plain
@@ -212,7 +212,7 @@ constexpr int kNoExp = -116;
 // scales (`top`: their maximum), and so the same E.
 template <typename C>
 __device__ __forceinline__ void write_meta(const PagedAttn& a, uint8_t* smem, uint32_t stage, int half, uint32_t valid, float ks, float vs,
-                                           float top, bool first, int& unit_exp) {
+                                           float top, bool first, int& unit_exp, bool plain) {
   const int lane = threadIdx.x & 31;
   uint8_t* meta = smem + C::kOffMeta + stage * C::kMetaBytes;
   if (lane == 0) reinterpret_cast<uint32_t*>(meta)[half] = valid;
@@ -220,6 +220,8 @@ __device__ __forceinline__ void write_meta(const PagedAttn& a, uint8_t* smem, ui
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     unit_exp = max(first ? kNoExp : unit_exp, (__float_as_int(top) >> 23) - 126);
+    // (each half says whether its rows are whole and seen by all, in its half of the word)
+    if (lane == 0) reinterpret_cast<uint16_t*>(meta + 12)[half] = plain && valid == 0xffffffffu ? 0 : 1;
     if (lane == 0 && half == 0) reinterpret_cast<int*>(meta)[2] = unit_exp;
     reinterpret_cast<float*>(meta + 16)[half * 32 + lane] = ks * a.scale_log2;
     reinterpret_cast<float*>(meta + 16)[kTile + half * 32 + lane] = vs * pow2i(6 - unit_exp);
@@ -374,7 +376,7 @@ __device__ void finish_tiles(const PagedAttn& a, TileCursor f, int end, uint8_t*
       widen_rows<ST, C>(src, st, half, is_v ? valid : 0xffffffffu);
       fence_proxy_async_smem();
     }
-    if (is_v) write_meta<C>(a, smem, hs.stage, half, valid, k1, v1, top, f1, unit_exp);
+    if (is_v) write_meta<C>(a, smem, hs.stage, half, valid, k1, v1, top, f1, unit_exp, p1);
     __syncwarp();
     if (lane == 0) {
       if constexpr (!C::kWide) mbar_arrive(&bars->raw_empty[is_v][ls.stage]);
@@ -493,7 +495,7 @@ __device__ void produce(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
       } else if (!((h.y & 1u) && h.x == 0xffffffffu)) {
         if (strip_rows<T, C>(st, half, h.x)) atomicOr(&bars->odd, h.y & 1u ? 2 : 1);
       }
-      write_meta<C>(a, smem, hs.stage, half, h.x, ks, vs, fmaxf(vs, vo), done == 0 || (h.y & 2u), unit_exp);
+      write_meta<C>(a, smem, hs.stage, half, h.x, ks, vs, fmaxf(vs, vo), done == 0 || (h.y & 2u), unit_exp, h.y & 1u);
     }
     fence_proxy_async_smem();
     __syncwarp();
@@ -699,14 +701,40 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->q_full);
     }
-    // ---- this row's ancestor bits (each thread its own: rows of one node repeat the
-    // walk, but no barrier stands between warps that may give up a wait)
+    // ---- this row's ancestor bits.  The warp copies parents[] to its own rows' place
+    // for the bits, every lane walks its row's chain there, and the bits go over it
+    // (rows of one node repeat the walk, but no barrier stands between warps that
+    // may give up a wait).
     int pos = cur.s.P + t;
     uint32_t* bits = s_bits + qrow * kWords;
-    if (a.parents && row_ok) {
+    if (a.parents) {
+      int32_t* par = reinterpret_cast<int32_t*>(s_bits + (wg * 128 + wq * 32) * kWords);
+      const int32_t* src = a.parents + static_cast<int64_t>(cur.b) * a.par_sb;
+      const int c = cur.s.c, P = cur.s.P;
+      __syncwarp();
 #pragma unroll
-      for (int w = 0; w < kWords; ++w) bits[w] = 0;
-      pos = cur.s.P + tree_bits(a, cur.s, cur.b, t, bits);
+      for (int k = 0; k < kWords; ++k)
+        if (lane + 32 * k < c) par[lane + 32 * k] = __ldg(src + lane + 32 * k);
+      __syncwarp();
+      uint32_t word[kWords] = {};
+      int at = row_ok ? t : -1, hop = 0;
+      for (; at >= 0 && hop <= c; ++hop) {
+        if (hop <= a.max_depth && (!a.window || hop < a.window || P + at < a.sinks)) {
+#pragma unroll
+          for (int k = 0; k < kWords; ++k)
+            if ((at >> 5) == k) word[k] |= 1u << (at & 31);
+        }
+        const int up = par[at];
+        if (up >= c) raise_device_error(a.pool.err, kErrBadParent);
+        if (up < 0 || up >= c) break;
+        at = up;
+      }
+      pos += hop - t;
+      if (hop > c) pos = P + c;  // (a cycle: no position is its own)
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) bits[k] = word[k];
+      __syncwarp();
     }
     const Common common(a, cur);
     // (8-bit: K's factors hold the softmax scale)
@@ -718,13 +746,13 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
       constexpr bool kMask = decltype(mask_tag)::value;
       const uint32_t bi = (i & 1u) * MT + wg;
       [[maybe_unused]] const uint8_t* meta = smem + C::kOffMeta + vr.stage * C::kMetaBytes;
-      if (kMask || !C::kWide) {  // the tile's valid keys and scales
+      if (kMask && C::kWide) {  // the tile's valid keys (8-bit: the caller waited for them and the scales)
         if (!warp_wait(&bars->v_full[vr.stage], vr.phase, abort, a.wait_ns)) return false;
       }
       uint64_t vw = ~0ull;
       if (kMask) vw = row_word(a, cur, pos, row_ok, bits, j0) & *reinterpret_cast<const uint64_t*>(meta);
       if (!warp_wait(&bars->s_full[bi], (i >> 1) & 1u, abort, a.wait_ns)) return false;
-      if (!kMask && *reinterpret_cast<volatile int*>(&bars->bad)) return true;  // (the caller looks at it too)
+      if (!kMask && C::kWide && *reinterpret_cast<volatile int*>(&bars->bad)) return true;  // (the caller looks at it too)
       if (C::kSoftmaxFreesK && wq == 0 && lane == 0) mbar_arrive(&bars->k_empty[i % C::kStages]);
       tc_fence_after();
       const uint32_t s_addr = lane_base + kColS + bi * kTile;
@@ -867,15 +895,22 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
       vr.next();
       return true;
     };
-    const int first_tile = cur.i, sink_tiles = cur.u.s_tiles, to_window = cur.u.lo_tile - cur.u.s_tiles;
 #pragma unroll 1
     for (int k = 0; k < n; ++k, ++i) {
-      const int at = first_tile + k;
-      const int j0 = (at < sink_tiles ? at : at + to_window) * kTile;
-      // (a plain tile lacks keys only where a page is bad, which is known before its scores are)
-      const uint32_t stage = vr.stage;
-      if (common.plain(a, j0) && !tile(std::false_type(), j0, k == 0)) return;
-      if (vr.stage == stage && !tile(std::true_type(), j0, k == 0)) return;
+      if constexpr (C::kWide) {
+        // (a plain tile lacks keys only where a page is bad, which is known before its scores are)
+        const uint32_t stage = vr.stage;
+        const int j0 = cur.u.tile(cur.i + k) * kTile;
+        if (common.plain(a, j0) && !tile(std::false_type(), j0, k == 0)) return;
+        if (vr.stage == stage && !tile(std::true_type(), j0, k == 0)) return;
+      } else {
+        if (!warp_wait(&bars->v_full[vr.stage], vr.phase, abort, a.wait_ns)) return;
+        if (reinterpret_cast<const uint32_t*>(smem + C::kOffMeta + vr.stage * C::kMetaBytes)[3] == 0) {
+          if (!tile(std::false_type(), 0, k == 0)) return;
+        } else {
+          if (!tile(std::true_type(), cur.u.tile(cur.i + k) * kTile, k == 0)) return;
+        }
+      }
     }
     // ---- epilogue
     const uint32_t lastv = i - 1;
