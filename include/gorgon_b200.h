@@ -498,17 +498,18 @@ GORGON_API int gorgon_paged_trim(const gorgon_paged_trim_params* p, void* stream
  *   ignored; n is then the largest count of new rows).
  * Row i of a sequence with c new rows, P = seq_lens[b] - c, sees position j
  *   without parents: iff j <= P + i;
- *   with parents (int32 [batch, n], stride 0 shared, every sequence brings n
- *   rows): iff j < P, or j - P is i or one of its ancestors within max_depth
- *   hops (max_depth < 0: all); its position is P + depth(i), depth counting
- *   the hops to its root;
+ *   with parents (int32 [batch, n], stride 0 shared; a sequence's tree is the
+ *   first c of its n): iff j < P, or j - P is i or one of its ancestors within
+ *   max_depth hops (max_depth < 0: all); its position is P + depth(i), depth
+ *   counting the hops to its root;
  * and with window > 0 only if j's position is less than `window` positions
  * before the row's own (a tree row's position as above), or j < sinks.
  * Hidden rows contribute nothing, whatever they hold.
  * out = softmax(q k^T * scale) v over the visible rows (scale 0: 1 /
  * sqrt(head_dim)); lse (nullable, float, strides) the natural-log sum of
- * exponentials.  Rows of an unused slot are 0 with lse -inf; packed rows
- * from cu_q[batch] on are left as they are. */
+ * exponentials.  Rows of an unused slot, and rows with nothing to see (all
+ * their pages are bad), are 0 with lse -inf; packed rows from cu_q[batch] on
+ * are left as they are. */
 typedef struct {
   gorgon_paged_kv kv;
   int64_t heads_q, n;

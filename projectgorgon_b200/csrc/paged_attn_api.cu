@@ -21,8 +21,8 @@ int make_args(const gorgon_paged_attn_params* p, PagedAttn* a) {
     return set_error(GORGON_ERR_UNSUPPORTED, "gorgon_paged_attn: too many query rows");
   if (p->parents && p->n > kPagedMaxNodes)
     return set_error(GORGON_ERR_UNSUPPORTED, "gorgon_paged_attn: trees above 1024 nodes");
-  if (p->parents && p->cu_q)
-    return set_error(GORGON_ERR_UNSUPPORTED, "gorgon_paged_attn: a tree needs n rows in every sequence (no cu_q)");
+  if (!(p->scale >= 0.f && p->scale < INFINITY))
+    return set_error(GORGON_ERR_INVALID, "gorgon_paged_attn: scale must be positive and finite");
   if (p->cu_q && (p->rows < 0 || p->rows > INT32_MAX))
     return set_error(GORGON_ERR_INVALID, "gorgon_paged_attn: bad count of packed rows");
   if (p->backend < GORGON_PAGED_AUTO || p->backend > GORGON_PAGED_TCGEN05)
@@ -57,22 +57,23 @@ bool empty(const PagedAttn& a) { return static_cast<int64_t>(a.pool.batch) * a.h
 
 enum class Kernel { kSimt, kMma, kTc, kNone };
 
-// The schedule's places fit 32 bits (it counts them per 64 positions or more).
-bool short_list(const PagedAttn& a) {
-  const int64_t blocks = static_cast<int64_t>(a.n) * a.group / 8 + 1;
+// The schedule's places fit 32 bits (it counts them per `m` packed rows and 64
+// positions, or more).
+bool short_list(const PagedAttn& a, int m) {
+  const int64_t blocks = static_cast<int64_t>(a.n) * a.group / m + 1;
   const int64_t tiles = static_cast<int64_t>(a.pool.table_cols) * a.pool.page_size / 64 + 6;
   return blocks * tiles < (int64_t(1) << 31) / (static_cast<int64_t>(a.pool.batch) * a.pool.hkv + 1);
 }
 
 Kernel choose(const gorgon_paged_attn_params* p, const PagedAttn& a) {
-  const bool mma = paged_mma_supported(a) && short_list(a);
+  const bool mma = paged_mma_supported(a) && short_list(a, 8), tc = paged_tc_supported(a) && short_list(a, 128);
   switch (p->backend) {
     case GORGON_PAGED_SIMT: return Kernel::kSimt;
     case GORGON_PAGED_MMA: return mma ? Kernel::kMma : Kernel::kNone;
-    case GORGON_PAGED_TCGEN05: return mma && paged_tc_supported(a) ? Kernel::kTc : Kernel::kNone;
+    case GORGON_PAGED_TCGEN05: return tc ? Kernel::kTc : Kernel::kNone;
     default:
       // up to 16 packed rows fill one tile of the warp-level kernel
-      if (static_cast<int64_t>(a.n) * a.group > 16 && mma && paged_tc_supported(a)) return Kernel::kTc;
+      if (static_cast<int64_t>(a.n) * a.group > 16 && tc) return Kernel::kTc;
       return mma ? Kernel::kMma : Kernel::kSimt;
   }
 }

@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
     if (u.wanted(j)) {
       int col;
       a.pool.split(j, col, prow);
-      page = __ldg(tb + col);  // col is inside: L fits the table
+      page = max(-1, __ldg(tb + col));  // col is inside: L fits the table
     }
   };
   auto issue = [&](int stage) {
@@ -729,7 +729,7 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
           if (whole) {
             const int pr = cur.qb * C::M + row, tt = group_div(a, pr), h = cur.kvh * a.group + pr - tt * a.group;
             T* out = reinterpret_cast<T*>(a.out) + (a.nr.cu ? 0 : cur.b * a.o_sb) + h * a.o_sh + (first + tt) * a.o_sn;
-            out[d] = Cvt<T>::from_f(sum * (1.f / L));
+            out[d] = Cvt<T>::from_f(L == 0.f ? 0.f : sum * (1.f / L));
             if (a.lse && d == 0)
               a.lse[(a.nr.cu ? 0 : cur.b * a.l_sb) + h * a.l_sh + (first + tt) * a.l_sn] = (top + log2f(L)) * 0.6931471805599453f;
           } else {

@@ -36,14 +36,16 @@ __global__ void __launch_bounds__(kWarps * 32) paged_simt_kernel(const PagedAttn
   const int t = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Seq s = sequence(a, b, threadIdx.x == 0 && t == 0 && h == 0);
-  if (t >= s.c || t >= a.n || !rows_inside(a, b, s.c)) return;
+  if (t >= s.c || !rows_inside(a, b, s.c)) return;
   const int64_t row = a.nr.cu ? a.nr.first(b) + t : t;
   T* out = reinterpret_cast<T*>(a.out) + (a.nr.cu ? 0 : b * a.o_sb) + h * a.o_sh + row * a.o_sn;
   float* lse = a.lse ? a.lse + (a.nr.cu ? 0 : b * a.l_sb) + h * a.l_sh + row * a.l_sn : nullptr;
   const int D = a.pool.d;
-  if (!s.ok) {
-    for (int d = threadIdx.x; d < D; d += blockDim.x) out[d] = Cvt<T>::from_f(0.f);
-    if (lse && threadIdx.x == 0) *lse = -INFINITY;
+  if (!s.ok) {  // (it may bring more rows than the n that the grid covers)
+    for (int64_t k = 0; t + k < s.c; k += a.n) {
+      for (int d = threadIdx.x; d < D; d += blockDim.x) out[k * a.o_sn + d] = Cvt<T>::from_f(0.f);
+      if (lse && threadIdx.x == 0) lse[k * a.l_sn] = -INFINITY;
+    }
     return;
   }
   int pos = s.P + t;
@@ -115,7 +117,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_simt_kernel(const PagedAttn
   for (int d = threadIdx.x; d < D; d += blockDim.x) {
     float x = 0.f;
     for (int w = 0; w < kWarps; ++w) x = fmaf(s_o[w][d], exp2f(s_m[w] - base), x);
-    out[d] = Cvt<T>::from_f(x / L);
+    out[d] = Cvt<T>::from_f(L == 0.f ? 0.f : x / L);
   }
   if (lse && threadIdx.x == 0) *lse = (M + log2f(L)) * 0.6931471805599453f;
 }
@@ -208,7 +210,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_kernel(const __g
   T* out = reinterpret_cast<T*>(a.out) + (a.nr.cu ? 0 : n.b * a.o_sb) + h * a.o_sh + r * a.o_sn + lane * V;
   const float inv = 1.f / L;
 #pragma unroll
-  for (int v = 0; v < V; ++v) out[v] = Cvt<T>::from_f(acc[v] * inv);
+  for (int v = 0; v < V; ++v) out[v] = Cvt<T>::from_f(L == 0.f ? 0.f : acc[v] * inv);
   if (a.lse && lane == 0)
     a.lse[(a.nr.cu ? 0 : n.b * a.l_sb) + h * a.l_sh + r * a.l_sn] = (M + log2f(L)) * 0.6931471805599453f;
 }
@@ -289,7 +291,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_merge_rows_kernel(cons
     const float inv = 1.f / Lk;
     T y[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) y[v] = Cvt<T>::from_f(acc[k][v] * inv);
+    for (int v = 0; v < V; ++v) y[v] = Cvt<T>::from_f(Lk == 0.f ? 0.f : acc[k][v] * inv);
     if (reinterpret_cast<uintptr_t>(out) % (V * sizeof(T)) == 0) {
       if constexpr (V == 4) *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(y);
       else *reinterpret_cast<uint32_t*>(out) = *reinterpret_cast<const uint32_t*>(y);

@@ -245,14 +245,14 @@ __device__ void load_tiles(const PagedAttn& a, const CUtensorMap* map, TileCurso
   constexpr uint32_t kSlotBytes = C::kWide ? C::kTileBytes : C::kRawBytes;
   const int R = box_rows(a.pool.page_size), boxes = kTile / R;
   const uint32_t box_bytes = static_cast<uint32_t>(R) * (C::kWide ? C::D * 2 : C::D);
-  int page = -2, row = 0;  // of box `lane` of the next tile
+  int page = -2, row = 0;  // of box `lane` of the next tile (-2: not wanted)
   auto look_up = [&]() {
     page = -2;
     const int p = f.tile() * kTile + lane * R;
     if (lane < boxes && p < f.u.hi && (p + R > f.u.lo || p < f.u.s_end)) {
       int col;
       a.pool.split(p, col, row);
-      page = __ldg(a.pool.table + static_cast<int64_t>(f.b) * a.pool.table_sb + col);
+      page = max(-1, __ldg(a.pool.table + static_cast<int64_t>(f.b) * a.pool.table_sb + col));
     }
   };
   look_up();
@@ -421,7 +421,7 @@ __device__ void produce(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
       if (f.u.wanted(j)) {
         int col;
         a.pool.split(j, col, rw);
-        pg = __ldg(a.pool.table + static_cast<int64_t>(f.b) * a.pool.table_sb + col);
+        pg = max(-1, __ldg(a.pool.table + static_cast<int64_t>(f.b) * a.pool.table_sb + col));
       }
     };
     one(f.tile() * kTile + half * 32 + lane, next_page, next_row);
@@ -920,7 +920,8 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
     const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (first_unit ? 0 : 1);
     const uint32_t o_addr = lane_base + kColO + wg * D;
     const float back = C::kWide ? 1.f : pow2i(unit_exp - 6);
-    const float f = whole ? back / l : (m_used == -INFINITY ? 0.f : back);
+    const bool none = m_used == -INFINITY && !(whole && l != 0.f);  // nothing but hidden keys (l: NaN where a score was)
+    const float f = whole ? back / l : back;
     const int odd = C::kWide ? *reinterpret_cast<volatile int*>(&bars->odd) : 0;
     // Adds what the producers took out of partly hidden V rows to a row that sees
     // it: columns [c0, c0 + 32), key by key from the pages.
@@ -957,7 +958,7 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
       tmem_wait_ld();
       float v[32];
 #pragma unroll
-      for (int c = 0; c < 32; ++c) v[c] = m_used == -INFINITY && !whole ? 0.f : __uint_as_float(ov[c]) * f;
+      for (int c = 0; c < 32; ++c) v[c] = none ? 0.f : __uint_as_float(ov[c]) * f;
       if (odd) put_back(ch * 32, v);
       if (!whole) {
 #pragma unroll

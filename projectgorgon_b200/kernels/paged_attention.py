@@ -8,6 +8,7 @@ them or a sliding window and the first few.
 """
 from __future__ import annotations
 
+import math
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
@@ -63,11 +64,12 @@ def paged_attention(
 
     Query head ``h`` reads kv head ``h // (Hq // Hkv)``.  A new row sees the
     cached rows and the new rows up to itself; with ``parents`` (``[n]`` or
-    ``[B, n]``, -1 for a root) the cached rows, itself and its ancestors within
+    ``[B, n]``, -1 for a root; with ``cu_q`` ``n`` is ``max_q``, and a sequence's tree
+    the first of them) the cached rows, itself and its ancestors within
     ``max_depth`` hops.  ``window`` hides rows ``window`` or more positions before
     a row's own (a tree row's position is the cached length plus its depth),
     except the first ``sinks`` rows.  Hidden rows contribute nothing, even when
-    they hold infinities or NaN.
+    they hold infinities or NaN.  ``scale`` (default ``D ** -0.5``) is positive.
 
     Returns ``out`` shaped like ``q``, and with ``return_lse`` also the
     natural-log sum of exponentials, float32 ``[B, Hq, n]`` (packed:
@@ -128,21 +130,20 @@ def paged_attention(
         l_sb, l_sh, l_sn = (0, 1, hq) if cu is not None else lse.stride()
     par, p_ptr, p_sb = None, 0, 0
     if parents is not None:
-        if cu is not None and batch * n != total:
-            raise RuntimeError("trees need the same number of rows in every sequence: give q as [batch, heads_q, n, "
-                               "head_dim], or cu_q with max_q rows in each")
         par = parents_tensor(parents, q.device)
-        if par.dim() == 1 and par.shape[0] == n:
+        if cu is not None:
+            n = 0 if total == 0 else par.shape[-1] if max_q is None else int(max_q)  # (may pass the packed rows' count)
+        if par.dim() == 1 and (par.shape[0] == n or n == 0):
             p_sb = 0
-        elif par.dim() == 2 and par.shape[0] == batch and par.shape[1] == n:
+        elif par.dim() == 2 and par.shape[0] == batch and (par.shape[1] == n or n == 0):
             p_sb = par.stride(0)
         else:
             raise RuntimeError(f"parents must be [{n}] or [{batch}, {n}], got {tuple(par.shape)}")
         p_ptr = par.data_ptr()
-        if cu is not None:  # equal counts: the packed rows are a batch with strides
-            cu, q_sb, o_sb, l_sb = None, n * q_sn, n * o_sn, n * l_sn
     if window is not None and window < 1:
         raise RuntimeError(f"window must be at least 1, got {window}")
+    if scale is not None and not 0.0 < scale < math.inf:
+        raise RuntimeError(f"scale must be positive and finite, got {scale}")
     if sinks < 0:
         raise RuntimeError(f"sinks must not be negative, got {sinks}")
     params = _ATTN.pack(*pool, hq, n, 0 if cu is None else total, q.data_ptr(), q_sb, q_sh, q_sn, out.data_ptr(), o_sb, o_sh, o_sn,

@@ -120,10 +120,12 @@ def test_other_refusals_and_empty_calls():
     assert "multiple" in _err(lib.gorgon_paged_attn(ctypes.byref(n), None, 0, None))[1]
     n.heads_q, n.window = 4, -1
     assert "negative" in _err(lib.gorgon_paged_attn(ctypes.byref(n), None, 0, None))[1]
-    n.window, n.parents, n.cu_q = 0, 4096, 4096
-    assert _err(lib.gorgon_paged_attn(ctypes.byref(n), None, 0, None))[0] == _abi.GORGON_ERR_UNSUPPORTED
-    n.cu_q, n.n = None, 1025
+    n.window, n.parents, n.n = 0, 4096, 1025
     assert "1024" in _err(lib.gorgon_paged_attn(ctypes.byref(n), None, 0, None))[1]
+    for bad in (-0.1, float("nan"), float("inf")):
+        n.n, n.scale = 1, bad
+        assert "scale" in _err(lib.gorgon_paged_attn(ctypes.byref(n), None, 0, None))[1]
+    n.scale = 0.0
     n.n, n.backend = 1, 99
     assert "backend" in _err(lib.gorgon_paged_attn(ctypes.byref(n), None, 0, None))[1]
     n.backend, n.q = 0, None
