@@ -154,6 +154,10 @@ __device__ __forceinline__ Place append_place(const AppendArgs& a, const int32_t
   if (cu) {
     if (r < cu[0] || r >= cu[a.pool.batch]) return p;  // padding behind the last sequence
     p.b = sequence_of(cu, a.pool.batch, r);
+    if (cu[p.b] < 0) {
+      if (report) raise_device_error(a.pool.err, kErrBadSeqlen);
+      return p;
+    }
     p.i = r - cu[p.b];
     c = cu[p.b + 1] - cu[p.b];
   } else {
@@ -162,7 +166,8 @@ __device__ __forceinline__ Place append_place(const AppendArgs& a, const int32_t
     p.i = r - p.b * c;
   }
   const int L = a.pool.lens[p.b];
-  if (L < c) {
+  // (a row outside its sequence: cu is out of order)
+  if (L < c || p.i < 0 || p.i >= c || L - c + p.i < 0) {
     if (L != 0 && report) raise_device_error(a.pool.err, kErrBadSeqlen);
     return p;
   }
@@ -275,14 +280,14 @@ __device__ __forceinline__ Place read_place(const ReadArgs& a, const int32_t* cu
   Place p{};
   if (r < cu[0] || r >= cu[a.pool.batch]) return p;
   p.b = sequence_of(cu, a.pool.batch, r);
-  p.i = r - cu[p.b];
-  const int pos = (a.starts ? a.starts[p.b] : 0) + p.i;
-  if (pos < 0) {
+  p.i = cu[p.b] < 0 ? -1 : r - cu[p.b];
+  const int64_t pos = static_cast<int64_t>(a.starts ? a.starts[p.b] : 0) + p.i;
+  if (p.i < 0 || pos < 0 || pos > INT32_MAX) {
     raise_device_error(a.pool.err, kErrBadSeqlen);
     return p;
   }
   int col;
-  a.pool.split(pos, col, p.row);
+  a.pool.split(static_cast<int>(pos), col, p.row);
   p.page = a.pool.page(p.b, col);
   p.ok = p.page >= 0;
   return p;

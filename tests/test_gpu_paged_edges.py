@@ -117,6 +117,29 @@ def test_counts_out_of_order_are_reported(cu, backend):
     assert G.device_error(clear=True) == BAD_LENGTH
 
 
+@pytest.mark.parametrize("cu", [[0, -3, 4, 6], [2, 5, 3, 6], [0, 5, 2, 6], [0, 2 ** 31 - 1, 3, 6], [-2 ** 31, 2, 3, 6], [0, 6, 0, 6]])
+def test_counts_out_of_order_leave_the_pages_alone(cu):
+    """Append and read: rows outside their sequence are skipped and reported; pages
+    that no row may go to keep their bytes."""
+    p = Paged([3, 60, 70], 2, 128, 16, torch.float16, seed=1, poison=False)
+    rows = torch.randn(6, 2, 128, device="cuda").half()
+    own = torch.unique(p.table[(p.table >= 0) & (p.table < p.k_pages.shape[0])]).cuda()
+    other = torch.ones(p.k_pages.shape[0], dtype=torch.bool, device="cuda")
+    other[own.long()] = False
+    before = p.k_pages.clone()
+    cu = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    G.paged_cache_append(rows, rows, p.k_pages, p.v_pages, p.table_d, p.lens_d, cu_q=cu)
+    torch.cuda.synchronize()
+    assert torch.equal(p.k_pages[other], before[other])
+    G.device_error(clear=True)
+    out = torch.full((2, 6, 2, 128), 4.0, device="cuda", dtype=torch.float16)
+    for starts in (None, [0, 0, 0], [2 ** 31 - 1] * 3, [-2 ** 31] * 3):
+        G.paged_cache_read(p.k_pages, p.v_pages, p.table_d, cu, 6, out=(out[0], out[1]),
+                           starts=None if starts is None else torch.tensor(starts, dtype=torch.int32, device="cuda"))
+        torch.cuda.synchronize()
+        assert G.device_error(clear=True) in (0, BAD_LENGTH, BAD_PAGE, BAD_LENGTH | BAD_PAGE)
+
+
 @pytest.mark.parametrize("batch", [129, 700, 1500])
 @pytest.mark.parametrize("packed", [False, True])
 def test_many_sequences(batch, packed):
