@@ -114,6 +114,15 @@ __device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool take) {
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// True on one lane of a converged warp, in a form that tells the compiler so: TMA
+// and tcgen05 instructions behind it take their operands from uniform registers
+// without a loop over the lanes that might be active.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}" : "=r"(yes));
+  return yes != 0;
+}
+
 template <int N>
 struct Slot {  // ring position
   uint32_t stage = 0, phase = 0;
@@ -177,7 +186,7 @@ __device__ __forceinline__ bool strip_rows(uint8_t* st, int half, uint32_t keep)
   constexpr int kCpr = C::D / 8, kRpi = 32 / kCpr;
   const int lane = threadIdx.x & 31, piece = lane % kCpr, rsub = lane / kCpr;
   bool odd = false;
-#pragma unroll 1
+#pragma unroll 4
   for (int it = 0; it < 32 / kRpi; ++it) {
     const int r = it * kRpi + rsub;
     uint4* w = reinterpret_cast<uint4*>(st + (piece >> 3) * C::kBlock + sw128(half * 32 + r, piece & 7));
@@ -245,21 +254,26 @@ __device__ void load_tiles(const PagedAttn& a, const CUtensorMap* map, TileCurso
   constexpr uint32_t kSlotBytes = C::kWide ? C::kTileBytes : C::kRawBytes;
   const int R = box_rows(a.pool.page_size), boxes = kTile / R;
   const uint32_t box_bytes = static_cast<uint32_t>(R) * (C::kWide ? C::D * 2 : C::D);
-  int page = -2, row = 0;  // of box `lane` of the next tile (-2: not wanted)
-  auto look_up = [&]() {
-    page = -2;
+  // Page of box `lane` of a tile (-2: not wanted, -1: bad), and the tile's row in it
+  // (a page smaller than a tile begins with its box).
+  auto look_up = [&](int& row) {
+    int page = -2;
     const int p = f.tile() * kTile + lane * R;
     if (lane < boxes && p < f.u.hi && (p + R > f.u.lo || p < f.u.s_end)) {
       int col;
       a.pool.split(p, col, row);
       page = max(-1, __ldg(a.pool.table + static_cast<int64_t>(f.b) * a.pool.table_sb + col));
     }
+    return page;
   };
-  look_up();
+  int next_row = 0, next_page = look_up(next_row);
   Slot<kSlots> s;
   int64_t issued = 0;
   bool more = true;
   while (more) {
+    const int page = next_page, row = __shfl_sync(0xffffffffu, next_row, 0), kvh = f.kvh;
+    more = f.next(a, end);
+    if (more) next_page = look_up(next_row);  // (in flight while this tile's boxes are sent)
     if (!warp_wait(&empty[s.stage], s.phase ^ 1u, abort, a.wait_ns)) break;
     const uint32_t go = __ballot_sync(0xffffffffu, page >= 0 && page < a.pool.num_pages);
     if (page != -2 && !((go >> lane) & 1u)) {
@@ -270,23 +284,22 @@ __device__ void load_tiles(const PagedAttn& a, const CUtensorMap* map, TileCurso
     if (lane == 0) mbar_arrive_expect_tx(&full[s.stage], __popc(go) * box_bytes);
     __syncwarp();
     uint8_t* dst = ring + s.stage * kSlotBytes;
-    for (int x = 0; x < boxes; ++x) {
-      const int pg = __shfl_sync(0xffffffffu, page, x), r = __shfl_sync(0xffffffffu, row, x);
-      if (!((go >> x) & 1u)) continue;
-      if (lane == 0) {
+#pragma unroll 1
+    for (int x = 0; x < boxes; ++x, dst += R * (C::kWide ? 128 : C::D)) {
+      const int pg = __shfl_sync(0xffffffffu, page, x);
+      if (((go >> x) & 1u) && elect_one()) {
         if constexpr (C::kWide) {
 #pragma unroll
-          for (int h = 0; h < C::kHalves; ++h)
-            tma_load_4d(dst + h * C::kBlock + x * R * 128, map, &full[s.stage], h * 64, r, f.kvh, pg);
+          for (int h = 0; h < C::kHalves; ++h) tma_load_4d(dst + h * C::kBlock, map, &full[s.stage], h * 64, row, kvh, pg);
         } else {
-          tma_load_4d(dst + x * R * C::D, map, &full[s.stage], 0, r, f.kvh, pg);
+          tma_load_4d(dst, map, &full[s.stage], 0, row, kvh, pg);
         }
       }
+      __syncwarp();
     }
+    __syncwarp();
     ++issued;
     s.next();
-    more = f.next(a, end);
-    if (more) look_up();
   }
   // Every issued load must land before the CTA leaves.
   if (lane == 0)
@@ -517,6 +530,12 @@ __device__ void produce(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
 }
 
 // ------------------------------------------------------------ issuers
+// M-tiles of the cursor's unit that hold rows.
+template <typename C>
+__device__ __forceinline__ int live_tiles(const PagedAttn& a, const TileCursor& c) {
+  return C::MT == 1 || c.s.c * a.group - c.qb * C::M <= 128 ? 1 : 2;
+}
+
 template <typename C>
 __device__ void issue_scores(const PagedAttn& a, TileCursor cur, int end, uint8_t* smem, TcBars<C>* bars, uint32_t tmem, uint32_t fmt) {
   volatile int* abort = &bars->abort;
@@ -529,7 +548,7 @@ __device__ void issue_scores(const PagedAttn& a, TileCursor cur, int end, uint8_
   while (ok) {
     if (!spin_wait(&bars->q_full, unit & 1u, abort, a.wait_ns)) break;
     ++unit;
-    const int n = min(cur.u.tiles - cur.i, end - cur.at);
+    const int n = min(cur.u.tiles - cur.i, end - cur.at), live = live_tiles<C>(a, cur);
     for (int t = 0; t < n && ok; ++t, ++i) {
       // Both probes before either result is used: the round trips overlap when the
       // K tile and the S buffer (its weights of two tiles ago) are ready, as they usually are.
@@ -544,6 +563,7 @@ __device__ void issue_scores(const PagedAttn& a, TileCursor cur, int end, uint8_
       tc_fence_after();
 #pragma unroll
       for (int mt = 0; mt < C::MT; ++mt) {
+        if (mt < live)
 #pragma unroll
         for (int ks = 0; ks < C::D / 16; ++ks)
           umma_f16_ss(tmem + kColS + ((i & 1u) * C::MT + mt) * kTile,
@@ -551,6 +571,12 @@ __device__ void issue_scores(const PagedAttn& a, TileCursor cur, int end, uint8_
                       k0 + static_cast<uint64_t>(kr.stage * (C::kTileBytes >> 4) + (ks >> 2) * (C::kBlock >> 4) + (ks & 3) * 2), idesc,
                       ks > 0 ? 1u : 0u);
         umma_commit(&bars->s_full[(i & 1u) * C::MT + mt]);
+        // The second M-tile's scores follow the first one's weights of the tile before, so
+        // that the two warpgroups' exponentials and the P V products alternate.
+        if (C::MT == 2 && mt == 0 && i > 0 && !spin_wait(&bars->p_full[((i - 1) & 1u) * C::MT], ((i - 1) >> 1) & 1u, abort, a.wait_ns)) {
+          ok = false;
+          break;
+        }
       }
       if (!C::kSoftmaxFreesK) umma_commit(&bars->k_empty[kr.stage]);
       kr.next();
@@ -572,7 +598,7 @@ __device__ void issue_outputs(const PagedAttn& a, TileCursor cur, int end, uint8
   uint32_t i = 0;
   bool ok = true;
   while (ok) {
-    const int n = min(cur.u.tiles - cur.i, end - cur.at);
+    const int n = min(cur.u.tiles - cur.i, end - cur.at), live = live_tiles<C>(a, cur);
     for (int t = 0; t < n && ok; ++t, ++i) {
       const uint32_t buf = i & 1u;
       if (!spin_wait(&bars->v_full[vr.stage], vr.phase, abort, a.wait_ns)) {
@@ -584,6 +610,7 @@ __device__ void issue_outputs(const PagedAttn& a, TileCursor cur, int end, uint8
           ok = false;
           break;
         }
+        if (mt >= live) continue;
         tc_fence_after();
 #pragma unroll
         for (int ks = 0; ks < kTile / 16; ++ks)
@@ -665,9 +692,19 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
     {
       const char* qb = a.q + (a.nr.cu ? 0 : cur.b * a.q_sb) + first * a.q_sn + static_cast<int64_t>(cur.kvh) * a.group * a.q_sh;
       const int p0 = cur.qb * C::M + wg * 128 + wq * 32;
+      if constexpr (!kScaleQ) {
+#pragma unroll
+        for (int k = 0; k < 32; k += kRows) {
+          const int p = p0 + k + rsub;
+          const int tt = group_div(a, p), gg = p - tt * a.group;
+          cp16(smem_u32(stage_row(k + rsub, chunk)), p < R ? qb + tt * a.q_sn + gg * a.q_sh + chunk * 16 : qb, p < R);
+        }
+        cp_commit();
+        cp_wait<0>();
+      }
       constexpr int kBatch = 8;
 #pragma unroll 1
-      for (int k0 = 0; k0 < 32; k0 += kBatch * kRows) {
+      for (int k0 = kScaleQ ? 0 : 32; k0 < 32; k0 += kBatch * kRows) {
         uint4 qv[kBatch];
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
@@ -895,8 +932,22 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
       vr.next();
       return true;
     };
+    // Whether the warp has rows in this unit: its lanes of the products are not read otherwise.
+    auto live = [&]() { return cur.qb * C::M + wg * 128 + wq * 32 < cur.s.c * a.group; };
+    const uint32_t done = i + n;
+    if (!live()) {
+      for (; i < done; ++i) {
+        const uint32_t bi = (i & 1u) * MT + wg;
+        if (!warp_wait(&bars->s_full[bi], (i >> 1) & 1u, abort, a.wait_ns)) return;
+        if (lane == 0) {
+          if (C::kSoftmaxFreesK && wq == 0) mbar_arrive(&bars->k_empty[i % C::kStages]);
+          mbar_arrive(&bars->p_full[bi]);
+        }
+        vr.next();
+      }
+    }
 #pragma unroll 1
-    for (int k = 0; k < n; ++k, ++i) {
+    for (int k = 0; i < done; ++k, ++i) {
       if constexpr (C::kWide) {
         // (a plain tile lacks keys only where a page is bad, which is known before its scores are)
         const uint32_t stage = vr.stage;
@@ -916,6 +967,7 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
     const uint32_t lastv = i - 1;
     if (!warp_wait(&bars->p_free[lastv & 1u], (lastv >> 1) & 1u, abort, a.wait_ns)) return;
     tc_fence_after();
+    const bool has_rows = live();
     const bool whole = cur.i + n == cur.u.tiles && !cut_start;
     const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (first_unit ? 0 : 1);
     const uint32_t o_addr = lane_base + kColO + wg * D;
@@ -953,6 +1005,7 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
     float* part = a.part_o + (slot * C::M + wg * 128 + wq * 32) * D;
 #pragma unroll
     for (int ch = 0; ch < D / 32; ++ch) {
+      if (!has_rows) break;
       uint32_t ov[32];
       tmem_ld32(o_addr + ch * 32, ov);
       tmem_wait_ld();
@@ -985,7 +1038,8 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
         for (int c = 0; c < 32; ++c) out[h * a.o_sh + (first + t) * a.o_sn + ch * 32 + c] = Cvt<T>::from_f(v[c]);
       }
     }
-    if (whole) {
+    if (!has_rows) {
+    } else if (whole) {
       if (vec_out) {
         __syncwarp();
         const int p0 = cur.qb * C::M + wg * 128 + wq * 32;
@@ -1076,7 +1130,7 @@ __global__ void __launch_bounds__(TcCfg<T, ST, D, MT>::kThreads, 1) paged_tc_ker
   if (warp < 8) {
     if (work) {
       if (warp == 0) {
-        if (lane == 0) issue_scores<C>(a, cur, end, smem, bars, tmem, fmt);
+        if (elect_one()) issue_scores<C>(a, cur, end, smem, bars, tmem, fmt);
       } else if (warp == 1) {
         if (lane == 0) issue_outputs<C>(a, cur, end, smem, bars, tmem, fmt);
       } else if (warp < 4) {
