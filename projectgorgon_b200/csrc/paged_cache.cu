@@ -90,6 +90,18 @@ __device__ __forceinline__ uint8_t store8(float x, float inv) {
 }
 
 template <int ST>
+__device__ __forceinline__ uint32_t store8x4(float a, float b, float c, float d, float inv) {
+  if constexpr (ST == GORGON_KV_INT8) {
+    return store8<ST>(a, inv) | store8<ST>(b, inv) << 8 | store8<ST>(c, inv) << 16 | static_cast<uint32_t>(store8<ST>(d, inv)) << 24;
+  } else {
+    const bool none = inv == 0.f;
+    const float2 x = none ? make_float2(0.f, 0.f) : make_float2(a * inv, b * inv), y = none ? make_float2(0.f, 0.f) : make_float2(c * inv, d * inv);
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(x, __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
+  }
+}
+
+template <int ST>
 __device__ __forceinline__ float load8(uint8_t s) {
   if constexpr (ST == GORGON_KV_INT8) {
     return static_cast<float>(static_cast<int8_t>(s));
@@ -179,59 +191,65 @@ __device__ __forceinline__ Place append_place(const AppendArgs& a, const int32_t
 }
 
 // 16-bit rows of D = 8 * LPR values: LPR threads hold a row's 16-byte pieces
-// of K and of V, and find its largest magnitude by shuffles.
-template <typename T, int ST, int LPR>
+// of K and of V, and find its largest magnitude by shuffles.  They take HP heads
+// of a row: where a row goes (its sequence, length and page: three dependent
+// loads) is found once for them, and their loads are in flight together.
+template <typename T, int ST, int LPR, int HP>
 __global__ void __launch_bounds__(kThreads) paged_append_vec_kernel(const AppendArgs a) {
   __shared__ int32_t s_cu[kCuCached + 1];
   const int32_t* cu = cached_cu(a.nr.cu, a.pool.batch, s_cu);
   const int sub = threadIdx.x % LPR;
   const int64_t item = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / LPR;
+  const int per_row = (a.pool.hkv + HP - 1) / HP;
   const bool live = item < a.items;
-  const int r = live ? static_cast<int>(item / a.pool.hkv) : 0;
-  const int h = live ? static_cast<int>(item - static_cast<int64_t>(r) * a.pool.hkv) : 0;
+  const int r = live ? static_cast<int>(item / per_row) : 0;
+  const int h0 = live ? static_cast<int>(item - static_cast<int64_t>(r) * per_row) * HP : 0;
   Place p{};
   if (live) p = append_place(a, cu, r, sub == 0);
   const int64_t rn = cu ? r : p.i;
   const int64_t rb = cu ? 0 : p.b;
-  uint4 raw[2] = {};
-  if (p.ok) {
-    raw[0] = __ldcs(reinterpret_cast<const uint4*>(a.k + rb * a.k_sb + h * a.k_sh + rn * a.k_sn) + sub);
-    raw[1] = __ldcs(reinterpret_cast<const uint4*>(a.v + rb * a.v_sb + h * a.v_sh + rn * a.v_sn) + sub);
-  }
-  char* dst[2] = {a.pool.k + p.page * a.pool.k_sp + h * a.pool.k_sh + p.row * a.pool.k_ss,
-                  a.pool.v + p.page * a.pool.v_sp + h * a.pool.v_sh + p.row * a.pool.v_ss};
-  if constexpr (ST == GORGON_KV_NATIVE) {
-    if (p.ok) {
-      reinterpret_cast<uint4*>(dst[0])[sub] = raw[0];
-      reinterpret_cast<uint4*>(dst[1])[sub] = raw[1];
+  uint4 raw[HP][2] = {};
+#pragma unroll
+  for (int k = 0; k < HP; ++k)
+    if (p.ok && h0 + k < a.pool.hkv) {
+      raw[k][0] = __ldcs(reinterpret_cast<const uint4*>(a.k + rb * a.k_sb + (h0 + k) * a.k_sh + rn * a.k_sn) + sub);
+      raw[k][1] = __ldcs(reinterpret_cast<const uint4*>(a.v + rb * a.v_sb + (h0 + k) * a.v_sh + rn * a.v_sn) + sub);
     }
-  } else {
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      const T* e = reinterpret_cast<const T*>(&raw[kv]);
-      float x[8];
-      uint32_t top = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = Cvt<T>::to_f(e[j]);
-        top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
+  for (int k = 0; k < HP; ++k) {
+    const int h = h0 + k;
+    const bool ok = p.ok && h < a.pool.hkv;
+    char* dst[2] = {a.pool.k + p.page * a.pool.k_sp + h * a.pool.k_sh + p.row * a.pool.k_ss,
+                    a.pool.v + p.page * a.pool.v_sp + h * a.pool.v_sh + p.row * a.pool.v_ss};
+    if constexpr (ST == GORGON_KV_NATIVE) {
+      if (ok) {
+        reinterpret_cast<uint4*>(dst[0])[sub] = raw[k][0];
+        reinterpret_cast<uint4*>(dst[1])[sub] = raw[k][1];
       }
+    } else {
 #pragma unroll
-      for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      float inv, scale;
-      row_scale<ST>(top, inv, scale);
-      uint8_t q[8];
+      for (int kv = 0; kv < 2; ++kv) {
+        // |x| as 16-bit integers, two at a time, orders like |x| (infinities and NaN on top)
+        const uint32_t* two = reinterpret_cast<const uint32_t*>(&raw[k][kv]);
+        uint32_t top = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) q[j] = store8<ST>(x[j], inv);
-      if (p.ok) {
-        uint2 w;
-        w.x = q[0] | (q[1] << 8) | (q[2] << 16) | (static_cast<uint32_t>(q[3]) << 24);
-        w.y = q[4] | (q[5] << 8) | (q[6] << 16) | (static_cast<uint32_t>(q[7]) << 24);
-        reinterpret_cast<uint2*>(dst[kv])[sub] = w;
-        if (sub == 0) {
-          float* sc = kv ? a.pool.vs + p.page * a.pool.vs_sp + h * a.pool.vs_sh + p.row * a.pool.vs_ss
-                         : a.pool.ks + p.page * a.pool.ks_sp + h * a.pool.ks_sh + p.row * a.pool.ks_ss;
-          *sc = scale;
+        for (int j = 0; j < 4; ++j) top = __vmaxu2(top, two[j] & 0x7fff7fffu);
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const uint16_t most = static_cast<uint16_t>(max(top & 0xffffu, top >> 16));
+        float inv, scale;
+        row_scale<ST>(__float_as_uint(Cvt<T>::to_f(*reinterpret_cast<const T*>(&most))), inv, scale);
+        const T* e = reinterpret_cast<const T*>(&raw[k][kv]);
+        if (ok) {
+          uint2 w;
+          w.x = store8x4<ST>(Cvt<T>::to_f(e[0]), Cvt<T>::to_f(e[1]), Cvt<T>::to_f(e[2]), Cvt<T>::to_f(e[3]), inv);
+          w.y = store8x4<ST>(Cvt<T>::to_f(e[4]), Cvt<T>::to_f(e[5]), Cvt<T>::to_f(e[6]), Cvt<T>::to_f(e[7]), inv);
+          reinterpret_cast<uint2*>(dst[kv])[sub] = w;
+          if (sub == 0) {
+            float* sc = kv ? a.pool.vs + p.page * a.pool.vs_sp + h * a.pool.vs_sh + p.row * a.pool.vs_ss
+                           : a.pool.ks + p.page * a.pool.ks_sp + h * a.pool.ks_sh + p.row * a.pool.ks_ss;
+            *sc = scale;
+          }
         }
       }
     }
@@ -302,39 +320,55 @@ __device__ __forceinline__ uint32_t pair16(float x, float y, __half) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Rows of 16 * LPR stored bytes to rows of T (the pages' own type when NATIVE).
-template <typename T, int ST, int LPR>
+// Rows of 16 * LPR stored bytes to rows of T (the pages' own type when NATIVE),
+// HP heads of a row for every LPR threads (as above).
+template <typename T, int ST, int LPR, int HP>
 __global__ void __launch_bounds__(kThreads) paged_read_vec_kernel(const ReadArgs a) {
   __shared__ int32_t s_cu[kCuCached + 1];
   const int32_t* cu = cached_cu(a.cu, a.pool.batch, s_cu);
   const int sub = threadIdx.x % LPR;
   const int64_t item = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / LPR;
   if (item >= a.items) return;
-  const int r = static_cast<int>(item / a.pool.hkv);
-  const int h = static_cast<int>(item - static_cast<int64_t>(r) * a.pool.hkv);
+  const int per_row = (a.pool.hkv + HP - 1) / HP;
+  const int r = static_cast<int>(item / per_row);
+  const int h0 = static_cast<int>(item - static_cast<int64_t>(r) * per_row) * HP;
   const Place p = read_place(a, cu, r);
   if (!p.ok) return;
-  const uint4 raw[2] = {
-      __ldcs(reinterpret_cast<const uint4*>(a.pool.k + p.page * a.pool.k_sp + h * a.pool.k_sh + p.row * a.pool.k_ss) + sub),
-      __ldcs(reinterpret_cast<const uint4*>(a.pool.v + p.page * a.pool.v_sp + h * a.pool.v_sh + p.row * a.pool.v_ss) + sub)};
-  uint4* out[2] = {reinterpret_cast<uint4*>(a.k + r * a.k_sn + h * a.k_sh),
-                   reinterpret_cast<uint4*>(a.v + r * a.v_sn + h * a.v_sh)};
-  if constexpr (ST == GORGON_KV_NATIVE) {
-    __stcs(out[0] + sub, raw[0]);
-    __stcs(out[1] + sub, raw[1]);
-  } else {
-    const float sc[2] = {a.pool.ks[p.page * a.pool.ks_sp + h * a.pool.ks_sh + p.row * a.pool.ks_ss],
-                         a.pool.vs[p.page * a.pool.vs_sp + h * a.pool.vs_sh + p.row * a.pool.vs_ss]};
+  const char* src[2] = {a.pool.k + p.page * a.pool.k_sp + p.row * a.pool.k_ss, a.pool.v + p.page * a.pool.v_sp + p.row * a.pool.v_ss};
+  uint4 raw[HP][2] = {};
+  float sc[HP][2] = {};
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      const uint8_t* e = reinterpret_cast<const uint8_t*>(&raw[kv]);
-      uint32_t w[8];
+  for (int k = 0; k < HP; ++k) {
+    const int h = h0 + k;
+    if (h >= a.pool.hkv) break;
+    raw[k][0] = __ldcs(reinterpret_cast<const uint4*>(src[0] + h * a.pool.k_sh) + sub);
+    raw[k][1] = __ldcs(reinterpret_cast<const uint4*>(src[1] + h * a.pool.v_sh) + sub);
+    if constexpr (ST != GORGON_KV_NATIVE) {
+      sc[k][0] = a.pool.ks[p.page * a.pool.ks_sp + h * a.pool.ks_sh + p.row * a.pool.ks_ss];
+      sc[k][1] = a.pool.vs[p.page * a.pool.vs_sp + h * a.pool.vs_sh + p.row * a.pool.vs_ss];
+    }
+  }
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        w[j] = pair16(stands_for(load8<ST>(e[2 * j]), sc[kv], type_top<T>()),
-                      stands_for(load8<ST>(e[2 * j + 1]), sc[kv], type_top<T>()), T{});
-      __stcs(out[kv] + 2 * sub, make_uint4(w[0], w[1], w[2], w[3]));
-      __stcs(out[kv] + 2 * sub + 1, make_uint4(w[4], w[5], w[6], w[7]));
+  for (int k = 0; k < HP; ++k) {
+    const int h = h0 + k;
+    if (h >= a.pool.hkv) break;
+    uint4* out[2] = {reinterpret_cast<uint4*>(a.k + r * a.k_sn + h * a.k_sh),
+                     reinterpret_cast<uint4*>(a.v + r * a.v_sn + h * a.v_sh)};
+    if constexpr (ST == GORGON_KV_NATIVE) {
+      __stcs(out[0] + sub, raw[k][0]);
+      __stcs(out[1] + sub, raw[k][1]);
+    } else {
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const uint8_t* e = reinterpret_cast<const uint8_t*>(&raw[k][kv]);
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          w[j] = pair16(stands_for(load8<ST>(e[2 * j]), sc[k][kv], type_top<T>()),
+                        stands_for(load8<ST>(e[2 * j + 1]), sc[k][kv], type_top<T>()), T{});
+        __stcs(out[kv] + 2 * sub, make_uint4(w[0], w[1], w[2], w[3]));
+        __stcs(out[kv] + 2 * sub + 1, make_uint4(w[4], w[5], w[6], w[7]));
+      }
     }
   }
 }
@@ -550,6 +584,18 @@ int by_lpr(int lpr, F&& f) {
 }
 inline bool pow2_upto32(int x) { return x >= 1 && x <= 32 && (x & (x - 1)) == 0; }
 
+// How many groups of LPR threads the (row, head) pairs take: `heads` heads each
+// once the pairs alone would fill the SMs (2048 threads each) twice over, where
+// the lookups' latency counts for every wave (a read of 16 sequences of up to
+// 8192 int8 rows: 75 us a head each, 66 us with four, 5.9 TB/s; an append of 8000
+// rows to e4m3: 18.1 us with four, 17.0 us with two, 2.9 TB/s, bound by the
+// conversions); one head each below, where all run at once (64 single rows:
+// 3.4 us either way, a launch).
+int64_t groups(int64_t items, int hkv, int lpr, int heads) {
+  if (items * lpr < int64_t(2) * 2048 * sm_count()) return items;
+  return items / hkv * ceil_div(hkv, heads);
+}
+
 template <typename T, int ST>
 int append_t(const AppendArgs& a, bool vec, cudaStream_t st) {
   if constexpr (sizeof(T) == 2) {
@@ -557,8 +603,12 @@ int append_t(const AppendArgs& a, bool vec, cudaStream_t st) {
     if (vec && a.pool.d % 8 == 0 && pow2_upto32(lpr))
       return by_lpr(lpr, [&](auto l) {
         constexpr int LPR = decltype(l)::value;
-        const int64_t blocks = ceil_div(a.items * LPR, kThreads);
-        paged_append_vec_kernel<T, ST, LPR><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(a);
+        constexpr int kHeads = 2;
+        AppendArgs x = a;
+        x.items = groups(a.items, a.pool.hkv, LPR, kHeads);
+        const unsigned blocks = static_cast<unsigned>(ceil_div(x.items * LPR, kThreads));
+        if (x.items < a.items) paged_append_vec_kernel<T, ST, LPR, kHeads><<<blocks, kThreads, 0, st>>>(x);
+        else paged_append_vec_kernel<T, ST, LPR, 1><<<blocks, kThreads, 0, st>>>(x);
         return check_cuda(cudaGetLastError(), "gorgon_paged_append launch");
       });
   }
@@ -583,8 +633,12 @@ int read_t(const ReadArgs& a, bool vec, cudaStream_t st) {
     if (vec && a.pool.d % per == 0 && pow2_upto32(lpr))
       return by_lpr(lpr, [&](auto l) {
         constexpr int LPR = decltype(l)::value;
-        const int64_t blocks = ceil_div(a.items * LPR, kThreads);
-        paged_read_vec_kernel<T, ST, LPR><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(a);
+        constexpr int kHeads = 4;
+        ReadArgs x = a;
+        x.items = groups(a.items, a.pool.hkv, LPR, kHeads);
+        const unsigned blocks = static_cast<unsigned>(ceil_div(x.items * LPR, kThreads));
+        if (x.items < a.items) paged_read_vec_kernel<T, ST, LPR, kHeads><<<blocks, kThreads, 0, st>>>(x);
+        else paged_read_vec_kernel<T, ST, LPR, 1><<<blocks, kThreads, 0, st>>>(x);
         return check_cuda(cudaGetLastError(), "gorgon_paged_read launch");
       });
   }
