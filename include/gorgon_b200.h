@@ -504,7 +504,8 @@ GORGON_API int gorgon_paged_trim(const gorgon_paged_trim_params* p, void* stream
  *   counting the hops to its root;
  * and with window > 0 only if j's position is less than `window` positions
  * before the row's own (a tree row's position as above), or j < sinks.
- * Hidden rows contribute nothing, whatever they hold.
+ * Hidden rows contribute nothing, whatever they hold (e4m3 bytes are never
+ * NaN: gorgon_paged_append writes such a row with a NaN scale).
  * out = softmax(q k^T * scale) v over the visible rows (scale 0: 1 /
  * sqrt(head_dim)); lse (nullable, float, strides) the natural-log sum of
  * exponentials.  Rows of an unused slot, and rows with nothing to see (all

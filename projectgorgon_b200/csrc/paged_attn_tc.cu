@@ -18,8 +18,8 @@
 // so that the products see the stored numbers and the scales are applied in
 // fp32: K's to the scores, V's to the weights.  Pages of other sizes are
 // gathered row by row by warps 4 to 7 with 16-byte cp.async copies (which took
-// 1700 cycles a tile of 2300, most of them waiting for issue slots, so TMA is
-// used where it can be).  V rows that no row of the unit sees are made zeros.
+// 1700 cycles a tile, most of them waiting for issue slots, so TMA is used where
+// it can be).  V rows that no row of the unit sees are made zeros.
 //
 // Softmax per row is owned by one thread (TMEM lane = row): no shuffles.  The
 // running max moves only when a tile's max exceeds it by more than 8 (log2
@@ -30,6 +30,12 @@
 // the search replaces them by zeros, and the epilogue adds them to the rows
 // that do see them.
 //
+// Measured: 2048 new tokens over 32768 bf16 rows (32 heads on 8, 128 wide) 967 us
+// (to 1026 us, by the card's power), 1.10 PFLOP/s, the tensor pipe busy 75 % and the exponentials' 61 % of the time;
+// 64-node trees of 16 sequences over 8192 e4m3 rows 267 us, bound by shared
+// memory (operands, widening and scales); bf16 pages of 16 rows cost 5 % over
+// pages of 64.
+
 // Every mbarrier wait is bounded; a wait that runs out raises kErrTimeout, and
 // the CTA drains its copies and products, frees TMEM and returns.
 #include <algorithm>
@@ -114,9 +120,9 @@ __device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool take) {
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// True on one lane of a converged warp, in a form that tells the compiler so: TMA
-// and tcgen05 instructions behind it take their operands from uniform registers
-// without a loop over the lanes that might be active.
+// True on one lane of a converged warp, in a form that the compiler knows to be
+// one: a TMA copy behind it is issued in a few cycles, behind `lane == 0` it took
+// about 250 (2048 new tokens over 16384 rows in pages of 16: 574 -> 472 us).
 __device__ __forceinline__ bool elect_one() {
   uint32_t yes;
   asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}" : "=r"(yes));
@@ -1132,6 +1138,7 @@ __global__ void __launch_bounds__(TcCfg<T, ST, D, MT>::kThreads, 1) paged_tc_ker
       if (warp == 0) {
         if (elect_one()) issue_scores<C>(a, cur, end, smem, bars, tmem, fmt);
       } else if (warp == 1) {
+        // (elected, P V goes out too closely packed for the exponentials beside it: pages of 16 rows 469 -> 514 us)
         if (lane == 0) issue_outputs<C>(a, cur, end, smem, bars, tmem, fmt);
       } else if (warp < 4) {
         if (a.tma) load_tiles<C>(a, warp == 3 ? &vmap : &kmap, cur, end, smem, bars, warp - 2);

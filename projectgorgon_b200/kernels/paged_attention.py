@@ -69,7 +69,9 @@ def paged_attention(
     ``max_depth`` hops.  ``window`` hides rows ``window`` or more positions before
     a row's own (a tree row's position is the cached length plus its depth),
     except the first ``sinks`` rows.  Hidden rows contribute nothing, even when
-    they hold infinities or NaN.  ``scale`` (default ``D ** -0.5``) is positive.
+    they hold infinities or NaN (an 8-bit row holds NaN in its scale, as
+    ``paged_cache_append`` writes it; a page filled otherwise must have no e4m3 NaN
+    among its bytes).  ``scale`` (default ``D ** -0.5``) is positive.
 
     Returns ``out`` shaped like ``q``, and with ``return_lse`` also the
     natural-log sum of exponentials, float32 ``[B, Hq, n]`` (packed:
