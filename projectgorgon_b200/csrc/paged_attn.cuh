@@ -312,11 +312,8 @@ __device__ __forceinline__ int tree_bits(const PagedAttn& a, const Seq& s, int b
     const bool in = !a.window || hop < a.window || s.P + cur < a.sinks;
     if (near && in) bits[cur >> 5] |= 1u << (cur & 31);
     const int up = par[cur];
-    if (up < 0) break;
-    if (up >= s.c) {
-      raise_device_error(a.pool.err, kErrBadParent);
-      break;
-    }
+    if (up < -1 || up >= s.c) raise_device_error(a.pool.err, kErrBadParent);
+    if (up < 0 || up >= s.c) break;
     cur = up;
   }
   return hop;

@@ -768,7 +768,7 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
             if ((at >> 5) == k) word[k] |= 1u << (at & 31);
         }
         const int up = par[at];
-        if (up >= c) raise_device_error(a.pool.err, kErrBadParent);
+        if (up < -1 || up >= c) raise_device_error(a.pool.err, kErrBadParent);
         if (up < 0 || up >= c) break;
         at = up;
       }

@@ -159,6 +159,40 @@ def test_large_trees(n):
     check(p, [n], 2, parents=[random_tree(n, rng, 12)], max_depth=7)
 
 
+@pytest.mark.parametrize("storage", STORES)
+@pytest.mark.parametrize("ps", [8, 32, 128, 192])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window", [None, 150])
+def test_page_sizes(storage, ps, D, window):
+    """Pages of every size that a copy takes in one box, of tiles that begin inside a page."""
+    p = Paged([100 + 40, 700 + 40, 40], 2, D, ps, torch.bfloat16, storage, seed=ps)
+    check(p, [40] * 3, 8, window=window, sinks=3)
+
+
+@pytest.mark.parametrize("storage", STORES)
+@pytest.mark.parametrize("n", [1, 40])
+def test_pages_repeated_by_strides(storage, n):
+    """Kv heads that are one head in memory (stride 0)."""
+    p = Paged([n + 90, n + 300], 1, 128, 16, torch.bfloat16, storage, seed=n)
+    q = torch.randn(2, 8, n, 128, device="cuda").bfloat16()
+    wide = lambda t: None if t is None else t.expand(-1, 4, *t.shape[2:])  # noqa: E731
+    out = G.paged_attention(q, wide(p.k_pages), wide(p.v_pages), p.table_d, p.lens_d, k_scale=wide(p.k_scale), v_scale=wide(p.v_scale))
+    for b in range(2):
+        near(out[b], q[b], p, b, visible(p.lens[b], n))
+
+
+@pytest.mark.parametrize("backend", ["auto", "mma", "tcgen05", "simt"])
+@pytest.mark.parametrize("bad", [-2, -2 ** 31, 3, 2 ** 31 - 1])
+def test_bad_parents_are_reported(backend, bad):
+    """A parent outside the tree ends the walk there, as a root's does."""
+    p = Paged([43, 63], 2, 128, 16, torch.bfloat16, seed=1)
+    q = torch.randn(2, 16, 3, 128, device="cuda").bfloat16()
+    out = G.paged_attention(q, *p.args, parents=torch.tensor([[-1, 0, 1], [-1, bad, 1]]), backend=backend)
+    assert G.device_error(clear=True) == 1
+    near(out[0], q[0], p, 0, visible(43, 3, [-1, 0, 1]))
+    near(out[1], q[1], p, 1, visible(63, 3, [-1, -1, 1]))
+
+
 @pytest.mark.parametrize("what", [math.inf, -math.inf])
 @pytest.mark.parametrize("n", [1, 5, 80])
 def test_infinite_keys(what, n):
