@@ -72,8 +72,12 @@ Kernel choose(const gorgon_paged_attn_params* p, const PagedAttn& a) {
     case GORGON_PAGED_MMA: return mma ? Kernel::kMma : Kernel::kNone;
     case GORGON_PAGED_TCGEN05: return tc ? Kernel::kTc : Kernel::kNone;
     default:
-      // up to 16 packed rows fill one tile of the warp-level kernel
-      if (static_cast<int64_t>(a.n) * a.group > 16 && tc) return Kernel::kTc;
+      // The warp-level kernel passes the cache once for every 16 packed rows, the
+      // tcgen05 kernel once for 256, at a higher price a pass where rows are widened.
+      // 16 sequences of 8192 rows, us, warp-level / tcgen05: 16-bit 104 / 125 for 16
+      // packed rows, 183 / 126 for 32; int8 92 / 201 for 16, 158 / 203 for 32, 235 / 204
+      // for 48.
+      if (static_cast<int64_t>(a.n) * a.group > (p->kv.storage == GORGON_KV_NATIVE ? 16 : 32) && tc) return Kernel::kTc;
       return mma ? Kernel::kMma : Kernel::kSimt;
   }
 }
