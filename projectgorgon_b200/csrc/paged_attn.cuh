@@ -319,6 +319,58 @@ __device__ __forceinline__ int tree_bits(const PagedAttn& a, const Seq& s, int b
   return hop;
 }
 
+// The unit of 8-bit rows' weights.  A weight (at most 2^8) times its V scale
+// enters the products as f16, in units of 2^(e - kUnit), where its scale lies in
+// [2^(e - 1 - kSpan), 2^e): it stays below 2^15, and what f16 takes off a weight
+// is at most half a step of 2^-10 of it, or 2^-27 (half of f16's smallest step,
+// at the smallest scale; a row's largest weight is 1 or more).  Rows outside that
+// span are not taken by the products: they are added in fp32, so that a large
+// row, seen or hidden, takes nothing from the small ones.  e follows the tiles up
+// and down, but stays within kRise of the smallest scale met: above, what f16
+// takes off a large row of little weight would count beside small rows of much.
+// The output row follows e by exact powers of two in fp32, which holds it while e
+// is within kReach of the largest scale met; scales that spread by more than both
+// allow leave every row to fp32 (only terms below 2^-130 of the largest leave its
+// range).  Scales below 2^-106, those of rows below 2^-100, do not count as
+// small: rows of zeros have them.
+// (With weights held below 2^4, kUnit 11, 64-node trees over 16 x 8192 e4m3 rows took 298 us, not 275.)
+constexpr int kUnit = 7, kSpan = 5, kRise = 10, kReach = 64;
+constexpr int kNoExp = -116;  // nothing met yet
+constexpr uint32_t kFloorBits = 21u << 23;  // 2^-106
+
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
+// The scale's bits above the floor's, for a minimum; wraps to the top below it.
+__device__ __forceinline__ uint32_t above_floor(float scale) { return (__float_as_uint(scale) & 0x7fffffffu) - kFloorBits; }
+
+struct VUnit {
+  int e = kNoExp;                   // the unit's exponent
+  int top = kNoExp, low = 1 << 20;  // the largest and smallest met (scale < 2^)
+  bool closed = false;              // every row is outside
+  // The tile's scales, largest `hi` (bits of a float) and smallest `lo`
+  // (above_floor), lie within the unit's span.
+  __device__ __forceinline__ bool fits(int hi, uint32_t lo) const {
+    return !closed && hi < (e + 127) << 23 && lo >= static_cast<uint32_t>(max(e - kSpan + 126 - 21, 0)) << 23;
+  }
+  // A scale in units of 2^(e - kUnit) is outside the span (a NaN is not).
+  static __device__ __forceinline__ bool outside(float f) {
+    return fabsf(f) >= static_cast<float>(1 << kUnit) || fabsf(f) < static_cast<float>(1 << kUnit) / (2 << kSpan);
+  }
+  // Follows a tile; true when rows outside the span remain.
+  __device__ __forceinline__ bool follow(int hi, uint32_t lo) {
+    if (fits(hi, lo)) return false;
+    const int e_hi = min((hi >> 23) - 126, 128);
+    const int e_lo = lo >> 31 ? e_hi : static_cast<int>((lo + kFloorBits) >> 23) - 126;
+    top = max(top, e_hi);
+    if (!(lo >> 31)) low = min(low, e_lo);
+    const int most = low + kRise;
+    // a tile that spreads keeps the unit; the first one takes its large rows, unless they are too large
+    const int want = e_hi - e_lo <= kSpan ? e_hi : e != kNoExp ? e : e_hi <= most ? e_hi : e_lo + kSpan;
+    e = max(min(want, most), max(top - kReach, kNoExp));
+    closed = e > most;
+    return !fits(hi, lo);
+  }
+};
+
 // Launches a kernel so that it may start while the one before it in the stream
 // ends (it waits for that itself, by griddepcontrol.wait).
 template <typename K, typename... More>

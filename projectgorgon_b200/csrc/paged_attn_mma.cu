@@ -17,7 +17,7 @@
 // softmax was padding).  P^T's fragment is S^T's transposed, by movmatrix.
 // 8-bit rows are widened in registers to f16, exactly, whatever the type of
 // Q: f16 takes the fewest instructions per value.  The K scale is applied to
-// the score and the V scale to the weight, in fp32.  bf16 queries enter as f16
+// the score and the V scale to the weight, in fp32 (see VUnit).  bf16 queries enter as f16
 // times a power of two per row that puts the row's largest value near 2^8
 // (exact but for values below 2^-22 of it, which lose less than the fp32 sum
 // of the score does).  So that a thread widens whole 16-byte pieces, the head
@@ -131,14 +131,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-
-// f16 weights times V scales need f16's range: they are taken in units of
-// 2^(E - 6), with 2^E above the largest V scale that the warp has met in the
-// unit, so that they stay below 2^14 (a weight is at most 2^8) and keep a row's
-// full precision down to 2^-20 of the largest.  E only grows; the output row
-// follows it as it follows the running max.
-__device__ __forceinline__ float pow2(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
-constexpr int kNoExp = -116;  // nothing met yet
 
 // What the loop does rarely lives in calls, so that the loop itself stays short
 // and in the instruction cache.
@@ -344,7 +336,7 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
   uint32_t qf[NT][D / 16][2];
   float o[NT][D / 16][4];
   float m[NT][2], l[NT][2], qscale[NT][2];
-  int unit_exp = kNoExp;
+  VUnit vunit;  // of the warp's weights times V scales
   float unit_scale = 1.f;
   bool first_unit = true;
   int stage = 0;
@@ -411,8 +403,8 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[nt][t2][e] = 0.f;
       }
-      unit_exp = kNoExp;
-      unit_scale = pow2(6 - kNoExp);
+      vunit = VUnit{};
+      unit_scale = pow2(kUnit - kNoExp);
     }
 
 #pragma unroll 1
@@ -465,28 +457,36 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
         // ---- softmax
         const float* sc = reinterpret_cast<const float*>(st + C::kOffWord + 16);
         float vsc[KB][2];
-        float regrade = 1.f;
+        uint32_t slow = 0;  // keys whose rows are added one by one: those outside the unit's span, or (16-bit) all
         if constexpr (!C::kWide) {
           float top = 0.f;
+          uint32_t low = 0xffffffffu;
 #pragma unroll
           for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
               vsc[b][hh] = sc[G + b * 16 + hh * 8 + g];  // (0 for keys that were not fetched)
-              top = fmaxf(top, vsc[b][hh]);
+              top = fmaxf(top, fabsf(vsc[b][hh]));        // (NaN never wins)
+              low = min(low, above_floor(vsc[b][hh]));
             }
-          if (__any_sync(0xffffffffu, __float_as_int(top) >= (unit_exp + 126) << 23)) {
+          if (__any_sync(0xffffffffu, !vunit.fits(__float_as_int(top), low))) {
+            const int was = vunit.e;
+            const bool far = vunit.follow(__reduce_max_sync(0xffffffffu, __float_as_int(top)), __reduce_min_sync(0xffffffffu, low));
+            if (far) slow = __ballot_sync(0xffffffffu, vunit.closed || vunit.outside(sc[G + lane] * pow2(kUnit - vunit.e)));
+            if (vunit.e != was) {
+              unit_scale = pow2(kUnit - vunit.e);
+              const int half = (was - vunit.e) / 2;  // (the whole step may pass fp32's range)
+              const float r0 = pow2(half), r1 = pow2(was - vunit.e - half);
 #pragma unroll
-            for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-            const int e = (__float_as_int(top) >> 23) - 126;  // top < 2^e
-            if (e > unit_exp) {
-              regrade = unit_exp == kNoExp ? 0.f : pow2(unit_exp - e);
-              unit_exp = e;
-              unit_scale = pow2(6 - e);
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) o[nt][t][e] = o[nt][t][e] * r0 * r1;
             }
           }
         }
-        bool move = regrade != 1.f;
+        bool move = false;
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
           const float k0 = C::kWide ? 1.f : sc[b * 16 + g], k1 = C::kWide ? 1.f : sc[b * 16 + 8 + g];
@@ -534,7 +534,6 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
               alpha[e] = ex2(m[nt][e] - (top == -INFINITY ? 0.f : top));
               m[nt][e] = top;
               l[nt][e] *= alpha[e];
-              alpha[e] *= regrade;
             }
 #pragma unroll
             for (int t = 0; t < D / 16; ++t) {
@@ -558,7 +557,6 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
             }
           }
         // ---- a partly hidden group of 16-bit rows: 0 * infinity must not reach a row that does not see it
-        bool slow = false;
         if constexpr (C::kWide) {
           if (!plain) {
             bool odd = false;
@@ -569,14 +567,14 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
 #pragma unroll
               for (int e = 0; e < 4; ++e) odd |= (ww[e] & top) == top || ((ww[e] >> 16) & top) == top;
             }
-            slow = __any_sync(0xffffffffu, odd);
+            if (__any_sync(0xffffffffu, odd)) slow = kAll;
           }
         }
         // ---- output rows
-        if (C::kWide && slow) {
-          // One key at a time on the CUDA cores.  The weights go over the K rows, which are done with.
+        if (slow) {
+          // Keys one at a time on the CUDA cores.  The weights go over the K rows, which are done with.
           float* w = reinterpret_cast<float*>(st);
-          static_assert(!C::kWide || C::M * G * 4 <= C::kHalf, "weights fit the K block");
+          static_assert(C::M * G * 4 <= C::kHalf, "weights fit the K block");
           __syncwarp();
 #pragma unroll
           for (int b = 0; b < KB; ++b)
@@ -588,21 +586,31 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
                     (hidden[b] >> (4 * nt + e)) & 1u ? -1.f : x[b][nt][e];
           __syncwarp();
 #pragma unroll 1
-          for (int k = 0; k < G; ++k)
+          for (uint32_t rest = slow; rest; rest &= rest - 1) {
+            const int k = __ffs(rest) - 1;
+            const float f = C::kWide ? 1.f : sc[G + k] * unit_scale;
 #pragma unroll
             for (int t = 0; t < D / 16; ++t)
 #pragma unroll
               for (int hh = 0; hh < 2; ++hh) {
-                const float v = Cvt<T>::to_f(*(reinterpret_cast<const T*>(st + C::kHalf + C::at(k, 2 * t + hh)) + g));
+                float v;
+                if constexpr (C::kWide) {
+                  v = Cvt<T>::to_f(*(reinterpret_cast<const T*>(st + C::kHalf + C::at(k, 2 * t + hh)) + g));
+                } else {
+                  const int d = g * (D / 8) + 2 * t + hh;
+                  v = byte_value<ST>(st[C::kHalf + C::at(k, d >> 4) + (d & 15)]);
+                }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                   for (int e = 0; e < 2; ++e) {
                     const float p = w[(nt * 8 + 2 * c + e) * G + k];
-                    if (!(p < 0.f)) o[nt][t][2 * hh + e] = fmaf(p, v, o[nt][t][2 * hh + e]);
+                    if (!(p < 0.f)) o[nt][t][2 * hh + e] = fmaf(C::kWide ? p : p * f, v, o[nt][t][2 * hh + e]);
                   }
               }
-        } else {
+          }
+        }
+        if (!C::kWide || !slow) {
 #pragma unroll
           for (int b = 0; b < KB; ++b) {
             uint32_t pf[NT][2];
@@ -614,8 +622,9 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
                 if constexpr (!C::kWide) {
                   const float f = vsc[b][hh] * unit_scale;
                   // (a hidden key's weight is 0 whatever its scale)
-                  p0 = !plain && p0 == 0.f ? 0.f : p0 * f;
-                  p1 = !plain && p1 == 0.f ? 0.f : p1 * f;
+                  const bool done = slow && ((slow >> (b * 16 + hh * 8 + g)) & 1u);
+                  p0 = done || (!plain && p0 == 0.f) ? 0.f : p0 * f;
+                  p1 = done || (!plain && p1 == 0.f) ? 0.f : p1 * f;
                 }
                 pf[nt][hh] = transpose8(pack2(p0, p1, X{}));
               }
@@ -699,7 +708,7 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float f = ex2(m[nt][e] - s_row[nt * 8 + 2 * c + e].x);
-        if constexpr (!C::kWide) f *= pow2(unit_exp - 6);
+        if constexpr (!C::kWide) f *= pow2(vunit.e - kUnit);
 #pragma unroll
         for (int t = 0; t < D / 16; ++t) {
           o[nt][t][e] = m[nt][e] == -INFINITY ? 0.f : o[nt][t][e] * f;  // (nothing seen: weight 0)

@@ -16,7 +16,8 @@
 // tiles that the products read.  8-bit rows land in a ring of raw bytes, and
 // warps 4 to 7 widen their 32 rows from there to f16, exactly (paged_widen.cuh),
 // so that the products see the stored numbers and the scales are applied in
-// fp32: K's to the scores, V's to the weights.  Pages of other sizes are
+// fp32: K's to the scores, V's to the weights (see VUnit; rows outside its span
+// are added after the tile's product, add_far).  Pages of other sizes are
 // gathered row by row by warps 4 to 7 with 16-byte cp.async copies (which took
 // 1700 cycles a tile, most of them waiting for issue slots, so TMA is used where
 // it can be).  V rows that no row of the unit sees are made zeros.
@@ -217,29 +218,27 @@ __device__ __forceinline__ bool strip_rows(uint8_t* st, int half, uint32_t keep)
   return odd;
 }
 
-__device__ __forceinline__ float pow2i(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
-constexpr int kNoExp = -116;
-
 // What the softmax needs of a tile: the half's valid word, and (8-bit) K's scales
-// times the softmax scale and V's scales in units of 2^(E - 6), with 2^E above
-// every V scale of the unit so far, so that weights (at most 2^8) times them
-// stay in f16's range (see paged_attn_mma.cu).  Both halves know all 64 V
-// scales (`top`: their maximum), and so the same E.
+// times the softmax scale and V's scales in the unit of the tile (VUnit).  Both
+// halves know all 64 V scales (`vs` its own, `vo` the other half's), and so the
+// same unit.  Rows outside its span keep their factor; the softmax knows them by it.
+constexpr uint32_t kFar = 2, kAllFar = 4;  // in the tile's word: it has such rows, all are
 template <typename C>
 __device__ __forceinline__ void write_meta(const PagedAttn& a, uint8_t* smem, uint32_t stage, int half, uint32_t valid, float ks, float vs,
-                                           float top, bool first, int& unit_exp, bool plain) {
+                                           float vo, bool first, VUnit& unit, bool plain) {
   const int lane = threadIdx.x & 31;
   uint8_t* meta = smem + C::kOffMeta + stage * C::kMetaBytes;
   if (lane == 0) reinterpret_cast<uint32_t*>(meta)[half] = valid;
   if constexpr (!C::kWide) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    unit_exp = max(first ? kNoExp : unit_exp, (__float_as_int(top) >> 23) - 126);
+    if (first) unit = VUnit{};
+    const float big = fmaxf(fmaxf(0.f, fabsf(vs)), fabsf(vo));  // (NaN never wins)
+    const bool far = unit.follow(__reduce_max_sync(0xffffffffu, __float_as_int(big)),
+                                 __reduce_min_sync(0xffffffffu, min(above_floor(vs), above_floor(vo))));
     // (each half says whether its rows are whole and seen by all, in its half of the word)
-    if (lane == 0) reinterpret_cast<uint16_t*>(meta + 12)[half] = plain && valid == 0xffffffffu ? 0 : 1;
-    if (lane == 0 && half == 0) reinterpret_cast<int*>(meta)[2] = unit_exp;
+    if (lane == 0) reinterpret_cast<uint16_t*>(meta + 12)[half] = (plain && valid == 0xffffffffu ? 0 : 1) | (far ? kFar : 0) | (unit.closed ? kAllFar : 0);
+    if (lane == 0 && half == 0) reinterpret_cast<int*>(meta)[2] = unit.e;
     reinterpret_cast<float*>(meta + 16)[half * 32 + lane] = ks * a.scale_log2;
-    reinterpret_cast<float*>(meta + 16)[kTile + half * 32 + lane] = vs * pow2i(6 - unit_exp);
+    reinterpret_cast<float*>(meta + 16)[kTile + half * 32 + lane] = vs * pow2(kUnit - unit.e);
   }
 }
 
@@ -353,7 +352,7 @@ __device__ void finish_tiles(const PagedAttn& a, TileCursor f, int end, uint8_t*
         vo = __ldg(a.pool.vs + page[1] * a.pool.vs_sp + kvh * a.pool.vs_sh + row[1] * a.pool.vs_ss);
     }
   };
-  int unit_exp = kNoExp;
+  VUnit unit;
   bool first = true;  // the tile is the unit's first here
   bool plain = Common(a, f).plain(a, f.tile() * kTile), next_plain = false;
   look_up();
@@ -369,7 +368,7 @@ __device__ void finish_tiles(const PagedAttn& a, TileCursor f, int end, uint8_t*
   Slot<C::kStages> hs;
   while (true) {
     const uint32_t valid = __ballot_sync(0xffffffffu, held);
-    const float k1 = ks, v1 = vs, top = fmaxf(vs, vo);  // (NaN never wins)
+    const float k1 = ks, v1 = vs, o1 = vo;
     const bool p1 = plain, f1 = first, again = more;
     if (more) {  // the next tile's scales, and the page of the one after
       take();
@@ -395,7 +394,7 @@ __device__ void finish_tiles(const PagedAttn& a, TileCursor f, int end, uint8_t*
       widen_rows<ST, C>(src, st, half, is_v ? valid : 0xffffffffu);
       fence_proxy_async_smem();
     }
-    if (is_v) write_meta<C>(a, smem, hs.stage, half, valid, k1, v1, top, f1, unit_exp, p1);
+    if (is_v) write_meta<C>(a, smem, hs.stage, half, valid, k1, v1, o1, f1, unit, p1);
     __syncwarp();
     if (lane == 0) {
       if constexpr (!C::kWide) mbar_arrive(&bars->raw_empty[is_v][ls.stage]);
@@ -494,7 +493,8 @@ __device__ void produce(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
     return true;
   };
   Slot<C::kStages> hs;  // the stage handed over
-  int done = 0, unit_exp = kNoExp;
+  int done = 0;
+  VUnit unit;
   // Hands tile `done` over: its copies have landed.
   auto hand_over = [&]() -> bool {
     const uint2 h = info[done % C::kInfo];
@@ -514,7 +514,7 @@ __device__ void produce(const PagedAttn& a, TileCursor cur, int end, uint8_t* sm
       } else if (!((h.y & 1u) && h.x == 0xffffffffu)) {
         if (strip_rows<T, C>(st, half, h.x)) atomicOr(&bars->odd, h.y & 1u ? 2 : 1);
       }
-      write_meta<C>(a, smem, hs.stage, half, h.x, ks, vs, fmaxf(vs, vo), done == 0 || (h.y & 2u), unit_exp, h.y & 1u);
+      write_meta<C>(a, smem, hs.stage, half, h.x, ks, vs, vo, done == 0 || (h.y & 2u), unit, h.y & 1u);
     }
     fence_proxy_async_smem();
     __syncwarp();
@@ -656,6 +656,46 @@ __device__ __forceinline__ uint64_t row_word(const PagedAttn& a, const TileCurso
   return w;
 }
 
+// Adds the columns of a tile whose rows lie outside the unit's span (`far`) to
+// the output rows of a warp, key by key from the pages, once the tile's product is
+// complete (the next one waits for this warp's next weights).  x: a row's scores
+// less its running max.  Called rarely: out of the loop's registers.
+template <int ST, int D>
+__device__ __noinline__ void add_far(const PagedAttn& a, const TileCursor& cur, int j0, uint64_t far, const float* x, uint32_t o_addr,
+                                     int unit_exp) {
+  const float in_unit = pow2(kUnit - unit_exp);
+#pragma unroll 1
+  for (int c0 = 0; c0 < D; c0 += 32) {
+    uint32_t ov[32];
+    tmem_ld32(o_addr + c0, ov);
+    tmem_wait_ld();
+#pragma unroll 1
+    for (uint64_t rest = far; rest; rest &= rest - 1) {
+      const int c = __ffsll(static_cast<long long>(rest)) - 1;
+      const float p = ex2_approx(x[c]);
+      if (!__any_sync(0xffffffffu, p != 0.f)) continue;  // (rows that were not fetched, too)
+      int col, prow;
+      a.pool.split(j0 + c, col, prow);
+      const int page = a.pool.page(cur.b, col);
+      if (page >= 0 && p != 0.f) {
+        const float w = p * (a.pool.vs[page * a.pool.vs_sp + cur.kvh * a.pool.vs_sh + prow * a.pool.vs_ss] * in_unit);
+        const uint4* src = reinterpret_cast<const uint4*>(a.pool.v + page * a.pool.v_sp + cur.kvh * a.pool.v_sh + prow * a.pool.v_ss + c0);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const uint4 b = __ldg(src + q);
+          const uint32_t b4[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            ov[q * 16 + e] = __float_as_uint(fmaf(w, byte_value<ST>(static_cast<uint8_t>(b4[e >> 2] >> (8 * (e & 3)))), __uint_as_float(ov[q * 16 + e])));
+        }
+      }
+      __syncwarp();
+    }
+    tmem_st32(o_addr + c0, ov);
+  }
+  tmem_wait_st();
+}
+
 template <typename T, int ST, typename C>
 __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, uint8_t* smem, TcBars<C>* bars, uint32_t tmem) {
   using X = typename C::X;
@@ -729,12 +769,12 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
 #pragma unroll
             for (int o = 1; o < kChunks; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
             const int e2 = max(static_cast<int>(top >> 23) - 127, -100);
-            const float f = pow2i(8 - e2);
+            const float f = pow2(8 - e2);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               x[e] = pack16x2(__uint_as_float(x[e] << 16) * f, __uint_as_float(x[e] & 0xffff0000u) * f, false);
             qv[k] = make_uint4(x[0], x[1], x[2], x[3]);
-            if (chunk == 0) s_qs[wg * 128 + wq * 32 + rr] = pow2i(e2 - 8);
+            if (chunk == 0) s_qs[wg * 128 + wq * 32 + rr] = pow2(e2 - 8);
           }
           *reinterpret_cast<uint4*>(stage_row(rr, chunk)) = qv[k];
         }
@@ -836,6 +876,7 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
       for (int c = 0; c < kTile; c += 2) mx[(c >> 1) & 3] = fmax3(mx[(c >> 1) & 3], x[c], x[c + 1]);
       const float top = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]);
       float alpha = 1.f;
+      [[maybe_unused]] float regrade = 1.f;
       bool need = false;
       if constexpr (C::kWide) {
         const float tmax = top * qs;
@@ -863,10 +904,26 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
       l *= alpha;
       if constexpr (!C::kWide) {
         const int e = reinterpret_cast<const int*>(meta)[2];
-        if (e > unit_exp) {
-          alpha *= unit_exp == kNoExp ? 0.f : pow2i(unit_exp - e);
+        if (e != unit_exp) {
+          const int half = (unit_exp - e) / 2;  // (the whole step may pass fp32's range)
+          alpha *= pow2(half);
+          regrade = pow2(unit_exp - e - half);
           unit_exp = e;
           need = !fresh;
+        }
+      }
+      // Columns whose rows lie outside the unit's span: their scores are kept for add_far.
+      [[maybe_unused]] uint64_t far = 0;
+      [[maybe_unused]] float far_x[kMask && !C::kWide ? kTile : 1];
+      if constexpr (kMask && !C::kWide) {
+        const uint32_t word = reinterpret_cast<const uint32_t*>(meta)[3];
+        if (word & kFar) {
+          const float* f = reinterpret_cast<const float*>(meta + 16) + kTile;
+          const bool all = word & kAllFar;
+          far = __ballot_sync(0xffffffffu, all || VUnit::outside(f[lane])) |
+                static_cast<uint64_t>(__ballot_sync(0xffffffffu, all || VUnit::outside(f[32 + lane]))) << 32;
+#pragma unroll
+          for (int c = 0; c < kTile; ++c) far_x[c] = x[c];
         }
       }
       const float nmb = m_used == -INFINITY ? 0.f : -m_used;
@@ -899,7 +956,7 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
           f2_unpack(p1, z[2], z[3]);
           if (kMask) {  // a hidden key's weight is 0 whatever its scale
 #pragma unroll
-            for (int e = 0; e < 4; ++e) z[e] = y[e] == 0.f ? 0.f : z[e];
+            for (int e = 0; e < 4; ++e) z[e] = y[e] == 0.f || ((far >> (c + e)) & 1u) ? 0.f : z[e];
           }
           packed[(c - c0) >> 1] = pack16x2(z[0], z[1], false);
           packed[((c - c0) >> 1) + 1] = pack16x2(z[2], z[3], false);
@@ -926,7 +983,7 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
           tmem_ld32(o_addr + ch * 32, ov);
           tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
+          for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(C::kWide ? __uint_as_float(ov[c]) * alpha : __uint_as_float(ov[c]) * alpha * regrade);
           tmem_st32(o_addr + ch * 32, ov);
         }
         tmem_wait_st();
@@ -936,6 +993,13 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->p_full[bi]);
       vr.next();
+      if constexpr (kMask && !C::kWide) {
+        if (far) {
+          if (!warp_wait(&bars->p_free[i & 1u], (i >> 1) & 1u, abort, a.wait_ns)) return false;
+          tc_fence_after();
+          add_far<ST, D>(a, cur, j0, far, far_x, lane_base + kColO + wg * D, unit_exp);
+        }
+      }
       return true;
     };
     // Whether the warp has rows in this unit: its lanes of the products are not read otherwise.
@@ -977,7 +1041,7 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
     const bool whole = cur.i + n == cur.u.tiles && !cut_start;
     const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (first_unit ? 0 : 1);
     const uint32_t o_addr = lane_base + kColO + wg * D;
-    const float back = C::kWide ? 1.f : pow2i(unit_exp - 6);
+    const float back = C::kWide ? 1.f : pow2(unit_exp - kUnit);
     const bool none = m_used == -INFINITY && !(whole && l != 0.f);  // nothing but hidden keys (l: NaN where a score was)
     const float f = whole ? back / l : back;
     const int odd = C::kWide ? *reinterpret_cast<volatile int*>(&bars->odd) : 0;

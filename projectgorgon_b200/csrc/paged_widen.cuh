@@ -2,6 +2,7 @@
 #pragma once
 
 #include <cuda_fp16.h>
+#include <cuda_fp8.h>
 #include <stdint.h>
 
 #include "gorgon_b200.h"
@@ -42,6 +43,15 @@ __device__ __forceinline__ void widen_word(uint32_t w, uint32_t& lo, uint32_t& h
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"(static_cast<uint16_t>(w)));
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"(static_cast<uint16_t>(w >> 16)));
   }
+}
+
+// A stored byte's number.
+template <int ST>
+__device__ __forceinline__ float byte_value(uint8_t x) {
+  if constexpr (ST == GORGON_KV_INT8) return static_cast<float>(static_cast<int8_t>(x));
+  __nv_fp8_e4m3 f;
+  f.__x = x;
+  return static_cast<float>(f);
 }
 
 }  // namespace gorgon
