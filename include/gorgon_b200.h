@@ -508,7 +508,8 @@ GORGON_API int gorgon_paged_trim(const gorgon_paged_trim_params* p, void* stream
  * NaN: gorgon_paged_append writes such a row with a NaN scale).
  * Rows of one sequence may differ in size: beside 8-bit V rows of any size,
  * seen or hidden, the others keep their precision (terms below 2^-130 of the
- * largest V scale, and rows below 2^-100 beside larger ones, count as nothing).
+ * largest V scale, and rows below 2^-100 beside larger ones, count as nothing;
+ * values of a bf16 query below 2^-32 of its largest lose bits).
  * out = softmax(q k^T * scale) v over the visible rows (scale 0: 1 /
  * sqrt(head_dim)); lse (nullable, float, strides) the natural-log sum of
  * exponentials.  Rows of an unused slot, and rows with nothing to see (all

@@ -18,9 +18,8 @@
 // 8-bit rows are widened in registers to f16, exactly, whatever the type of
 // Q: f16 takes the fewest instructions per value.  The K scale is applied to
 // the score and the V scale to the weight, in fp32 (see VUnit).  bf16 queries enter as f16
-// times a power of two per row that puts the row's largest value near 2^8
-// (exact but for values below 2^-22 of it, which lose less than the fp32 sum
-// of the score does).  So that a thread widens whole 16-byte pieces, the head
+// times a power of two per row that puts the row's largest value at 2^15 or above, just
+// inside f16: exact, but for values below 2^-32 of it.  So that a thread widens whole 16-byte pieces, the head
 // dimension is taken in another order than the fragments': thread c of a quad
 // holds values 16 (c + 4 i) + 4 s .. + 3 for K step (i, s), Q in the same
 // order, and row r of output tile t is value D / 8 (r % 8) + 2 t + r / 8.
@@ -384,8 +383,8 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
           top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
           // (an infinity or a NaN stays one; a row below 2^-100 is small enough to enter as it is scaled for 2^-100)
           const int e = max(static_cast<int>(top >> 23) - 127, -100);
-          const float f = pow2(8 - e);
-          back = pow2(e - 8);
+          const float f = pow2(15 - e);
+          back = pow2(e - 15);
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll

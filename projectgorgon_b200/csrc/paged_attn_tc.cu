@@ -769,12 +769,12 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
 #pragma unroll
             for (int o = 1; o < kChunks; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
             const int e2 = max(static_cast<int>(top >> 23) - 127, -100);
-            const float f = pow2(8 - e2);
+            const float f = pow2(15 - e2);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               x[e] = pack16x2(__uint_as_float(x[e] << 16) * f, __uint_as_float(x[e] & 0xffff0000u) * f, false);
             qv[k] = make_uint4(x[0], x[1], x[2], x[3]);
-            if (chunk == 0) s_qs[wg * 128 + wq * 32 + rr] = pow2(e2 - 8);
+            if (chunk == 0) s_qs[wg * 128 + wq * 32 + rr] = pow2(e2 - 15);
           }
           *reinterpret_cast<uint4*>(stage_row(rr, chunk)) = qv[k];
         }

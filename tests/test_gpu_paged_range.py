@@ -160,3 +160,24 @@ def test_pieces_of_other_sizes(storage, n, Hq):
     p = Paged([L], 1, 128, 16, torch.bfloat16, storage, seed=n, scale_of=scale_of)
     check(p, [n], Hq)
     check(p, [n], Hq, window=5000, sinks=200)
+
+
+@pytest.mark.parametrize("backend", KERNELS)
+@pytest.mark.parametrize("storage", EIGHT)
+@pytest.mark.parametrize("n", [1, 40])
+def test_queries_with_one_large_channel(backend, storage, n):
+    """A channel 2^28 times the others, where K is 0: the others make the scores."""
+    p = sized([n + 200, n + 40], lambda L: slice(0, 0), storage, torch.bfloat16, 1.0)
+    p.k_pages.view(torch.uint8)[..., 5] = 0  # (zero bytes are 0 in both formats)
+    for k in p.k64:
+        k[..., 5] = 0
+    q = torch.randn(2, 8, n, 128, generator=torch.Generator().manual_seed(9)).bfloat16()
+    q[..., 5] = 2.0 ** 28
+    out, lse = G.paged_attention(q.cuda(), *p.args, backend=backend, return_lse=True, **p.held)
+    for b in range(2):
+        # (the channel adds exact zeros: it takes no part in what the scores lose)
+        small = q[b].clone()
+        small[..., 5] = 0
+        want, weight, slip, wl = attend(small, p.k64[b], p.v64[b], visible(p.lens[b], n), 128 ** -0.5)
+        assert bool(((out[b].cpu().double() - want).abs() <= tolerance(want, weight, slip, torch.bfloat16)).all())
+        assert bool(((lse[b].cpu().double() - wl).abs() <= 2 * slip[..., 0] + 64 * 2.0 ** -22 + wl.abs() * 2.0 ** -22).all())
