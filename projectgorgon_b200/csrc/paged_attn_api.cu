@@ -7,6 +7,12 @@
 namespace gorgon {
 namespace {
 
+// Nothing to write.  (Packed rows are, even where no sequence may bring any: they
+// are too many then.  Rows of no values have a log-sum-exp.)
+bool empty(const PagedAttn& a) {
+  return a.pool.batch == 0 || a.hq == 0 || (a.n == 0 && !(a.nr.cu && a.rows > 0)) || (a.pool.d == 0 && !a.lse);
+}
+
 int make_args(const gorgon_paged_attn_params* p, PagedAttn* a) {
   if (!p) return set_error(GORGON_ERR_INVALID, "gorgon_paged_attn: params is null");
   PagedAttn& x = *a;
@@ -27,8 +33,6 @@ int make_args(const gorgon_paged_attn_params* p, PagedAttn* a) {
     return set_error(GORGON_ERR_INVALID, "gorgon_paged_attn: bad count of packed rows");
   if (p->backend < GORGON_PAGED_AUTO || p->backend > GORGON_PAGED_TCGEN05)
     return set_error(GORGON_ERR_INVALID, "gorgon_paged_attn: unknown backend");
-  if (p->kv.batch * p->heads_q * p->n * p->kv.head_dim > 0 && (!p->q || !p->out || !p->kv.seq_lens))
-    return set_error(GORGON_ERR_INVALID, "gorgon_paged_attn: null q, out or seq_lens");
   const int64_t es = static_cast<int64_t>(dtype_bytes(p->kv.dtype));
   x.nr = NewRows{p->cu_q, static_cast<int>(p->n)};
   x.q = static_cast<const char*>(p->q);
@@ -50,10 +54,10 @@ int make_args(const gorgon_paged_attn_params* p, PagedAttn* a) {
   const float scale = p->scale != 0.f ? p->scale : (x.pool.d > 0 ? 1.f / std::sqrt(static_cast<float>(x.pool.d)) : 1.f);
   x.scale_log2 = scale * 1.4426950408889634f;
   x.wait_ns = wait_limit_ns();
+  if (!empty(x) && (!p->kv.seq_lens || (x.pool.d > 0 && (!p->out || (x.n > 0 && !p->q))) || (!p->kv.block_table && p->kv.table_cols > 0)))
+    return set_error(GORGON_ERR_INVALID, "gorgon_paged_attn: null q, out, seq_lens or block table");
   return GORGON_OK;
 }
-
-bool empty(const PagedAttn& a) { return static_cast<int64_t>(a.pool.batch) * a.hq * a.n * a.pool.d == 0; }
 
 enum class Kernel { kSimt, kMma, kTc, kNone };
 
@@ -66,6 +70,7 @@ bool short_list(const PagedAttn& a, int m) {
 }
 
 Kernel choose(const gorgon_paged_attn_params* p, const PagedAttn& a) {
+  if (a.n == 0 || a.pool.d == 0) return Kernel::kSimt;
   const bool mma = paged_mma_supported(a) && short_list(a, 8), tc = paged_tc_supported(a) && short_list(a, 128);
   switch (p->backend) {
     case GORGON_PAGED_SIMT: return Kernel::kSimt;

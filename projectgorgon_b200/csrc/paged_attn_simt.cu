@@ -41,8 +41,8 @@ __global__ void __launch_bounds__(kWarps * 32) paged_simt_kernel(const PagedAttn
   T* out = reinterpret_cast<T*>(a.out) + (a.nr.cu ? 0 : b * a.o_sb) + h * a.o_sh + row * a.o_sn;
   float* lse = a.lse ? a.lse + (a.nr.cu ? 0 : b * a.l_sb) + h * a.l_sh + row * a.l_sn : nullptr;
   const int D = a.pool.d;
-  if (!s.ok) {  // (it may bring more rows than the n that the grid covers)
-    for (int64_t k = 0; t + k < s.c; k += a.n) {
+  if (!s.ok) {  // (it may bring more rows than the grid covers)
+    for (int64_t k = 0; t + k < s.c; k += gridDim.x) {
       for (int d = threadIdx.x; d < D; d += blockDim.x) out[k * a.o_sn + d] = Cvt<T>::from_f(0.f);
       if (lse && threadIdx.x == 0) lse[k * a.l_sn] = -INFINITY;
     }
@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_simt_kernel(const PagedAttn
     x = warp_sum(x);
     float vsc = 1.f;
     if constexpr (ST != GORGON_KV_NATIVE) {
-      x *= a.pool.ks[page * a.pool.ks_sp + kvh * a.pool.ks_sh + r * a.pool.ks_ss];
+      if (D > 0) x *= a.pool.ks[page * a.pool.ks_sp + kvh * a.pool.ks_sh + r * a.pool.ks_ss];
       vsc = a.pool.vs[page * a.pool.vs_sp + kvh * a.pool.vs_sh + r * a.pool.vs_ss];
     }
     const float mn = fmaxf(m, x);
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_simt_kernel(const PagedAttn
 
 template <typename T>
 int launch_t(const PagedAttn& a, cudaStream_t st) {
-  const dim3 grid(static_cast<unsigned>(a.n), static_cast<unsigned>(a.hq), static_cast<unsigned>(a.pool.batch));
+  const dim3 grid(static_cast<unsigned>(std::max(a.n, 1)), static_cast<unsigned>(a.hq), static_cast<unsigned>(a.pool.batch));
   switch (a.pool.storage) {
     case GORGON_KV_NATIVE: paged_simt_kernel<T, GORGON_KV_NATIVE><<<grid, kWarps * 32, 0, st>>>(a); break;
     case GORGON_KV_INT8: paged_simt_kernel<T, GORGON_KV_INT8><<<grid, kWarps * 32, 0, st>>>(a); break;

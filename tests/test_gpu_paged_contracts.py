@@ -1,0 +1,56 @@
+"""What the paged operators' documentation promises at its edges."""
+from __future__ import annotations
+
+import math
+import random
+
+import pytest
+import torch
+
+import projectgorgon_b200 as G
+from paged_reference import Paged, attend, tolerance, visible
+from projectgorgon_b200 import _abi
+
+pytestmark = pytest.mark.gpu
+
+STORES = ["native", "int8", "fp8"]
+
+
+@pytest.fixture(autouse=True)
+def no_device_error():
+    G.device_error(clear=True)
+    yield
+    assert G.device_error(clear=True) == 0
+
+
+@pytest.mark.parametrize("backend", ["auto", "mma", "tcgen05", "simt"])
+@pytest.mark.parametrize("tree", [False, True])
+def test_rows_where_max_q_is_zero(backend, tree):
+    """max_q = 0 is a bound that every sequence with rows passes: zeros, and reported, as for any other."""
+    p = Paged([50, 0, 70], 2, 128, 16, torch.bfloat16, seed=1)
+    q = torch.randn(9, 8, 128, device="cuda").bfloat16()
+    cu = torch.tensor([0, 3, 5, 7], dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, 3.0)
+    parents = torch.tensor([-1, 0, 1]) if tree else None
+    _, lse = G.paged_attention(q, *p.args, cu_q=cu, max_q=0, parents=parents, out=out, return_lse=True, backend=backend)
+    assert G.device_error(clear=True) == _abi.ERR_BAD_SEQLEN
+    assert bool((out[:7] == 0).all()) and bool((lse[:7] == -math.inf).all()) and bool((out[7:] == 3.0).all())
+    # nothing but unused slots: zeros, and nothing to report
+    out.fill_(3.0)
+    _, lse = G.paged_attention(q, p.k_pages, p.v_pages, p.table_d, torch.zeros_like(p.lens_d), cu_q=cu, max_q=0, parents=parents,
+                               out=out, return_lse=True, backend=backend)
+    assert bool((out[:7] == 0).all()) and bool((lse[:7] == -math.inf).all()) and bool((out[7:] == 3.0).all())
+
+
+@pytest.mark.parametrize("storage", STORES)
+@pytest.mark.parametrize("backend", ["auto", "simt"])
+def test_log_sum_exp_of_rows_of_no_values(storage, backend):
+    """head_dim 0: every score is 0, so the log-sum-exp is the log of how many keys a row sees."""
+    p = Paged([5, 40], 2, 8, 16, torch.bfloat16, storage, seed=1)
+    q = torch.empty(2, 4, 3, 0, device="cuda", dtype=torch.bfloat16)
+    out, lse = G.paged_attention(q, p.k_pages[..., :0], p.v_pages[..., :0], p.table_d, p.lens_d, window=20, return_lse=True,
+                                 backend=backend, **p.held)
+    assert out.shape == q.shape
+    for b, L in enumerate(p.lens):
+        want = visible(L, 3, window=20).sum(-1).double().log()
+        assert bool(((lse[b].cpu().double() - want).abs() <= want * 4 * 2.0 ** -23 + 2.0 ** -22).all())
