@@ -443,8 +443,9 @@ typedef struct {
  * by strides, or with cu_q (int32 [batch + 1]) packed rows: sequence b's are
  * cu_q[b] .. cu_q[b + 1] - 1 of `rows` packed rows (the batch stride is
  * ignored).  Row i of a sequence with c new rows goes to position
- * seq_lens[b] - c + i.  Two sequences must not write the same row of a page:
- * its contents are then undefined (nothing faults). */
+ * seq_lens[b] - c + i.  Two sequences, or two kv heads by a stride of 0,
+ * must not write the same row of a page: its contents are then undefined
+ * (nothing faults). */
 typedef struct {
   gorgon_paged_kv kv;
   const void* k; int64_t k_stride_b, k_stride_h, k_stride_n;
@@ -479,6 +480,10 @@ GORGON_API int gorgon_paged_read(const gorgon_paged_read_params* p, void* stream
  * read before any is written.  A layer's pages lie k_stride_l / v_stride_l
  * elements (scales ks_stride_l / vs_stride_l) after the one before; all
  * layers share the block table.  max_len <= 256; kv.seq_lens is not used.
+ * No row that one sequence of a call writes may be one that another reads or
+ * writes, so a sequence must not be named twice (what its rows hold is then
+ * undefined; nothing faults); strides of 0 between layers, pages, heads or rows
+ * are refused.
  * A bad index sets bit 1 of the device error word and leaves the sequence as
  * it is, as in gorgon_kv_trim; so does a page outside the pool, with bit 6. */
 typedef struct {

@@ -729,6 +729,16 @@ extern "C" int gorgon_paged_trim(const gorgon_paged_trim_params* p, void* stream
   if (p->layers > 32767) return set_error(GORGON_ERR_UNSUPPORTED, "gorgon_paged_trim: layers > 32767");
   if (p->layers == 0 || a.pool.batch == 0 || a.pool.d == 0 || p->max_len == 0) return GORGON_OK;
   if (!p->src_idx || !p->lens || !a.pool.table) return set_error(GORGON_ERR_INVALID, "gorgon_paged_trim: null pointer");
+  // Rows that are one in memory would be read and written by several warps at once.
+  auto repeats = [&](int64_t layer, int64_t page, int64_t head, int64_t row) {
+    return (p->layers > 1 && layer == 0) || (p->kv.num_pages > 1 && page == 0) || (p->kv.heads_kv > 1 && head == 0) ||
+           (p->kv.page_size > 1 && row == 0);
+  };
+  const gorgon_paged_kv& kv = p->kv;
+  if (repeats(p->k_stride_l, kv.k_stride_p, kv.k_stride_h, kv.k_stride_s) || repeats(p->v_stride_l, kv.v_stride_p, kv.v_stride_h, kv.v_stride_s) ||
+      (kv.storage != GORGON_KV_NATIVE && (repeats(p->ks_stride_l, kv.ks_stride_p, kv.ks_stride_h, kv.ks_stride_s) ||
+                                          repeats(p->vs_stride_l, kv.vs_stride_p, kv.vs_stride_h, kv.vs_stride_s))))
+    return set_error(GORGON_ERR_UNSUPPORTED, "gorgon_paged_trim: layers, pages, kv heads or rows repeated by a stride of 0");
   const int64_t es = storage_bytes(p->kv.storage, p->kv.dtype);
   a.k_sl = p->k_stride_l * es;
   a.v_sl = p->v_stride_l * es;

@@ -37,8 +37,8 @@ def paged_cache_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, 
     ``paged_attention``'s.  8-bit pages get, per row and head, the bytes
     ``round(x * inv)`` and the scale ``1 / inv``, with ``inv = largest / amax`` cut to
     12 significant bits (``largest`` 127 for int8, 448 for e4m3); a row with an
-    infinity or a NaN reads back as NaN.  Two sequences of one call must not
-    share the page row that they write."""
+    infinity or a NaN reads back as NaN.  Two sequences of one call, or
+    two kv heads (by a stride of 0), must not share the page row that they write."""
     dev = device_index("k, v, pages, block_table and seq_lens", k, v, k_pages, v_pages, block_table, seq_lens, k_scale,
                        v_scale, cu_q)
     dtype = compute_dtype(k.dtype, "k")
@@ -138,7 +138,9 @@ def paged_cache_trim(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: 
     ``GorgonKVCache.trim``'s arguments, over ``[layers, pages, Hkv, page_size, D]``
     (or one layer's ``[pages, Hkv, page_size, D]``); ``dst_start`` ``[B]``, an int, or
     None for 0.  At most 256 rows per sequence.  A bad index sets the device
-    error bits and leaves its sequence as it is."""
+    error bits and leaves its sequence as it is.  A call must not name a sequence
+    twice, nor move rows into pages that another of its sequences reads; pages
+    expanded over layers or kv heads (strides of 0) are refused."""
     dev = device_index("pages, block_table, src_idx and lens", k_pages, v_pages, block_table, src_idx, lens, k_scale,
                        v_scale, dst_start if isinstance(dst_start, torch.Tensor) else None)
     lead = 1 if k_pages.dim() == 5 else 0

@@ -54,3 +54,20 @@ def test_log_sum_exp_of_rows_of_no_values(storage, backend):
     for b, L in enumerate(p.lens):
         want = visible(L, 3, window=20).sum(-1).double().log()
         assert bool(((lse[b].cpu().double() - want).abs() <= want * 4 * 2.0 ** -23 + 2.0 ** -22).all())
+
+
+@pytest.mark.parametrize("storage", STORES)
+def test_trim_refuses_expanded_pages(storage):
+    """Kv heads or layers that are one in memory; a single one may have any stride."""
+    p = Paged([40], 1, 64, 16, torch.bfloat16, storage, seed=1, poison=False)
+    idx, ln = torch.tensor([[3, 1]], device="cuda"), torch.tensor([2], device="cuda")
+    before = [x.clone() for x in (p.k_pages, p.v_pages)]
+    for wide in (lambda t: None if t is None else t.expand(-1, 4, *t.shape[2:]), lambda t: None if t is None else t.expand(2, *t.shape)):
+        with pytest.raises(RuntimeError, match="stride of 0"):
+            G.paged_cache_trim(wide(p.k_pages), wide(p.v_pages), p.table_d, idx, ln, 0, k_scale=wide(p.k_scale), v_scale=wide(p.v_scale))
+    as_bytes = lambda t: t.view(torch.uint8)  # noqa: E731
+    assert all(torch.equal(as_bytes(a), as_bytes(b)) for a, b in zip(before, (p.k_pages, p.v_pages)))
+    one = lambda t: None if t is None else t.as_strided((1,) + t.shape, (0,) + t.stride())  # noqa: E731
+    G.paged_cache_trim(one(p.k_pages), one(p.v_pages), p.table_d, idx, ln, 0, k_scale=one(p.k_scale), v_scale=one(p.v_scale))
+    first = int(p.table[0, 0])
+    assert torch.equal(as_bytes(p.k_pages)[first, :, :2], as_bytes(before[0])[first][:, [3, 1]])
