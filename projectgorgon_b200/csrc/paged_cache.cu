@@ -511,9 +511,14 @@ __global__ void __launch_bounds__(kTrimWarps * 32) paged_trim_warp_kernel(const 
   }
 }
 
-// Any row size: a CTA per (layer, sequence, head) and K or V, through shared memory.
+// Any row size: a CTA per (layer, sequence, head) and K or V, through shared memory,
+// `width` bytes of every row at a time (a column of the rows depends on that
+// column alone, so rows may overlap all the same).  The stage is one that every
+// launch may have: a larger limit is an attribute of the kernel, which two host
+// threads would set for each other.
 constexpr int kTrimThreads = 128;
-__global__ void __launch_bounds__(kTrimThreads) paged_trim_kernel(const TrimArgs a) {
+constexpr int kTrimStage = 46 * 1024;
+__global__ void __launch_bounds__(kTrimThreads) paged_trim_kernel(const TrimArgs a, int width) {
   extern __shared__ uint8_t stage[];
   __shared__ float s_scale[256];
   __shared__ int s_ok;
@@ -544,21 +549,25 @@ __global__ void __launch_bounds__(kTrimThreads) paged_trim_kernel(const TrimArgs
     page = tb[col];
   };
   int page, row;
-  for (int e = threadIdx.x; e < len * a.row_bytes; e += kTrimThreads) {
-    const int r = e / a.row_bytes, c = e - r * a.row_bytes;
-    at(a.idx[b * a.idx_sb + r], page, row);
-    stage[e] = static_cast<uint8_t>(base[page * sp + row * ss + c]);
-  }
   if (scaled)
     for (int r = threadIdx.x; r < len; r += kTrimThreads) {
       at(a.idx[b * a.idx_sb + r], page, row);
       s_scale[r] = sbase[page * ssp + row * sss];
     }
-  __syncthreads();
-  for (int e = threadIdx.x; e < len * a.row_bytes; e += kTrimThreads) {
-    const int r = e / a.row_bytes, c = e - r * a.row_bytes;
-    at(d0 + r, page, row);
-    base[page * sp + row * ss + c] = static_cast<char>(stage[e]);
+  for (int c0 = 0; c0 < a.row_bytes; c0 += width) {
+    const int w = min(width, a.row_bytes - c0);
+    for (int e = threadIdx.x; e < len * w; e += kTrimThreads) {
+      const int r = e / w, c = c0 + e - r * w;
+      at(a.idx[b * a.idx_sb + r], page, row);
+      stage[e] = static_cast<uint8_t>(base[page * sp + row * ss + c]);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < len * w; e += kTrimThreads) {
+      const int r = e / w, c = c0 + e - r * w;
+      at(d0 + r, page, row);
+      base[page * sp + row * ss + c] = static_cast<char>(stage[e]);
+    }
+    __syncthreads();
   }
   if (scaled)
     for (int r = threadIdx.x; r < len; r += kTrimThreads) {
@@ -763,15 +772,10 @@ extern "C" int gorgon_paged_trim(const gorgon_paged_trim_params* p, void* stream
     else paged_trim_warp_kernel<8><<<grid, kTrimWarps * 32, 0, st>>>(a);
     return check_cuda(cudaGetLastError(), "gorgon_paged_trim launch");
   }
-  const size_t smem = static_cast<size_t>(p->max_len) * a.row_bytes;
-  if (smem > 200 * 1024) return set_error(GORGON_ERR_UNSUPPORTED, "gorgon_paged_trim: max_len * row bytes > 200 KiB");
-  if (smem > 46 * 1024) {
-    rc = check_cuda(cudaFuncSetAttribute(paged_trim_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(smem)), "gorgon_paged_trim smem attribute");
-    if (rc) return rc;
-  }
+  const int width = static_cast<int>(std::min<int64_t>(a.row_bytes, kTrimStage / p->max_len));  // (at most 256 rows)
+  const size_t smem = static_cast<size_t>(p->max_len) * width;
   const dim3 grid(static_cast<unsigned>(a.pool.hkv), static_cast<unsigned>(a.pool.batch),
                   2u * static_cast<unsigned>(p->layers));
-  paged_trim_kernel<<<grid, kTrimThreads, smem, st>>>(a);
+  paged_trim_kernel<<<grid, kTrimThreads, smem, st>>>(a, width);
   return check_cuda(cudaGetLastError(), "gorgon_paged_trim launch");
 }

@@ -2,13 +2,13 @@
 from __future__ import annotations
 
 import math
-import random
+import threading
 
 import pytest
 import torch
 
 import projectgorgon_b200 as G
-from paged_reference import Paged, attend, tolerance, visible
+from paged_reference import Paged, visible
 from projectgorgon_b200 import _abi
 
 pytestmark = pytest.mark.gpu
@@ -71,3 +71,56 @@ def test_trim_refuses_expanded_pages(storage):
     G.paged_cache_trim(one(p.k_pages), one(p.v_pages), p.table_d, idx, ln, 0, k_scale=one(p.k_scale), v_scale=one(p.v_scale))
     first = int(p.table[0, 0])
     assert torch.equal(as_bytes(p.k_pages)[first, :, :2], as_bytes(before[0])[first][:, [3, 1]])
+
+
+@pytest.mark.parametrize("dtype,D,storage,layout,m", [
+    (torch.float32, 256, "native", "HSD", 256), (torch.float32, 256, "native", "pad", 201), (torch.bfloat16, 256, "native", "HSD", 256),
+    (torch.float32, 33, "native", "HSD", 256), (torch.bfloat16, 250, "fp8", "HSD", 256), (torch.float16, 128, "int8", "HSD", 255)])
+def test_trim_of_as_many_rows_as_documented(dtype, D, storage, layout, m):
+    """256 rows of any size, overlapping: a reversal and a shift."""
+    H, ps, L = 2, 16, 600
+    p = Paged([L, L], H, D, ps, dtype, storage, seed=D, layout=layout, poison=False)
+    src = torch.stack([torch.arange(m - 1, -1, -1), torch.arange(m) + 7]).to(torch.int32)
+    dst = torch.tensor([0, 3], dtype=torch.int32)
+    ln = torch.tensor([m, m - 1], dtype=torch.int32)
+    as_bytes = lambda t: t.contiguous().view(torch.uint8) if t.element_size() == 1 else t.contiguous()  # noqa: E731
+    want = [as_bytes(t).clone() if t is not None else None for t in (p.k_pages, p.v_pages, p.k_scale, p.v_scale)]
+    for t in want:
+        if t is not None:
+            old = t.clone()
+            for b in range(2):
+                for r in range(int(ln[b])):
+                    i, o = int(src[b, r]), int(dst[b]) + r
+                    t[int(p.table[b, o // ps]), :, o % ps] = old[int(p.table[b, i // ps]), :, i % ps]
+    G.paged_cache_trim(p.k_pages, p.v_pages, p.table_d, src.cuda(), ln.cuda(), dst.cuda(), **p.held)
+    for t, w in zip((p.k_pages, p.v_pages, p.k_scale, p.v_scale), want):
+        if w is not None:
+            assert torch.equal(as_bytes(t), w)
+
+
+def test_trims_of_several_host_threads():
+    """Trims of different widths, launched by four threads at once, each on its own pages."""
+    errors = []
+
+    def work(m):
+        try:
+            st = torch.cuda.Stream()
+            with torch.cuda.stream(st):
+                p = Paged([300], 2, 128, 16, torch.float32, seed=m, poison=False)
+                want = p.k_pages.clone()
+                first, second = int(p.table[0, 0]), int(p.table[0, m // 16])
+                want[first, :, 0] = p.k_pages[second, :, m % 16]
+                idx = torch.full((1, m), m, dtype=torch.int32, device="cuda")
+                ln = torch.ones(1, dtype=torch.int32, device="cuda")
+                for _ in range(300):
+                    G.paged_cache_trim(p.k_pages, p.v_pages, p.table_d, idx, ln)
+                st.synchronize()
+                assert torch.equal(p.k_pages, want)
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(m,)) for m in (100, 256, 130, 200)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
