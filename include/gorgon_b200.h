@@ -419,6 +419,9 @@ GORGON_API int gorgon_head_candidate_tree(const gorgon_head_candidate_params* p,
  * columns, sets bit 6 of the device error word; the row is skipped, never
  * dereferenced.  seq_lens[b] below the sequence's new rows sets bit 3, and
  * the sequence is treated as an unused slot.
+ * Cumulative counts (cu_q, cu_rows) that fall or begin below 0 set bit 3 too:
+ * the attention leaves out the sequences that they give no count of rows, append
+ * and read the rows that a binary search does not find inside a sequence.
  * ---------------------------------------------------------------------- */
 typedef enum {
   GORGON_KV_NATIVE = 0,

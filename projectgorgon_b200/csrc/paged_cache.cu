@@ -154,6 +154,15 @@ __device__ __forceinline__ const int32_t* cached_cu(const int32_t* cu, int batch
   return buf;
 }
 
+// Cumulative counts that fall, or begin below 0, are reported (by one CTA): rows
+// are found by a search among them, so some of a call's rows may be left out.
+__device__ __forceinline__ void report_counts(const int32_t* cu, int batch, uint32_t* err) {
+  if (!cu || blockIdx.x != 0) return;
+  bool bad = threadIdx.x == 0 && cu[0] < 0;
+  for (int i = threadIdx.x; i < batch; i += blockDim.x) bad |= cu[i] > cu[i + 1];
+  if (bad) raise_device_error(err, kErrBadSeqlen);
+}
+
 struct Place {
   int b, i;      // sequence, number among its new rows
   int page, row;
@@ -198,6 +207,7 @@ template <typename T, int ST, int LPR, int HP>
 __global__ void __launch_bounds__(kThreads) paged_append_vec_kernel(const AppendArgs a) {
   __shared__ int32_t s_cu[kCuCached + 1];
   const int32_t* cu = cached_cu(a.nr.cu, a.pool.batch, s_cu);
+  report_counts(cu, a.pool.batch, a.pool.err);
   const int sub = threadIdx.x % LPR;
   const int64_t item = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / LPR;
   const int per_row = (a.pool.hkv + HP - 1) / HP;
@@ -261,6 +271,7 @@ template <typename T, int ST>
 __global__ void __launch_bounds__(kThreads) paged_append_kernel(const AppendArgs a) {
   __shared__ int32_t s_cu[kCuCached + 1];
   const int32_t* cu = cached_cu(a.nr.cu, a.pool.batch, s_cu);
+  report_counts(cu, a.pool.batch, a.pool.err);
   const int lane = threadIdx.x & 31;
   const int64_t item = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / 32;
   if (item >= a.items) return;
@@ -326,6 +337,7 @@ template <typename T, int ST, int LPR, int HP>
 __global__ void __launch_bounds__(kThreads) paged_read_vec_kernel(const ReadArgs a) {
   __shared__ int32_t s_cu[kCuCached + 1];
   const int32_t* cu = cached_cu(a.cu, a.pool.batch, s_cu);
+  report_counts(cu, a.pool.batch, a.pool.err);
   const int sub = threadIdx.x % LPR;
   const int64_t item = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / LPR;
   if (item >= a.items) return;
@@ -377,6 +389,7 @@ template <typename T, int ST>
 __global__ void __launch_bounds__(kThreads) paged_read_kernel(const ReadArgs a) {
   __shared__ int32_t s_cu[kCuCached + 1];
   const int32_t* cu = cached_cu(a.cu, a.pool.batch, s_cu);
+  report_counts(cu, a.pool.batch, a.pool.err);
   const int lane = threadIdx.x & 31;
   const int64_t item = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / 32;
   if (item >= a.items) return;

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import projectgorgon_b200 as G
-from paged_reference import Paged, visible
+from paged_reference import Paged, quantise, visible
 from projectgorgon_b200 import _abi
 
 pytestmark = pytest.mark.gpu
@@ -124,3 +124,73 @@ def test_trims_of_several_host_threads():
     for t in threads:
         t.join()
     assert not errors, errors
+
+
+def found(cu, batch, r):
+    """The (sequence, number in it) that a search for row r among the counts ends at, or None."""
+    if r < cu[0] or r >= cu[batch]:
+        return None
+    lo, hi = 0, batch - 1
+    while lo < hi:
+        mid = (lo + hi + 1) // 2
+        if cu[mid] <= r:
+            lo = mid
+        else:
+            hi = mid - 1
+    if cu[lo] < 0 or not 0 <= r - cu[lo] < cu[lo + 1] - cu[lo]:
+        return None
+    return lo, r - cu[lo]
+
+
+COUNTS = [[0, -3, 4, 6], [2, 5, 3, 6], [0, 5, 2, 6], [0, 2 ** 31 - 1, 3, 6], [-2 ** 31, 2, 3, 6], [0, 6, 0, 6], [0, 2, 4, 1], [0, 2, 0, 0],
+          [-1, 2, 3, 6], [0, 0, 0, -1], [1, 1, 0, 6]]
+IN_ORDER = [[0, 2, 4, 6], [1, 1, 3, 4], [0, 0, 6, 6], [2, 5, 5, 5], [6, 6, 6, 6]]
+
+
+@pytest.mark.parametrize("cu", COUNTS + IN_ORDER)
+@pytest.mark.parametrize("storage", ["native", "int8"])
+@pytest.mark.parametrize("D", [128, 40])
+@pytest.mark.parametrize("batch", [3, 1500])
+def test_counts_are_checked_row_by_row(cu, storage, D, batch):
+    """Append and read: every row lands where a search for it says and nowhere else; counts out of order are reported."""
+    lens = [60, 50, 70]
+    p = Paged(lens, 2, D, 16, torch.float16, storage, seed=1, poison=False)
+    rows = torch.randn(2, 6, 2, D, device="cuda").half()
+    many = cu + [cu[-1]] * (batch - 3)  # (more sequences than are kept in shared memory, all unused)
+    counts = torch.tensor(many, dtype=torch.int32, device="cuda")
+    pad = lambda t: torch.cat([t, t.new_zeros((batch - 3,) + t.shape[1:])])  # noqa: E731
+    table, seq_lens = pad(p.table_d), pad(p.lens_d)
+    word = _abi.ERR_BAD_SEQLEN if cu in COUNTS else 0
+    where = [found(many, batch, r) for r in range(6)]
+    where = [w if w is None or w[0] < 3 else None for w in where]
+    # read first, from the pages as they are
+    out = torch.full((2, 6, 2, D), 4.0, device="cuda", dtype=torch.float16)
+    every = G.paged_cache_read(p.k_pages, p.v_pages, p.table_d, torch.tensor([0, 60, 110, 180], dtype=torch.int32, device="cuda"), 180,
+                               dtype=torch.float16, **p.held)
+    G.paged_cache_read(p.k_pages, p.v_pages, table, counts, 6, out=(out[0], out[1]), **p.held)
+    assert G.device_error(clear=True) == word
+    first = [0, 60, 110]
+    for x, whole in zip(out, every):
+        for r, w in enumerate(where):
+            want = torch.full_like(x[r], 4.0) if w is None else whole[first[w[0]] + w[1]]
+            assert torch.equal(x[r], want), (r, w)
+    # append: what the rows say, and every other byte as it was
+    want = [t.clone() if t is not None else None for t in (p.k_pages, p.v_pages, p.k_scale, p.v_scale)]
+    for r, w in enumerate(where):
+        if w is not None:
+            b, i = w
+            pos = lens[b] - (cu[b + 1] - cu[b]) + i
+            if pos < 0 or lens[b] < cu[b + 1] - cu[b]:
+                continue
+            pg, at = int(p.table[b, pos // 16]), pos % 16
+            for k in range(2):
+                if storage == "native":
+                    want[k][pg, :, at] = rows[k, r]
+                else:
+                    q, s = quantise(rows[k, r].cpu(), storage)
+                    want[k][pg, :, at] = q.to(torch.int8).cuda()
+                    want[2 + k][pg, :, at] = s.cuda()
+    G.paged_cache_append(rows[0], rows[1], p.k_pages, p.v_pages, table, seq_lens, cu_q=counts, **p.held)
+    assert G.device_error(clear=True) == word
+    for t, w in zip((p.k_pages, p.v_pages, p.k_scale, p.v_scale), want):
+        assert t is None or torch.equal(t, w)
