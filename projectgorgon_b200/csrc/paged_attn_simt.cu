@@ -56,7 +56,8 @@ __global__ void __launch_bounds__(kWarps * 32) paged_simt_kernel(const PagedAttn
     __syncthreads();
     pos = s.P + s_depth;
   }
-  const int lo = a.window ? max(0, pos - a.window + 1) : 0;
+  int lo = a.window ? max(0, pos - a.window + 1) : 0;
+  if (a.parents) lo = min(lo, s.P);  // tree rows go by their bits: an ancestor may stand anywhere among them
   const int s_end = min(a.sinks, lo);
   const int hi = a.parents ? s.L : pos + 1;
   const int kvh = h / a.group;

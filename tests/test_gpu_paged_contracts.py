@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import math
+import random
 import threading
 
 import pytest
@@ -10,6 +11,8 @@ import torch
 import projectgorgon_b200 as G
 from paged_reference import Paged, quantise, visible
 from projectgorgon_b200 import _abi
+from projectgorgon_b200.trees import random_tree
+from test_gpu_paged_attention import check
 
 pytestmark = pytest.mark.gpu
 
@@ -194,3 +197,32 @@ def test_counts_are_checked_row_by_row(cu, storage, D, batch):
     assert G.device_error(clear=True) == word
     for t, w in zip((p.k_pages, p.v_pages, p.k_scale, p.v_scale), want):
         assert t is None or torch.equal(t, w)
+
+
+@pytest.mark.parametrize("backend", ["mma", "tcgen05", "simt"])
+@pytest.mark.parametrize("n,window,sinks,P", [(2, 1, 0, 20), (31, 4, 2, 50), (64, 3, 0, 0), (64, 9, 30, 5), (100, 1, 0, 64), (40, 200, 0, 400)])
+def test_trees_in_any_order(backend, n, window, sinks, P):
+    """Parents may stand behind their children."""
+    rng = random.Random(n + window)
+    trees = []
+    for _ in range(2):
+        tree, at = random_tree(n, rng, 12), list(range(n))
+        rng.shuffle(at)
+        moved = [-1] * n
+        for i, up in enumerate(tree):
+            moved[at[i]] = -1 if up < 0 else at[up]
+        trees.append(moved)
+    trees[0][:2] = [1, -1]  # (whatever hangs below them stays a tree: they are one root and its child)
+    trees[0] = [up if i < 2 or up != i else -1 for i, up in enumerate(trees[0])]
+    p = Paged([n + P, n + 2 * P + 1], 2, 128, 16, torch.float16, seed=n)
+    for depth in (None, 2):
+        check(p, [n] * 2, 6, parents=trees, max_depth=depth, window=window, sinks=sinks, backend=backend)
+        check(p, [n] * 2, 6, parents=trees, max_depth=depth, backend=backend)
+
+
+@pytest.mark.parametrize("n,window", [(9, 2), (37, 5)])
+def test_float32_trees_in_any_order(n, window):
+    """The same in a type that the CUDA cores alone take."""
+    parents = [i + 1 for i in range(n - 1)] + [-1]  # a chain from the last row to the first
+    p = Paged([n + 30], 2, 64, 16, torch.float32, seed=n)
+    check(p, [n], 4, parents=parents, window=window, sinks=1)
