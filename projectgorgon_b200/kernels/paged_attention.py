@@ -20,6 +20,7 @@ from .._util import parents_tensor
 _ATTN = packer("qqq" + "Pqqq" * 3 + "PPqiqqfi")
 _BACKENDS = {"auto": _abi.PAGED_AUTO, "simt": _abi.PAGED_SIMT, "mma": _abi.PAGED_MMA,
              "tcgen05": _abi.PAGED_TCGEN05}
+_MANY = 2 ** 31 - 1  # more than any sequence has: options above it mean the same
 
 
 def _workspace_size_on(dev: int, params: bytes) -> int:
@@ -61,6 +62,7 @@ def paged_attention(
                  ``block_table[b, p // page_size]``; unused entries may hold anything
     seq_lens     int ``[B]``: rows of each sequence, its new ones last; 0 marks an
                  unused slot, whose output rows are 0 (log-sum-exp ``-inf``)
+    Integer tensors are int32, or int64 with values that fit 32 bits.
 
     Query head ``h`` reads kv head ``h // (Hq // Hkv)``.  A new row sees the
     cached rows and the new rows up to itself; with ``parents`` (``[n]`` or
@@ -150,7 +152,8 @@ def paged_attention(
         raise RuntimeError(f"sinks must not be negative, got {sinks}")
     params = _ATTN.pack(*pool, hq, n, 0 if cu is None else total, q.data_ptr(), q_sb, q_sh, q_sn, out.data_ptr(), o_sb, o_sh, o_sn,
                         l_ptr, l_sb, l_sh, l_sn, 0 if cu is None else cu.data_ptr(), p_ptr, p_sb,
-                        -1 if max_depth is None else int(max_depth), 0 if window is None else int(window), int(sinks),
+                        -1 if max_depth is None else min(int(max_depth), _MANY), 0 if window is None else min(int(window), _MANY),
+                        min(int(sinks), _MANY),
                         0.0 if scale is None else float(scale), be)
     lib = _abi.lib()
     nbytes = lib.gorgon_paged_attn_workspace_size(params) if dev == torch._C._cuda_getDevice() else \

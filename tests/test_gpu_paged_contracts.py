@@ -226,3 +226,13 @@ def test_float32_trees_in_any_order(n, window):
     parents = [i + 1 for i in range(n - 1)] + [-1]  # a chain from the last row to the first
     p = Paged([n + 30], 2, 64, 16, torch.float32, seed=n)
     check(p, [n], 4, parents=parents, window=window, sinks=1)
+
+
+@pytest.mark.parametrize("backend", ["mma", "tcgen05", "simt"])
+@pytest.mark.parametrize("many", [2 ** 30, 2 ** 31 - 1, 2 ** 31, 2 ** 63 - 1, 10 ** 30])
+def test_options_larger_than_any_sequence(backend, many):
+    p = Paged([40, 90], 2, 128, 16, torch.bfloat16, seed=1)
+    q = torch.randn(2, 8, 3, 128, device="cuda").bfloat16()
+    want = G.paged_attention(q, *p.args, parents=[-1, 0, 1], backend=backend)
+    got = G.paged_attention(q, *p.args, parents=[-1, 0, 1], max_depth=many, window=many, sinks=many, backend=backend)
+    assert torch.equal(got, want)
