@@ -17,7 +17,7 @@
 // warps 4 to 7 widen their 32 rows from there to f16, exactly (paged_widen.cuh),
 // so that the products see the stored numbers and the scales are applied in
 // fp32: K's to the scores, V's to the weights (see VUnit; rows outside its span
-// are added after the tile's product, add_far).  Pages of other sizes are
+// are added before the tile's product, add_far).  Pages of other sizes are
 // gathered row by row by warps 4 to 7 with 16-byte cp.async copies (which took
 // 1700 cycles a tile, most of them waiting for issue slots, so TMA is used where
 // it can be).  V rows that no row of the unit sees are made zeros.
@@ -618,10 +618,12 @@ __device__ void issue_outputs(const PagedAttn& a, TileCursor cur, int end, uint8
         }
         if (mt >= live) continue;
         tc_fence_after();
+        // A unit's output begins with its first product, or with what the softmax put there (add_far).
+        const bool begun = t > 0 || (!C::kWide && (reinterpret_cast<const uint32_t*>(smem + C::kOffMeta + vr.stage * C::kMetaBytes)[3] & kFar));
 #pragma unroll
         for (int ks = 0; ks < kTile / 16; ++ks)
           umma_f16_ts(tmem + kColO + mt * C::D, tmem + kColS + (buf * C::MT + mt) * kTile + ks * 8,
-                      v0 + static_cast<uint64_t>(vr.stage * (C::kTileBytes >> 4) + ks * (2048 >> 4)), idesc, (ks > 0 || t > 0) ? 1u : 0u);
+                      v0 + static_cast<uint64_t>(vr.stage * (C::kTileBytes >> 4) + ks * (2048 >> 4)), idesc, (ks > 0 || begun) ? 1u : 0u);
       }
       if (!ok) break;
       umma_commit(&bars->p_free[buf]);
@@ -656,41 +658,49 @@ __device__ __forceinline__ uint64_t row_word(const PagedAttn& a, const TileCurso
   return w;
 }
 
-// Adds the columns of a tile whose rows lie outside the unit's span (`far`) to
-// the output rows of a warp, key by key from the pages, once the tile's product is
-// complete (the next one waits for this warp's next weights).  x: a row's scores
-// less its running max.  Called rarely: out of the loop's registers.
-template <int ST, int D>
-__device__ __noinline__ void add_far(const PagedAttn& a, const TileCursor& cur, int j0, uint64_t far, const float* x, uint32_t o_addr,
-                                     int unit_exp) {
-  const float in_unit = pow2(kUnit - unit_exp);
+// The rare correction of a warp's output rows before a tile's product: they are
+// multiplied by alpha and regrade (or begin at 0, `fresh`), and the tile's columns
+// whose rows lie outside the unit's span (`far`) are added, key by key from the V
+// tile `v`.  x: a row's scores less its running max; `factor`: V's scales in the unit.
+// Out of the loop's registers.
+template <typename C>
+__device__ __noinline__ void add_far(uint32_t o_addr, bool fresh, float alpha, float regrade, uint64_t far, const float* x,
+                                     const uint8_t* v, const float* factor) {
 #pragma unroll 1
-  for (int c0 = 0; c0 < D; c0 += 32) {
-    uint32_t ov[32];
-    tmem_ld32(o_addr + c0, ov);
-    tmem_wait_ld();
+  for (int c0 = 0; c0 < C::D; c0 += 32) {
+    float o[32];
+    if (fresh) {
+#pragma unroll
+      for (int k = 0; k < 32; ++k) o[k] = 0.f;
+    } else {
+      uint32_t ov[32];
+      tmem_ld32(o_addr + c0, ov);
+      tmem_wait_ld();
+#pragma unroll
+      for (int k = 0; k < 32; ++k) o[k] = __uint_as_float(ov[k]) * alpha * regrade;
+    }
+    const uint8_t* blk = v + (c0 >> 6) * C::kBlock;
 #pragma unroll 1
     for (uint64_t rest = far; rest; rest &= rest - 1) {
       const int c = __ffsll(static_cast<long long>(rest)) - 1;
       const float p = ex2_approx(x[c]);
       if (!__any_sync(0xffffffffu, p != 0.f)) continue;  // (rows that were not fetched, too)
-      int col, prow;
-      a.pool.split(j0 + c, col, prow);
-      const int page = a.pool.page(cur.b, col);
-      if (page >= 0 && p != 0.f) {
-        const float w = p * (a.pool.vs[page * a.pool.vs_sp + cur.kvh * a.pool.vs_sh + prow * a.pool.vs_ss] * in_unit);
-        const uint4* src = reinterpret_cast<const uint4*>(a.pool.v + page * a.pool.v_sp + cur.kvh * a.pool.v_sh + prow * a.pool.v_ss + c0);
+      const float w = p == 0.f ? 0.f : p * factor[c];    // (a hidden row's factor may be an infinity)
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const uint4 b = __ldg(src + q);
-          const uint32_t b4[4] = {b.x, b.y, b.z, b.w};
+      for (int q = 0; q < 4; ++q) {
+        const uint4 b = *reinterpret_cast<const uint4*>(blk + sw128(static_cast<uint32_t>(c), static_cast<uint32_t>(((c0 & 63) >> 3) + q)));
+        const uint32_t b4[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            ov[q * 16 + e] = __float_as_uint(fmaf(w, byte_value<ST>(static_cast<uint8_t>(b4[e >> 2] >> (8 * (e & 3)))), __uint_as_float(ov[q * 16 + e])));
+        for (int e = 0; e < 4; ++e) {
+          const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&b4[e]));
+          o[q * 8 + 2 * e] = fmaf(w, y.x, o[q * 8 + 2 * e]);
+          o[q * 8 + 2 * e + 1] = fmaf(w, y.y, o[q * 8 + 2 * e + 1]);
         }
       }
-      __syncwarp();
     }
+    uint32_t ov[32];
+#pragma unroll
+    for (int k = 0; k < 32; ++k) ov[k] = __float_as_uint(o[k]);
     tmem_st32(o_addr + c0, ov);
   }
   tmem_wait_st();
@@ -825,8 +835,8 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
     float m_used = -INFINITY, l = 0.f;
     int unit_exp = kNoExp;
     // One tile of this row: scores to weights against the lazy running max.
-    auto tile = [&](auto mask_tag, int j0, bool fresh) -> bool {
-      constexpr bool kMask = decltype(mask_tag)::value;
+    auto tile = [&](auto mask_tag, auto far_tag, int j0, bool fresh) -> bool {
+      constexpr bool kMask = decltype(mask_tag)::value, kHasFar = decltype(far_tag)::value;
       const uint32_t bi = (i & 1u) * MT + wg;
       [[maybe_unused]] const uint8_t* meta = smem + C::kOffMeta + vr.stage * C::kMetaBytes;
       if (kMask && C::kWide) {  // the tile's valid keys (8-bit: the caller waited for them and the scales)
@@ -914,17 +924,14 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
       }
       // Columns whose rows lie outside the unit's span: their scores are kept for add_far.
       [[maybe_unused]] uint64_t far = 0;
-      [[maybe_unused]] float far_x[kMask && !C::kWide ? kTile : 1];
-      if constexpr (kMask && !C::kWide) {
-        const uint32_t word = reinterpret_cast<const uint32_t*>(meta)[3];
-        if (word & kFar) {
-          const float* f = reinterpret_cast<const float*>(meta + 16) + kTile;
-          const bool all = word & kAllFar;
-          far = __ballot_sync(0xffffffffu, all || VUnit::outside(f[lane])) |
-                static_cast<uint64_t>(__ballot_sync(0xffffffffu, all || VUnit::outside(f[32 + lane]))) << 32;
+      [[maybe_unused]] float far_x[kHasFar ? kTile : 1];
+      if constexpr (kHasFar) {
+        const float* f = reinterpret_cast<const float*>(meta + 16) + kTile;
+        const bool all = reinterpret_cast<const uint32_t*>(meta)[3] & kAllFar;
+        far = __ballot_sync(0xffffffffu, all || VUnit::outside(f[lane])) |
+              static_cast<uint64_t>(__ballot_sync(0xffffffffu, all || VUnit::outside(f[32 + lane]))) << 32;
 #pragma unroll
-          for (int c = 0; c < kTile; ++c) far_x[c] = x[c];
-        }
+        for (int c = 0; c < kTile; ++c) far_x[c] = x[c];
       }
       const float nmb = m_used == -INFINITY ? 0.f : -m_used;
       [[maybe_unused]] const uint64_t qs2 = f2_pack(qs, qs), nmb2 = f2_pack(nmb, nmb);
@@ -956,7 +963,7 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
           f2_unpack(p1, z[2], z[3]);
           if (kMask) {  // a hidden key's weight is 0 whatever its scale
 #pragma unroll
-            for (int e = 0; e < 4; ++e) z[e] = y[e] == 0.f || ((far >> (c + e)) & 1u) ? 0.f : z[e];
+            for (int e = 0; e < 4; ++e) z[e] = y[e] == 0.f || (kHasFar && ((far >> (c + e)) & 1u)) ? 0.f : z[e];
           }
           packed[(c - c0) >> 1] = pack16x2(z[0], z[1], false);
           packed[((c - c0) >> 1) + 1] = pack16x2(z[2], z[3], false);
@@ -972,34 +979,34 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
         f2_unpack(f2_add(f2_add(acc[0], acc[1]), f2_add(acc[2], acc[3])), s0, s1);
         l += s0 + s1;
       }
-      if (__any_sync(0xffffffffu, need)) {
-        const uint32_t pv = i - 1;
-        if (!warp_wait(&bars->p_free[pv & 1u], (pv >> 1) & 1u, abort, a.wait_ns)) return false;
-        tc_fence_after();
+      if (kHasFar || __any_sync(0xffffffffu, need)) {
         const uint32_t o_addr = lane_base + kColO + wg * D;
-#pragma unroll
-        for (int ch = 0; ch < D / 32; ++ch) {
-          uint32_t ov[32];
-          tmem_ld32(o_addr + ch * 32, ov);
-          tmem_wait_ld();
-#pragma unroll
-          for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(C::kWide ? __uint_as_float(ov[c]) * alpha : __uint_as_float(ov[c]) * alpha * regrade);
-          tmem_st32(o_addr + ch * 32, ov);
+        if (!fresh) {  // (before a unit's first tile the epilogue has waited)
+          const uint32_t pv = i - 1;
+          if (!warp_wait(&bars->p_free[pv & 1u], (pv >> 1) & 1u, abort, a.wait_ns)) return false;
+          tc_fence_after();
         }
-        tmem_wait_st();
+        if constexpr (kHasFar) {
+          add_far<C>(o_addr, fresh, alpha, regrade, far, far_x, smem + C::kOffV + vr.stage * C::kTileBytes,
+                     reinterpret_cast<const float*>(meta + 16) + kTile);
+        } else {
+#pragma unroll
+          for (int ch = 0; ch < D / 32; ++ch) {
+            uint32_t ov[32];
+            tmem_ld32(o_addr + ch * 32, ov);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(C::kWide ? __uint_as_float(ov[c]) * alpha : __uint_as_float(ov[c]) * alpha * regrade);
+            tmem_st32(o_addr + ch * 32, ov);
+          }
+          tmem_wait_st();
+        }
       }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->p_full[bi]);
       vr.next();
-      if constexpr (kMask && !C::kWide) {
-        if (far) {
-          if (!warp_wait(&bars->p_free[i & 1u], (i >> 1) & 1u, abort, a.wait_ns)) return false;
-          tc_fence_after();
-          add_far<ST, D>(a, cur, j0, far, far_x, lane_base + kColO + wg * D, unit_exp);
-        }
-      }
       return true;
     };
     // Whether the warp has rows in this unit: its lanes of the products are not read otherwise.
@@ -1022,14 +1029,17 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
         // (a plain tile lacks keys only where a page is bad, which is known before its scores are)
         const uint32_t stage = vr.stage;
         const int j0 = cur.u.tile(cur.i + k) * kTile;
-        if (common.plain(a, j0) && !tile(std::false_type(), j0, k == 0)) return;
-        if (vr.stage == stage && !tile(std::true_type(), j0, k == 0)) return;
+        if (common.plain(a, j0) && !tile(std::false_type(), std::false_type(), j0, k == 0)) return;
+        if (vr.stage == stage && !tile(std::true_type(), std::false_type(), j0, k == 0)) return;
       } else {
         if (!warp_wait(&bars->v_full[vr.stage], vr.phase, abort, a.wait_ns)) return;
-        if (reinterpret_cast<const uint32_t*>(smem + C::kOffMeta + vr.stage * C::kMetaBytes)[3] == 0) {
-          if (!tile(std::false_type(), 0, k == 0)) return;
+        const uint32_t word = reinterpret_cast<const uint32_t*>(smem + C::kOffMeta + vr.stage * C::kMetaBytes)[3];
+        if (word == 0) {
+          if (!tile(std::false_type(), std::false_type(), 0, k == 0)) return;
+        } else if (!(word & kFar)) {
+          if (!tile(std::true_type(), std::false_type(), cur.u.tile(cur.i + k) * kTile, k == 0)) return;
         } else {
-          if (!tile(std::true_type(), cur.u.tile(cur.i + k) * kTile, k == 0)) return;
+          if (!tile(std::true_type(), std::true_type(), cur.u.tile(cur.i + k) * kTile, k == 0)) return;
         }
       }
     }

@@ -236,3 +236,79 @@ def test_options_larger_than_any_sequence(backend, many):
     want = G.paged_attention(q, *p.args, parents=[-1, 0, 1], backend=backend)
     got = G.paged_attention(q, *p.args, parents=[-1, 0, 1], max_depth=many, window=many, sinks=many, backend=backend)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("storage", STORES)
+def test_captured_behind_copies_and_other_streams(n, storage):
+    """Lengths and tables that a copy, or a kernel on a joined stream, writes just before a captured call: each replay sees its own."""
+    lens = [n + 300, n + 20]
+    p = Paged(lens, 2, 128, 16, torch.bfloat16, storage, seed=n)
+    q = torch.randn(2, 8, n, 128, device="cuda").bfloat16()
+    fresh_lens, seq_lens, table = p.lens_d.clone(), torch.zeros_like(p.lens_d), torch.zeros_like(p.table_d)
+    fresh_table = p.table_d.clone()
+    call = lambda: G.paged_attention(q, p.k_pages, p.v_pages, table, seq_lens, return_lse=True, **p.held)  # noqa: E731
+    cases = [p.lens_d.clone(), torch.tensor([n + 17, n + 5], dtype=torch.int32, device="cuda"), torch.tensor([0, n], dtype=torch.int32, device="cuda")]
+    want = [G.paged_attention(q, p.k_pages, p.v_pages, p.table_d, x, return_lse=True, **p.held) for x in cases]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+
+    def by_copy():
+        table.copy_(fresh_table)
+        seq_lens.copy_(fresh_lens)
+        first = call()
+        seq_lens.copy_(fresh_lens)
+        return first, call()
+
+    def by_join():
+        table.copy_(fresh_table)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.add(fresh_lens, 0, out=seq_lens)
+        torch.cuda.current_stream().wait_stream(side)
+        first = call()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            second = call()
+        torch.cuda.current_stream().wait_stream(side)
+        return first, second
+
+    for step in (by_copy, by_join):
+        fresh_lens.copy_(cases[0])
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step()
+        for x, w in list(zip(cases, want)) * 3:
+            fresh_lens.copy_(x)
+            seq_lens.zero_()
+            table.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            for got in outs:
+                assert all(torch.equal(a, b) for a, b in zip(got, w))
+        del graph
+
+
+def test_calls_of_several_host_threads():
+    """Attention of both tensor-core kernels, each thread on its own stream."""
+    errors = []
+
+    def work(n, storage):
+        try:
+            st = torch.cuda.Stream()
+            with torch.cuda.stream(st):
+                p = Paged([n + 200, n + 900], 2, 128, 16, torch.bfloat16, storage, seed=n)
+                q = torch.randn(2, 8, n, 128, device="cuda").bfloat16()
+                want = G.paged_attention(q, *p.args, **p.held)
+                for _ in range(50):
+                    assert torch.equal(G.paged_attention(q, *p.args, **p.held), want)
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=a) for a in ((1, "native"), (2, "int8"), (70, "native"), (64, "fp8"))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors

@@ -181,3 +181,24 @@ def test_queries_with_one_large_channel(backend, storage, n):
         want, weight, slip, wl = attend(small, p.k64[b], p.v64[b], visible(p.lens[b], n), 128 ** -0.5)
         assert bool(((out[b].cpu().double() - want).abs() <= tolerance(want, weight, slip, torch.bfloat16)).all())
         assert bool(((lse[b].cpu().double() - wl).abs() <= 2 * slip[..., 0] + 64 * 2.0 ** -22 + wl.abs() * 2.0 ** -22).all())
+
+
+@pytest.mark.parametrize("backend", KERNELS)
+@pytest.mark.parametrize("storage", EIGHT)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("ps,Hq,new", [(12, 10, [1, 40, 0, 3]), (64, 2, [130, 1, 7, 1]), (16, 14, [5, 5, 60, 1])])
+def test_narrow_heads_and_ragged_batches(backend, storage, dtype, ps, Hq, new):
+    """head_dim 64, packed rows, a window: rows of three sizes in turn; and the same bits from call to call."""
+    before = [200, 77, 9, 500]
+    lens = [c + before[b] if c else 0 for b, c in enumerate(new)]
+
+    def scale_of(b, name):
+        i = torch.arange(lens[b]).view(-1, 1, 1)
+        return torch.exp2((i % 7 == 3) * 13.0 - (i % 11 == 5) * 12.0) if name == "v" else 1.0
+    p = Paged(lens, 2, 64, ps, dtype, storage, seed=ps, scale_of=scale_of)
+    check(p, new, Hq, packed=True, window=60, sinks=3, backend=backend)
+    check(p, new, Hq, packed=True, backend=backend)
+    cu = torch.tensor([sum(new[:b]) for b in range(len(new) + 1)], dtype=torch.int32, device="cuda")
+    q = torch.randn(sum(new), Hq, 64, device="cuda").to(dtype)
+    first = G.paged_attention(q, *p.args, cu_q=cu, max_q=max(new), backend=backend, **p.held)
+    assert all(torch.equal(first, G.paged_attention(q, *p.args, cu_q=cu, max_q=max(new), backend=backend, **p.held)) for _ in range(3))
