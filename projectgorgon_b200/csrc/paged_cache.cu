@@ -525,15 +525,16 @@ __global__ void __launch_bounds__(kTrimWarps * 32) paged_trim_warp_kernel(const 
 }
 
 // Any row size: a CTA per (layer, sequence, head) and K or V, through shared memory,
-// `width` bytes of every row at a time (a column of the rows depends on that
-// column alone, so rows may overlap all the same).  The stage is one that every
-// launch may have: a larger limit is an attribute of the kernel, which two host
-// threads would set for each other.
+// as many bytes of every row at a time as the stage holds (a column of the rows
+// depends on that column alone, so rows may overlap all the same).  The stage is one that every launch may have: a larger limit
+// is an attribute of the kernel, which two host threads would set for each other.
 constexpr int kTrimThreads = 128;
-constexpr int kTrimStage = 46 * 1024;
-__global__ void __launch_bounds__(kTrimThreads) paged_trim_kernel(const TrimArgs a, int width) {
+constexpr int kTrimRows = 256;
+constexpr int kTrimStage = 44 * 1024;
+__global__ void __launch_bounds__(kTrimThreads) paged_trim_kernel(const TrimArgs a, int stage_bytes) {
   extern __shared__ uint8_t stage[];
-  __shared__ float s_scale[256];
+  __shared__ int64_t s_row[kTrimRows];  // byte offsets of the rows read, then of those written
+  __shared__ float s_scale[kTrimRows];
   __shared__ int s_ok;
   const int h = blockIdx.x, b = blockIdx.y;
   const int layer = blockIdx.z >> 1, kv = blockIdx.z & 1;
@@ -562,29 +563,45 @@ __global__ void __launch_bounds__(kTrimThreads) paged_trim_kernel(const TrimArgs
     page = tb[col];
   };
   int page, row;
-  if (scaled)
+  auto look_up = [&](auto pos, bool scales) {
     for (int r = threadIdx.x; r < len; r += kTrimThreads) {
-      at(a.idx[b * a.idx_sb + r], page, row);
-      s_scale[r] = sbase[page * ssp + row * sss];
-    }
-  for (int c0 = 0; c0 < a.row_bytes; c0 += width) {
-    const int w = min(width, a.row_bytes - c0);
-    for (int e = threadIdx.x; e < len * w; e += kTrimThreads) {
-      const int r = e / w, c = c0 + e - r * w;
-      at(a.idx[b * a.idx_sb + r], page, row);
-      stage[e] = static_cast<uint8_t>(base[page * sp + row * ss + c]);
+      at(pos(r), page, row);
+      s_row[r] = page * sp + row * ss;
+      if (scales) s_scale[r] = sbase[page * ssp + row * sss];
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < len * w; e += kTrimThreads) {
-      const int r = e / w, c = c0 + e - r * w;
-      at(d0 + r, page, row);
-      base[page * sp + row * ss + c] = static_cast<char>(stage[e]);
-    }
+  };
+  auto source = [&](int r) { return a.idx[b * a.idx_sb + r]; };
+  auto target = [&](int r) { return d0 + r; };
+  const int width = min(a.row_bytes, stage_bytes / len);
+  for (int c0 = 0; c0 < a.row_bytes; c0 += width) {
+    const int w = min(width, a.row_bytes - c0);
+    // (four loads before their stores: the compiler keeps loads of offsets behind stores of bytes)
+    auto move = [&](auto load, auto store) {
+      for (int e0 = threadIdx.x; e0 < len * w; e0 += kTrimThreads * 4) {
+        uint8_t x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int e = e0 + k * kTrimThreads, r = e / w;
+          if (e < len * w) x[k] = load(e, r, c0 + e - r * w);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int e = e0 + k * kTrimThreads, r = e / w;
+          if (e < len * w) store(e, r, c0 + e - r * w, x[k]);
+        }
+      }
+    };
+    look_up(source, scaled && c0 == 0);
+    move([&](int, int r, int c) { return static_cast<uint8_t>(base[s_row[r] + c]); }, [&](int e, int, int, uint8_t x) { stage[e] = x; });
+    __syncthreads();
+    look_up(target, false);
+    move([&](int e, int, int) { return stage[e]; }, [&](int, int r, int c, uint8_t x) { base[s_row[r] + c] = static_cast<char>(x); });
     __syncthreads();
   }
   if (scaled)
     for (int r = threadIdx.x; r < len; r += kTrimThreads) {
-      at(d0 + r, page, row);
+      at(target(r), page, row);
       sbase[page * ssp + row * sss] = s_scale[r];
     }
 }
@@ -747,7 +764,7 @@ extern "C" int gorgon_paged_trim(const gorgon_paged_trim_params* p, void* stream
   int rc = make_pool(&p->kv, "gorgon_paged_trim", &a.pool);
   if (rc) return rc;
   if (p->layers < 0 || p->max_len < 0) return set_error(GORGON_ERR_INVALID, "gorgon_paged_trim: negative size");
-  if (p->max_len > 256) return set_error(GORGON_ERR_UNSUPPORTED, "gorgon_paged_trim: max_len > 256");
+  if (p->max_len > kTrimRows) return set_error(GORGON_ERR_UNSUPPORTED, "gorgon_paged_trim: max_len > 256");
   if (p->layers > 32767) return set_error(GORGON_ERR_UNSUPPORTED, "gorgon_paged_trim: layers > 32767");
   if (p->layers == 0 || a.pool.batch == 0 || a.pool.d == 0 || p->max_len == 0) return GORGON_OK;
   if (!p->src_idx || !p->lens || !a.pool.table) return set_error(GORGON_ERR_INVALID, "gorgon_paged_trim: null pointer");
@@ -785,10 +802,10 @@ extern "C" int gorgon_paged_trim(const gorgon_paged_trim_params* p, void* stream
     else paged_trim_warp_kernel<8><<<grid, kTrimWarps * 32, 0, st>>>(a);
     return check_cuda(cudaGetLastError(), "gorgon_paged_trim launch");
   }
-  const int width = static_cast<int>(std::min<int64_t>(a.row_bytes, kTrimStage / p->max_len));  // (at most 256 rows)
-  const size_t smem = static_cast<size_t>(p->max_len) * width;
+  static_assert(kTrimStage / kTrimRows > 0 && kTrimStage + kTrimRows * 12 + 64 <= 48 * 1024, "a stage for every launch");
+  const int smem = static_cast<int>(std::min<int64_t>(p->max_len * a.row_bytes, kTrimStage));
   const dim3 grid(static_cast<unsigned>(a.pool.hkv), static_cast<unsigned>(a.pool.batch),
                   2u * static_cast<unsigned>(p->layers));
-  paged_trim_kernel<<<grid, kTrimThreads, smem, st>>>(a, width);
+  paged_trim_kernel<<<grid, kTrimThreads, static_cast<size_t>(smem), st>>>(a, smem);
   return check_cuda(cudaGetLastError(), "gorgon_paged_trim launch");
 }
