@@ -542,8 +542,8 @@ typedef struct {
 typedef enum {
   GORGON_PAGED_AUTO = 0,
   GORGON_PAGED_SIMT = 1, /* CUDA cores: any dtype, head_dim and alignment */
-  GORGON_PAGED_MMA = 2,  /* tensor cores, warp by warp, for few new rows: 16-bit dtype, head_dim
-                            64 or 128, rows of whole 16-byte pieces */
+  GORGON_PAGED_MMA = 2,  /* tensor cores, warp by warp, for few new rows and trees of more than 256:
+                            16-bit dtype, head_dim 64 or 128, rows of whole 16-byte pieces */
   GORGON_PAGED_TCGEN05 = 3 /* tcgen05, for many new rows; the same, and trees of at most 256 rows */
 } gorgon_paged_backend;
 

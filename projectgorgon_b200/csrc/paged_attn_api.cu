@@ -80,8 +80,9 @@ Kernel choose(const gorgon_paged_attn_params* p, const PagedAttn& a) {
       // The warp-level kernel passes the cache once for every 16 packed rows, the
       // tcgen05 kernel once for 256, at a higher price a pass where rows are widened.
       // 16 sequences of 8192 rows, us, warp-level / tcgen05: 16-bit 104 / 125 for 16
-      // packed rows, 183 / 126 for 32; int8 92 / 201 for 16, 158 / 203 for 32, 235 / 204
-      // for 48.
+      // packed rows, 183 / 126 for 32; int8 93 / 215 for 16, 164 / 216 for 32, 243 / 217
+      // for 48.  One sequence turns later (4096 rows: 16-bit 20 / 27 for 20, 33 / 27 for
+      // 96; int8 25 / 31 for 48, 32 / 31 for 96).
       if (static_cast<int64_t>(a.n) * a.group > (p->kv.storage == GORGON_KV_NATIVE ? 16 : 32) && tc) return Kernel::kTc;
       return mma ? Kernel::kMma : Kernel::kSimt;
   }

@@ -31,11 +31,12 @@
 // the search replaces them by zeros, and the epilogue adds them to the rows
 // that do see them.
 //
-// Measured: 2048 new tokens over 32768 bf16 rows (32 heads on 8, 128 wide) 967 us
-// (to 1026 us, by the card's power), 1.10 PFLOP/s, the tensor pipe busy 75 % and the exponentials' 61 % of the time;
-// 64-node trees of 16 sequences over 8192 e4m3 rows 267 us, bound by shared
-// memory (operands, widening and scales); bf16 pages of 16 rows cost 5 % over
-// pages of 64.
+// Measured: 2048 new tokens over 32768 bf16 rows (32 heads on 8, 128 wide) 930 to
+// 1026 us by the card's power, 1.04 to 1.14 PFLOP/s, the tensor pipe busy 75 % and
+// the exponentials' 61 % of the time; 64-node trees of 16 sequences over 8192 e4m3
+// rows 280 us with nothing saturated (shared memory 67 %, issue slots 42 %, tensor
+// pipe 33 %): the producers' chain of wait, widening and hand-over; bf16 pages of 16
+// rows cost 5 % over pages of 64.
 
 // Every mbarrier wait is bounded; a wait that runs out raises kErrTimeout, and
 // the CTA drains its copies and products, frees TMEM and returns.

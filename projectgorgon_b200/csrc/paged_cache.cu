@@ -627,8 +627,8 @@ inline bool pow2_upto32(int x) { return x >= 1 && x <= 32 && (x & (x - 1)) == 0;
 // once the pairs alone would fill the SMs (2048 threads each) twice over, where
 // the lookups' latency counts for every wave (a read of 16 sequences of up to
 // 8192 int8 rows: 75 us a head each, 66 us with four, 5.9 TB/s; an append of 8000
-// rows to e4m3: 18.1 us with four, 17.0 us with two, 2.9 TB/s, bound by the
-// conversions); one head each below, where all run at once (64 single rows:
+// rows to e4m3: 18.1 us with four, 17.0 us with two, 2.9 TB/s, the issue slots 67 %
+// busy); one head each below, where all run at once (64 single rows:
 // 3.4 us either way, a launch).
 int64_t groups(int64_t items, int hkv, int lpr, int heads) {
   if (items * lpr < int64_t(2) * 2048 * sm_count()) return items;

@@ -137,7 +137,8 @@ def paged_cache_trim(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: 
     ``r < lens[b]``, in every layer and head, as stored (bytes and scales).
     ``GorgonKVCache.trim``'s arguments, over ``[layers, pages, Hkv, page_size, D]``
     (or one layer's ``[pages, Hkv, page_size, D]``); ``dst_start`` ``[B]``, an int, or
-    None for 0.  At most 256 rows per sequence.  A bad index sets the device
+    None for 0.  At most 256 columns; few are faster, whatever ``lens`` (of a
+    verifier's path pass the first ``max_depth + 1``).  A bad index sets the device
     error bits and leaves its sequence as it is.  A call must not name a sequence
     twice, nor move rows into pages that another of its sequences reads; pages
     expanded over layers or kv heads (strides of 0) are refused."""

@@ -53,7 +53,8 @@ def paged_attention(
     q            ``[B, Hq, n, D]``, ``n`` new rows per sequence, or with ``cu_q``
                  (int ``[B + 1]``) packed ``[total, Hq, D]``: sequence ``b``'s are
                  rows ``cu_q[b] .. cu_q[b + 1] - 1``, at most ``max_q`` of them
-                 (default: ``total``; a tight bound makes a better schedule)
+                 (default: ``total``, for which single tokens run on the
+                 kernel for chunks: give the bound)
     k_pages, v_pages  ``[pages, Hkv, page_size, D]`` of q's dtype, or int8 /
                  float8_e4m3fn with ``k_scale``, ``v_scale`` float32
                  ``[pages, Hkv, page_size]``; any strides, ``D`` contiguous.  The
@@ -78,7 +79,11 @@ def paged_attention(
     Returns ``out`` shaped like ``q``, and with ``return_lse`` also the
     natural-log sum of exponentials, float32 ``[B, Hq, n]`` (packed:
     ``[total, Hq]``).  Packed rows from ``cu_q[B]`` on are not written: a given
-    ``out`` keeps them.  All lengths stay on the device, so a call can be captured
+    ``out`` keeps them.  16-bit rows of head_dim 64 or 128 in whole 16-byte pieces,
+    and 8-bit pages of such, run on the tensor cores; trees of more than 256 nodes
+    there pass the cache once per 16 (row, head) pairs.  Everything else, and calls
+    whose table's columns times rows of ``max_q`` pass 2^31 units of work, runs on
+    the CUDA cores, far slower.  All lengths stay on the device, so a call can be captured
     in a CUDA graph and replayed with other lengths (within the block table).
     """
     dev = device_index("q, pages, block_table and seq_lens", q, k_pages, v_pages, block_table, seq_lens, k_scale,
