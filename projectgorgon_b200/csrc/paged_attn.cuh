@@ -19,6 +19,8 @@
 // order of the CTAs, so results do not depend on timing.
 #pragma once
 
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace gorgon {
@@ -318,6 +320,13 @@ __device__ __forceinline__ int tree_bits(const PagedAttn& a, const Seq& s, int b
   }
   return hop;
 }
+
+// f16 weights over 16-bit pages are taken against the running max less 7 (log2
+// units): at most 2^15, as far up in f16 as they go, so that weights keep their bits
+// down to 2^-21 of the largest and count down to 2^-32.  (A first key may take
+// nearly all weight and hold next to nothing.)  bf16 has the range.
+template <typename X, bool kWide>
+__host__ __device__ constexpr float headroom() { return kWide && std::is_same_v<X, __half> ? 7.f : 0.f; }
 
 // The unit of 8-bit rows' weights.  A weight (at most 2^8) times its V scale
 // enters the products as f16, in units of 2^(e - kUnit), where its scale lies in

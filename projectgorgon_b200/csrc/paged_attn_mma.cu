@@ -175,6 +175,7 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
   constexpr int KB = C::KB, G = C::G;
   constexpr uint32_t kAll = G == 32 ? 0xffffffffu : (1u << (G & 31)) - 1u;
   constexpr bool kScaleQ = !C::kWide && std::is_same_v<T, __nv_bfloat16>;
+  constexpr float kHead = headroom<X, C::kWide>();
   extern __shared__ __align__(128) uint8_t smem[];
   static_assert(sizeof(ShareScratch) <= kRedFloats * 4, "scratch");
   ShareScratch* sh = reinterpret_cast<ShareScratch*>(smem + C::kOffRed);
@@ -516,19 +517,20 @@ __global__ void __launch_bounds__(Cfg<T, ST, D, NT>::kThreads, kCtasPerSm) paged
           for (int e = 0; e < 2; ++e) {
             float top = fmaxf(x[0][nt][e], x[0][nt][e + 2]);
             if constexpr (KB == 2) top = fmaxf(top, fmaxf(x[KB - 1][nt][e], x[KB - 1][nt][e + 2]));
-            move |= top > m[nt][e] + 8.f;
+            move |= top > m[nt][e] + (8.f + kHead);
           }
         // The running max moves only when a score exceeds it by 8 (log2 units), so
-        // the usual group needs no shuffles and no rescaling.
+        // the usual group needs no shuffles and no rescaling.  (m is the max less kHead.)
         if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float alpha[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float top = m[nt][e];
+              float top = -INFINITY;
 #pragma unroll
               for (int b = 0; b < KB; ++b) top = fmaxf(top, fmaxf(x[b][nt][e], x[b][nt][e + 2]));
+              top = fmaxf(top - kHead, m[nt][e]);
 #pragma unroll
               for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
               alpha[e] = ex2(m[nt][e] - (top == -INFINITY ? 0.f : top));

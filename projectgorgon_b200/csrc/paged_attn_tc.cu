@@ -711,6 +711,7 @@ template <typename T, int ST, typename C>
 __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, uint8_t* smem, TcBars<C>* bars, uint32_t tmem) {
   using X = typename C::X;
   constexpr bool kScaleQ = !C::kWide && std::is_same_v<T, __nv_bfloat16>;
+  constexpr float kHead = headroom<X, C::kWide>();
   constexpr int MT = C::MT, D = C::D;
   constexpr int kChunks = D / 8;          // 16-byte pieces of a 16-bit row
   constexpr int kRows = 32 / kChunks;     // rows that a warp instruction covers
@@ -890,7 +891,7 @@ __device__ void softmax(const PagedAttn& a, const TileCursor& start, int end, ui
       [[maybe_unused]] float regrade = 1.f;
       bool need = false;
       if constexpr (C::kWide) {
-        const float tmax = top * qs;
+        const float tmax = top * qs - kHead;
         if (fresh) {
           m_used = tmax;
         } else if (tmax > m_used + 8.f) {

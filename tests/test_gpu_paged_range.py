@@ -202,3 +202,37 @@ def test_narrow_heads_and_ragged_batches(backend, storage, dtype, ps, Hq, new):
     q = torch.randn(sum(new), Hq, 64, device="cuda").to(dtype)
     first = G.paged_attention(q, *p.args, cu_q=cu, max_q=max(new), backend=backend, **p.held)
     assert all(torch.equal(first, G.paged_attention(q, *p.args, cu_q=cu, max_q=max(new), backend=backend, **p.held)) for _ in range(3))
+
+
+@pytest.mark.parametrize("backend", KERNELS)
+@pytest.mark.parametrize("storage", ["native", "int8", "fp8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("gap", [8.0, 14.0, 17.0])
+def test_a_sink_that_holds_nothing(backend, storage, dtype, n, gap):
+    """The first key takes nearly all weight and its V row is zeros: what the others weigh, e^-gap and less of it, is the output."""
+    L, D, Hq = n + 600, 128, 8
+    p = sized([L], lambda _: [0], storage, dtype, 0.0)
+    q = torch.randn(1, Hq, n, D, generator=torch.Generator().manual_seed(4)).to(dtype)
+    q[..., 0] = 16.0
+    pg = int(p.table[0, 0])
+    row = torch.zeros(2, D)
+    row[:, 0] = 8.0  # as stored, and as a value: a score of `gap` with the scale below, 0 from the other columns
+    if storage == "fp8":
+        p.k_pages.view(torch.uint8)[pg, :, 0] = row.to(torch.float8_e4m3fn).view(torch.uint8).cuda()
+    else:
+        p.k_pages[pg, :, 0] = row.to(p.k_pages.dtype).cuda()
+    if storage != "native":
+        p.k_scale[pg, :, 0] = 1.0
+    p.k64[0][0] = row.double()
+    # the others' scores: about 0, of a standard deviation of at most 1.5
+    p.k_pages.view(torch.uint8 if storage != "native" else dtype)[:, :, :, 0] = 0
+    p.k_pages.view(torch.uint8 if storage != "native" else dtype)[pg, :, 0, 0] = \
+        row[0, 0].to(torch.float8_e4m3fn).view(torch.uint8).item() if storage == "fp8" else 8
+    p.k64[0][1:, :, 0] = 0
+    scale = gap / 128.0
+    out = G.paged_attention(q.cuda(), *p.args, backend=backend, scale=scale, **p.held)
+    want, weight, slip, _ = attend(q[0], p.k64[0], p.v64[0], visible(L, n), scale)
+    tol = tolerance(want, weight, slip, dtype)
+    off = (out[0].cpu().double() - want).abs()
+    assert bool((off <= tol).all()), float((off / tol).max())
